@@ -128,6 +128,40 @@ EXPORTED = (
     "ssla_engine_rings_attach", "ssla_engine_drain_rings", "ssla_engine_serve_rings",
     "ssla_replay_start", "ssla_replay_stop", "ssla_replay_join",
 )
+
+class SslaLinAttn(C.Structure):
+    """include/ssla_ops.h SslaLinAttn."""
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "out", "decay", "state")] +
+                [(n, C.c_longlong) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head",
+                                             "out_row", "out_head", "decay_row", "decay_head")] +
+                [(n, C.c_int) for n in ("n_rows", "heads", "q_heads", "k_heads", "dk", "dv", "dtype", "n_slots",
+                                        "device")] + [("scale", C.c_float)])
+
+
+class SslaStateCache(C.Structure):
+    """include/ssla_ops.h SslaStateCache."""
+    _fields_ = ([(n, C.c_void_p) for n in ("codes", "scales", "slots")] +
+                [(n, C.c_longlong) for n in ("x_state", "x_row")] +
+                [(n, C.c_int) for n in ("n", "n_slots", "rows", "cols", "block", "format", "dtype", "device")])
+
+
+class SslaGroupNorm(C.Structure):
+    """include/ssla_ops.h SslaGroupNorm."""
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "y", "weight", "bias")] +
+                [(n, C.c_longlong) for n in ("x_sample", "x_pos", "y_sample", "y_pos")] +
+                [(n, C.c_int) for n in ("n", "positions", "channels", "groups", "dtype", "activation", "device")] +
+                [("eps", C.c_float)])
+
+
+# Every symbol include/ssla_ops.h declares.
+OPS_EXPORTED = (
+    "ssla_linattn_chunk", "ssla_linattn_chunk_workspace", "ssla_linattn_step",
+    "ssla_state_store", "ssla_state_load", "ssla_group_norm", "ssla_group_norm_workspace",
+)
+DT_F32, DT_BF16, DT_F16 = range(3)
+FMT_INT8, FMT_E4M3 = range(2)
+ACT_NONE, ACT_SILU = range(2)
+LINATTN_MAX_DK, LINATTN_MAX_DV = 128, 256
 # SSLA_STRIP_ERR_* bits
 STRIP_ERR_CAPACITY, STRIP_ERR_TIMEOUT, STRIP_ERR_MISMATCH = 1, 2, 4
 # Every symbol include/stage01_to_gpu.h declares (the libstage01_to_gpu ABI).

@@ -1,0 +1,106 @@
+// ssla_ops.cuh -- what the recurrent-state operators (include/ssla_ops.h)
+// share: element types, error returns of their C entries, launches.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+#include <string>
+
+#include "ssla_b200.h"
+#include "ssla_ops.h"
+
+namespace ssla {
+
+void set_last_error(const std::string& msg);   // ssla_engine.cu
+
+namespace ops {
+
+// Sets the calling thread's error text; never throws.
+inline int fail(int code, const char* fmt, ...) noexcept {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    std::vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    try {
+        set_last_error(buf);
+    } catch (...) {
+    }
+    return code;
+}
+
+// Makes `dev` current for the scope; `err` is SSLA_OK or the code to return.
+struct OnDevice {
+    int prev = -1, err = SSLA_OK;
+    explicit OnDevice(int dev) noexcept {
+        int n = 0;
+        if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+            cudaGetLastError();
+            err = fail(SSLA_ERR_NO_DEVICE, "no CUDA device");
+            return;
+        }
+        if (dev < 0 || dev >= n) {
+            err = fail(SSLA_ERR_ARG, "device %d of %d", dev, n);
+            return;
+        }
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+        if (prev == dev) {
+            prev = -1;
+        } else if (cudaError_t e = cudaSetDevice(dev); e != cudaSuccess) {
+            err = fail(SSLA_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(e));
+        }
+    }
+    ~OnDevice() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
+inline int launched(const char* what) noexcept {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? SSLA_OK : fail(SSLA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+inline bool dtype_ok(int dt) { return dt == SSLA_DT_F32 || dt == SSLA_DT_BF16 || dt == SSLA_DT_F16; }
+inline int dtype_size(int dt) { return dt == SSLA_DT_F32 ? 4 : 2; }
+inline bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// Whether byte ranges [a, a + na) and [b, b + nb) meet.
+inline bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return na && nb && x < y + nb && y < x + na;
+}
+
+template <typename T> __device__ __forceinline__ float to_f(T x);
+template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
+
+template <typename T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+
+// V consecutive values at p (aligned to V * sizeof(T)) as floats, and back.
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const T* p, float (&x)[V]) {
+    const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = to_f<T>(k.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[V]) {
+    Pack<T, V> k;
+#pragma unroll
+    for (int i = 0; i < V; ++i) k.v[i] = from_f<T>(x[i]);
+    *reinterpret_cast<Pack<T, V>*>(p) = k;
+}
+
+}  // namespace ops
+}  // namespace ssla

@@ -79,6 +79,13 @@ def load_library() -> C.CDLL:
         "ssla_s2s3_drain_n_multi": (i, [C.POINTER(abi.HybridS2S3Config), vp, vp, vp, vp, vp]),
         "ssla_s2s3_drain_n": (i, [C.POINTER(abi.HybridS2S3Config), vp, vp, i, i, vp, vp, vp, vp, vp]),
         "ssla_s2s3_gate_codes_noalloc": (i, [C.POINTER(abi.HybridS2S3Config), vp, vp, vp, vp]),
+        "ssla_linattn_chunk": (i, [C.POINTER(abi.SslaLinAttn), vp, vp, vp, i, vp, C.c_size_t, vp]),
+        "ssla_linattn_chunk_workspace": (i, [C.POINTER(abi.SslaLinAttn), vp, vp, i, C.POINTER(C.c_size_t)]),
+        "ssla_linattn_step": (i, [C.POINTER(abi.SslaLinAttn), vp, vp]),
+        "ssla_state_store": (i, [C.POINTER(abi.SslaStateCache), vp, vp]),
+        "ssla_state_load": (i, [C.POINTER(abi.SslaStateCache), vp, vp]),
+        "ssla_group_norm": (i, [C.POINTER(abi.SslaGroupNorm), vp, C.c_size_t, vp]),
+        "ssla_group_norm_workspace": (i, [C.POINTER(abi.SslaGroupNorm), C.POINTER(C.c_size_t)]),
         "ssla_engine_set_profiling": (i, [vp, i]),
         "ssla_engine_phase_times": (i, [vp, vp, i, C.POINTER(C.c_int)]),
         "ssla_measure_fp32_peak": (i, [i, C.POINTER(C.c_double)]),
