@@ -9,37 +9,20 @@
 #include <new>
 #include <vector>
 
-#include "ssla_ops.cuh"
+#include "ssla_linattn.cuh"
 
 namespace ssla {
 namespace ops {
 namespace {
 
 // ---------------------------------------------------------------------------
-// The recurrence, token by token: one CTA holds a head's state columns
-// [c0, c0 + 32) in registers and walks the tokens of one sequence (chunked
-// entry) or the rows that name one slot (step entry).
+// One token per row: a CTA holds a head's state columns [c0, c0 + 32) in
+// registers and applies the rows that name its slot.
 //
 // Thread (tx, rg): columns c0 + tx * VEC .. + VEC, state rows rg + i * RG.
 // ---------------------------------------------------------------------------
 constexpr int kStepThreads = 128;
 constexpr int kStepCols = 32;
-constexpr int kSeqTable = 256;      // sequences of one launch
-
-struct SeqTable {
-    int start[kSeqTable], len[kSeqTable], slot[kSeqTable];
-};
-
-struct LinArgs {
-    const void *q, *k, *v;
-    void* out;
-    const float* decay;
-    float* state;
-    long long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head, decay_row, decay_head;
-    int n_rows, heads, q_share, k_share, dk, dv, n_slots;
-    float scale;
-};
-
 template <typename T, int VEC, int RPT>
 struct StepTile {
     static constexpr int TX = kStepCols / VEC, RG = kStepThreads / TX;
@@ -55,12 +38,6 @@ struct StepTile {
     }
     __device__ float* at(const LinArgs& a, int slot, int h) const {
         return a.state + (static_cast<size_t>(slot) * a.heads + h) * a.dk * a.dv + c0;
-    }
-    __device__ void clear() {
-#pragma unroll
-        for (int i = 0; i < RPT; ++i)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) s[i][j] = 0.0f;
     }
     __device__ void load(const LinArgs& a, int slot, int h) {
         const float* p = at(a, slot, h);
@@ -157,20 +134,6 @@ __global__ void __launch_bounds__(kStepThreads) k_linattn_step(LinArgs a, const 
     t.store(a, slot, h);
 }
 
-template <typename T, int VEC, int RPT>
-__global__ void __launch_bounds__(kStepThreads)
-k_linattn_walk(LinArgs a, const __grid_constant__ SeqTable seqs) {
-    __shared__ float red[kStepThreads / 32 * kStepCols];
-    StepTile<T, VEC, RPT> t;
-    t.place(a);
-    const int h = blockIdx.y, i = blockIdx.z, slot = seqs.slot[i], n = seqs.len[i];
-    if (n == 0) return;
-    t.clear();
-    if (slot >= 0) t.load(a, slot, h);
-    for (int r = seqs.start[i]; r < seqs.start[i] + n; ++r) t.token(a, r, h, red);
-    if (slot >= 0) t.store(a, slot, h);
-}
-
 // ---- host ----------------------------------------------------------------
 
 template <typename F> int with_tile(int dtype, bool vec4, int dk, F&& f) {
@@ -206,6 +169,7 @@ Span span_of(const void* p, long long row, long long head, int n_rows, int heads
 int check_args(const SslaLinAttn* a, const char* who, bool need_state) {
     if (!a) return fail(SSLA_ERR_ARG, "%s: null argument", who);
     if (!dtype_ok(a->dtype)) return fail(SSLA_ERR_ARG, "%s: dtype %d is not an SSLA_DT_* value", who, a->dtype);
+    if (a->n_rows > INT_MAX - 65536) return fail(SSLA_ERR_ARG, "%s: %d rows, at most 2^31 - 2^16", who, a->n_rows);
     if (a->n_rows < 0 || a->n_slots < 0) return fail(SSLA_ERR_ARG, "%s: negative n_rows or n_slots", who);
     if (a->heads < 1 || a->heads > 65535 || a->q_heads < 1 || a->k_heads < 1 || a->heads % a->q_heads ||
         a->heads % a->k_heads)
@@ -257,10 +221,6 @@ LinArgs device_args(const SslaLinAttn* a) {
 }
 
 bool state_vec4(const SslaLinAttn* a) { return a->dv % 4 == 0 && aligned(a->state, 16); }
-
-struct Seq {
-    int start, len, slot;
-};
 
 // The sequences of a chunked call, checked against each other and the rows.
 int check_seqs(const SslaLinAttn* a, const int* offsets, const int* lengths, const int* slots, int n_seq,
@@ -332,43 +292,33 @@ int ssla_linattn_chunk_workspace(const SslaLinAttn* a, const int* offsets, const
                                  size_t* bytes) {
     if (!bytes) return fail(SSLA_ERR_ARG, "linear attention: null argument");
     if (const int rc = check_args(a, "linear attention", false); rc != SSLA_OK) return rc;
-    if (n_seq < 0 || (n_seq > 0 && !offsets)) return fail(SSLA_ERR_ARG, "linear attention: no offsets");
-    (void)lengths;
-    *bytes = 0;
-    return SSLA_OK;
+    try {
+        std::vector<Seq> seqs;
+        if (const int rc = check_seqs(a, offsets, lengths, nullptr, n_seq, seqs); rc != SSLA_OK) return rc;
+        *bytes = a->n_rows ? chunk_workspace(device_args(a), a->dtype, seqs) : 0;
+        return SSLA_OK;
+    } catch (const std::exception&) {
+        return fail(SSLA_ERR_CUDA, "linear attention: host allocation failed");
+    }
 }
 
 int ssla_linattn_chunk(const SslaLinAttn* a, const int* offsets, const int* lengths, const int* slots, int n_seq,
                        void* workspace, size_t workspace_bytes, void* stream) {
-    if (const int rc = check_args(a, "linear attention", false); rc != SSLA_OK) return rc;
-    (void)workspace;
-    (void)workspace_bytes;
+    const char* who = "linear attention";
+    if (const int rc = check_args(a, who, false); rc != SSLA_OK) return rc;
     try {
         std::vector<Seq> seqs;
         if (const int rc = check_seqs(a, offsets, lengths, slots, n_seq, seqs); rc != SSLA_OK) return rc;
         if (a->n_rows == 0 || seqs.empty()) return SSLA_OK;
+        const LinArgs d = device_args(a);
+        const size_t need = chunk_workspace(d, a->dtype, seqs);
+        if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+            return fail(SSLA_ERR_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who, workspace_bytes, need);
         OnDevice dev(a->device);
         if (dev.err != SSLA_OK) return dev.err;
-        const LinArgs d = device_args(a);
-        for (size_t i0 = 0; i0 < seqs.size(); i0 += kSeqTable) {
-            SeqTable tab;
-            const int n = static_cast<int>(std::min<size_t>(kSeqTable, seqs.size() - i0));
-            for (int i = 0; i < n; ++i) {
-                tab.start[i] = seqs[i0 + i].start;
-                tab.len[i] = seqs[i0 + i].len;
-                tab.slot[i] = seqs[i0 + i].slot;
-            }
-            const int rc = with_tile(a->dtype, state_vec4(a), a->dk, [&](auto t, auto v, auto r) {
-                const dim3 grid((a->dv + kStepCols - 1) / kStepCols, a->heads, n);
-                k_linattn_walk<decltype(t), decltype(v)::value, decltype(r)::value>
-                    <<<grid, kStepThreads, 0, static_cast<cudaStream_t>(stream)>>>(d, tab);
-                return launched("k_linattn_walk");
-            });
-            if (rc != SSLA_OK) return rc;
-        }
-        return SSLA_OK;
-    } catch (const std::bad_alloc&) {
-        return fail(SSLA_ERR_CUDA, "linear attention: host allocation failed");
+        return chunk_launch(d, a->dtype, seqs, workspace, static_cast<cudaStream_t>(stream));
+    } catch (const std::exception&) {
+        return fail(SSLA_ERR_CUDA, "%s: host allocation failed", who);
     }
 }
 

@@ -1,0 +1,593 @@
+// ssla_linattn_chunk.cu -- linear attention over whole sequences, 64 tokens
+// (a chunk) at a time on the tensor cores.
+//
+// With G_t the sum of a chunk's log decays up to token t and S_0 the state
+// before the chunk,
+//     out_t = scale (e^{G_t} q_t S_0 + sum_{s<=t} e^{G_t - G_s} (q_t . k_s) v_s)
+//     S     = e^{G_C} S_0 + sum_s e^{G_C - G_s} k_s v_s^T
+// so that a chunk is four small matrix products and the state moves once per
+// chunk.  A CTA walks the chunks of one segment of a sequence for one head
+// and DV state columns, the state in registers.
+//
+// Precision.  The matrix instructions take bf16 operands and add in 32 bits.
+// A 32-bit operand goes through as the sum of bf16 pieces (8 bits each):
+// bf16 inputs are one piece and exact, fp16 two and exact, fp32 three.
+// What is computed (decayed scores, decayed keys, the state) goes through as
+// two pieces, 2^-16, where it only reaches a 16-bit output, as three, 2^-24,
+// where it reaches a 32-bit output or the state.  Products of pieces whose
+// combined order is below those are left out.  Each chunk's sum is added to
+// the state by an ordinary 32-bit fma, so that the truncating adders of the
+// matrix unit never accumulate over a sequence.
+//
+// Long sequences.  Where the sequences and heads alone do not fill the GPU, a
+// sequence is divided into segments: k_chunk<OUT = false> leaves every
+// segment's own end state (from zero) and decay in the workspace,
+// k_chunk_join chains them into the segments' first states, and
+// k_chunk<OUT = true> runs all segments at once.
+//
+// Non-finite values.  A value in token s may not reach the outputs of tokens
+// before s, but 0 * inf in a masked place would take it there.  Masked scores
+// are replaced, not multiplied, and a non-finite v is taken out of the tile
+// and put back as NaN into its column from its own token on.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "ssla_linattn.cuh"
+
+namespace ssla {
+namespace ops {
+namespace {
+
+constexpr int kChunk = 64;
+constexpr int kThreads = 128;
+constexpr int kTable = 256;          // sequences of one launch
+
+struct Table {
+    int n;
+    int start[kTable], len[kTable], slot[kTable];
+    int seg0[kTable + 1];            // first segment of each sequence
+    int step[kTable];                // tokens of a segment (a multiple of kChunk)
+};
+
+// Pieces of the inputs and of what reaches only the outputs.
+template <typename T> struct Pieces;
+template <> struct Pieces<float> { static constexpr int in = 3, mid = 3, order = 2; };
+template <> struct Pieces<__half> { static constexpr int in = 2, mid = 2, order = 1; };
+template <> struct Pieces<__nv_bfloat16> { static constexpr int in = 1, mid = 2, order = 1; };
+
+template <typename T, int DK, int DV> struct Tile {
+    static constexpr int IN = Pieces<T>::in, MID = Pieces<T>::mid;
+    static constexpr int LK = DK + 8, LV = DV + 8;      // row lengths: 16-byte rows on distinct banks
+    static constexpr int kQ = 0, kK = kQ + IN * kChunk * LK, kV = kK + IN * kChunk * LK,
+                         kS = kV + IN * kChunk * LV, kEnd = kS + MID * DK * LV;
+    static constexpr int bytes = kEnd * 2 + (4 * kChunk + 4 + DV) * 4;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const __nv_bfloat16* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_addr(p)));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const __nv_bfloat16* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_addr(p)));
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+}
+// The next piece of (x, y); what is left stays in them.
+__device__ __forceinline__ uint32_t take(float& x, float& y) {
+    const uint32_t p = pack2(x, y);
+    const float2 f = unpack2(p);
+    x -= f.x;
+    y -= f.y;
+    return p;
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// Eight values of a row at p + c (zero from `width` on).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int c, int width, bool wide, float (&x)[8]) {
+    if (wide && c + 8 <= width) {
+        if constexpr (sizeof(T) == 2) {
+            load_vec<T, 8>(p + c, x);
+        } else {
+            float lo[4], hi[4];
+            load_vec<T, 4>(p + c, lo);
+            load_vec<T, 4>(p + c + 4, hi);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = lo[j], x[j + 4] = hi[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = c + j < width ? to_f<T>(p[c + j]) : 0.0f;
+    }
+}
+
+// Stages rows [0, rows) x [0, width) of a token tile as IN pieces.  With
+// `bad`, non-finite values become zero and their first row is noted by column.
+template <typename T, int D, int IN>
+__device__ __forceinline__ bool stage(__nv_bfloat16* s, const T* p, long long stride, int rows, int width, bool wide,
+                                      int* bad) {
+    constexpr int LD = D + 8, G = D / 8;
+    bool any = false;
+#pragma unroll
+    for (int i = threadIdx.x; i < kChunk * G; i += kThreads) {
+        const int r = i / G, c = i % G * 8;
+        float x[8] = {};
+        if (r < rows && c < width) load8<T>(p + r * stride, c, width, wide, x);
+        if (bad) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!finite(x[j])) {
+                    atomicMin(bad + c + j, r);
+                    x[j] = 0.0f;
+                    any = true;
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < IN; ++n) {
+            uint4 u;
+            u.x = take(x[0], x[1]); u.y = take(x[2], x[3]); u.z = take(x[4], x[5]); u.w = take(x[6], x[7]);
+            *reinterpret_cast<uint4*>(s + n * kChunk * LD + r * LD + c) = u;
+        }
+    }
+    return any;
+}
+
+// One float2 of a state row, bounds-checked.
+__device__ __forceinline__ float2 state_load2(const float* p, int r, int c, int dk, int dv) {
+    float2 x = make_float2(0.0f, 0.0f);
+    if (r < dk) {
+        if (c < dv) x.x = p[static_cast<size_t>(r) * dv + c];
+        if (c + 1 < dv) x.y = p[static_cast<size_t>(r) * dv + c + 1];
+    }
+    return x;
+}
+__device__ __forceinline__ void state_store2(float* p, int r, int c, int dk, int dv, float x, float y) {
+    if (r < dk) {
+        if (c < dv) p[static_cast<size_t>(r) * dv + c] = x;
+        if (c + 1 < dv) p[static_cast<size_t>(r) * dv + c + 1] = y;
+    }
+}
+
+// Segment states: [segment][head][dk][dv]; segment decays: [segment][head].
+template <typename T, int DK, int DV, bool OUT>
+__global__ void __launch_bounds__(kThreads)
+k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* seg_decay, int wide) {
+    using L = Tile<T, DK, DV>;
+    constexpr int IN = L::IN, MID = L::MID, ORD = Pieces<T>::order, LK = L::LK, LV = L::LV, NT = DV / 8;
+    constexpr int MT = DK >= 64 ? DK / 64 : 1;            // 16-row state tiles of a warp
+    constexpr int SN = DK >= 64 ? NT : NT / 2;            // and its 8-column tiles
+    extern __shared__ __align__(16) uint8_t smem[];
+    __nv_bfloat16* sb = reinterpret_cast<__nv_bfloat16*>(smem);
+    __nv_bfloat16 *sQ = sb + L::kQ, *sK = sb + L::kK, *sV = sb + L::kV, *sS = sb + L::kS;
+    float* ghi = reinterpret_cast<float*>(sb + L::kEnd);
+    float *glo = ghi + kChunk, *wk = glo + kChunk, *eg = wk + kChunk, *gam = eg + kChunk;
+    int* bad = reinterpret_cast<int*>(gam + 4);
+
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g8 = lane / 4, t2 = lane % 4 * 2;
+    const int h = blockIdx.y, c0 = blockIdx.x * DV;
+    // this CTA's sequence and segment
+    int lo = 0, hi = tab.n;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) / 2;
+        if (tab.seg0[m] <= static_cast<int>(blockIdx.z)) lo = m;
+        else hi = m;
+    }
+    const int seq = lo, seg = blockIdx.z - tab.seg0[seq], nseg = tab.seg0[seq + 1] - tab.seg0[seq];
+    if (!OUT && seg == nseg - 1) return;
+    const int first = seg * tab.step[seq], last = first + min(tab.len[seq] - first, tab.step[seq]);
+    const int slot = tab.slot[seq];
+    const size_t head_state = static_cast<size_t>(a.dk) * a.dv;
+    const int m0 = (DK >= 64 ? warp * MT : warp % 2) * 16, n0 = DK >= 64 ? 0 : warp / 2 * SN * 8;
+
+    float S[MT][SN][4];
+    const float* from = nullptr;
+    if (OUT && seg > 0) from = seg_state + (static_cast<size_t>(blockIdx.z - 1) * a.heads + h) * head_state;
+    else if (OUT && slot >= 0) from = a.state + (static_cast<size_t>(slot) * a.heads + h) * head_state;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < SN; ++j) {
+            float2 x = make_float2(0.0f, 0.0f), y = x;
+            if (from) {
+                x = state_load2(from, m0 + i * 16 + g8, c0 + n0 + j * 8 + t2, a.dk, a.dv);
+                y = state_load2(from, m0 + i * 16 + g8 + 8, c0 + n0 + j * 8 + t2, a.dk, a.dv);
+            }
+            S[i][j][0] = x.x; S[i][j][1] = x.y; S[i][j][2] = y.x; S[i][j][3] = y.y;
+        }
+    bool zero = from == nullptr;                           // S is zero: no product with it
+    double total = 0.0;
+
+    const int row0 = tab.start[seq];
+    const T* Q = static_cast<const T*>(a.q) + (h / a.q_share) * a.q_head;
+    const T* K = static_cast<const T*>(a.k) + (h / a.k_share) * a.k_head;
+    const T* V = static_cast<const T*>(a.v) + h * a.v_head + c0;
+
+    if (tid < DV) bad[tid] = kChunk;
+    __syncthreads();
+    for (int c = first; c < last; c += kChunk) {
+        const int n = min(kChunk, last - c);
+        const long long row = static_cast<long long>(row0) + c;
+        // ---- the chunk's tiles, decays and the state's pieces into shared memory ----
+        if (OUT) stage<T, DK, IN>(sQ, Q + row * a.q_row, a.q_row, n, a.dk, wide & 1, nullptr);
+        stage<T, DK, IN>(sK, K + row * a.k_row, a.k_row, n, a.dk, wide & 2, nullptr);
+        bool any = stage<T, DV, IN>(sV, V + row * a.v_row, a.v_row, n, a.dv - c0, wide & 4, bad);
+        if (OUT && !zero) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < SN; ++j) {
+                    float x0 = S[i][j][0], x1 = S[i][j][1], y0 = S[i][j][2], y1 = S[i][j][3];
+                    __nv_bfloat16* p = sS + (m0 + i * 16 + g8) * LV + n0 + j * 8 + t2;
+#pragma unroll
+                    for (int m = 0; m < MID; ++m) {
+                        *reinterpret_cast<uint32_t*>(p + m * DK * LV) = take(x0, x1);
+                        *reinterpret_cast<uint32_t*>(p + m * DK * LV + 8 * LV) = take(y0, y1);
+                    }
+                }
+        }
+        if (warp == 0) {
+            // inclusive sums of the log2 decays, in 64 bits: differences of them are exponents below
+            double s[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int t = 2 * lane + j;
+                float x = t < n ? a.decay[(row + t) * a.decay_row + h * a.decay_head] : 0.0f;
+                if (x < -1e5f) x = -1e5f;                   // e^-1e5 is 0 as well, and -inf - -inf is not
+                s[j] = x * 1.4426950408889634;
+            }
+            s[1] += s[0];
+            double run = s[1];
+#pragma unroll
+            for (int m = 1; m < 32; m <<= 1) {
+                const double o = __shfl_up_sync(0xFFFFFFFFu, run, m);
+                if (lane >= m) run += o;
+            }
+            const double all = __shfl_sync(0xFFFFFFFFu, run, 31), before = run - s[1];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int t = 2 * lane + j;
+                const double G = j ? run : before + s[0];
+                const float x = static_cast<float>(G);
+                ghi[t] = x;
+                glo[t] = static_cast<float>(G - x);
+                eg[t] = exp2f(x);
+                wk[t] = exp2f(static_cast<float>(all - G));
+            }
+            if (lane == 0) gam[0] = exp2f(static_cast<float>(all));
+            total += all;
+        }
+        any = __syncthreads_or(any);
+
+        if (OUT && warp * 16 < n) {
+            const int r0 = warp * 16;
+            float A[8][4], O[NT][4];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) A[j][0] = A[j][1] = A[j][2] = A[j][3] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) O[j][0] = O[j][1] = O[j][2] = O[j][3] = 0.0f;
+            // ---- scores q k^T up to the diagonal, and q S ----
+#pragma unroll 2
+            for (int ks = 0; ks < DK; ks += 16) {
+                if (ks >= a.dk) break;
+                uint32_t qa[IN][4];
+#pragma unroll
+                for (int i = 0; i < IN; ++i)
+                    ldsm4(qa[i], sQ + i * kChunk * LK + (r0 + lane % 16) * LK + ks + lane / 16 * 8);
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+                    if (p <= warp)
+#pragma unroll
+                        for (int i = 0; i < IN; ++i) {
+                            uint32_t b[4];
+                            ldsm4(b, sK + i * kChunk * LK + (p * 16 + lane % 8 + lane / 16 * 8) * LK + ks + lane / 8 % 2 * 8);
+#pragma unroll
+                            for (int q = 0; q < IN; ++q)
+                                if (q + i <= (IN == 1 ? 0 : ORD)) {
+                                    mma(A[2 * p], qa[q], b[0], b[1]);
+                                    mma(A[2 * p + 1], qa[q], b[2], b[3]);
+                                }
+                        }
+                if (!zero)
+#pragma unroll
+                    for (int p = 0; p < NT / 2; ++p)
+#pragma unroll
+                        for (int i = 0; i < MID; ++i) {
+                            uint32_t b[4];
+                            ldsm4t(b, sS + i * DK * LV + (ks + lane % 16) * LV + p * 16 + lane / 16 * 8);
+#pragma unroll
+                            for (int q = 0; q < IN; ++q)
+                                if (q + i <= ORD) {
+                                    mma(O[2 * p], qa[q], b[0], b[1]);
+                                    mma(O[2 * p + 1], qa[q], b[2], b[3]);
+                                }
+                        }
+            }
+            const int ra = r0 + g8, rb = ra + 8;
+            const float ea = eg[ra], eb = eg[rb], ha = ghi[ra], la = glo[ra], hb = ghi[rb], lb = glo[rb];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) O[j][0] *= ea, O[j][1] *= ea, O[j][2] *= eb, O[j][3] *= eb;
+            // ---- decayed scores (masked ones replaced), times v ----
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+                if (p <= warp && p * 16 < n) {
+                    float P[2][4];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int s = p * 16 + j * 8 + t2 + e;
+                            const float hs = ghi[s], ls = glo[s];
+                            P[j][e] = s <= ra ? A[2 * p + j][e] * exp2f((ha - hs) + (la - ls)) : 0.0f;
+                            P[j][2 + e] = s <= rb ? A[2 * p + j][2 + e] * exp2f((hb - hs) + (lb - ls)) : 0.0f;
+                        }
+                    uint32_t pa[MID][4];
+#pragma unroll
+                    for (int i = 0; i < MID; ++i) {
+                        pa[i][0] = take(P[0][0], P[0][1]);
+                        pa[i][1] = take(P[0][2], P[0][3]);
+                        pa[i][2] = take(P[1][0], P[1][1]);
+                        pa[i][3] = take(P[1][2], P[1][3]);
+                    }
+#pragma unroll
+                    for (int m = 0; m < NT / 2; ++m)
+#pragma unroll
+                        for (int i = 0; i < IN; ++i) {
+                            uint32_t b[4];
+                            ldsm4t(b, sV + i * kChunk * LV + (p * 16 + lane % 16) * LV + m * 16 + lane / 16 * 8);
+#pragma unroll
+                            for (int q = 0; q < MID; ++q)
+                                if (q + i <= ORD) {
+                                    mma(O[2 * m], pa[q], b[0], b[1]);
+                                    mma(O[2 * m + 1], pa[q], b[2], b[3]);
+                                }
+                        }
+                }
+            if (any)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int b = bad[j * 8 + t2 + e];
+                        if (ra >= b) O[j][e] = __int_as_float(0x7FC00000);
+                        if (rb >= b) O[j][2 + e] = __int_as_float(0x7FC00000);
+                    }
+            T* po = static_cast<T*>(a.out) + h * a.out_head + c0;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int col = j * 8 + t2 + e;
+                    if (c0 + col < a.dv) {
+                        if (ra < n) po[(row + ra) * a.out_row + col] = from_f<T>(O[j][e] * a.scale);
+                        if (rb < n) po[(row + rb) * a.out_row + col] = from_f<T>(O[j][2 + e] * a.scale);
+                    }
+                }
+        }
+        // ---- the state: decayed keys, transposed, times v ----
+        const float gc = gam[0];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            if (m0 + i * 16 >= a.dk) break;
+            float U[SN][4];
+#pragma unroll
+            for (int j = 0; j < SN; ++j) U[j][0] = U[j][1] = U[j][2] = U[j][3] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < kChunk; ks += 16) {
+                if (ks >= n) break;
+                const int kr = ks + lane % 8 + lane / 16 * 8, kc = m0 + i * 16 + lane / 8 % 2 * 8;
+                float2 f[4] = {};
+#pragma unroll
+                for (int m = 0; m < IN; ++m) {
+                    uint32_t r[4];
+                    ldsm4t(r, sK + m * kChunk * LK + kr * LK + kc);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 x = unpack2(r[e]);
+                        f[e].x += x.x;
+                        f[e].y += x.y;
+                    }
+                }
+                const float w0 = wk[ks + t2], w1 = wk[ks + t2 + 1], w2 = wk[ks + t2 + 8], w3 = wk[ks + t2 + 9];
+                f[0].x *= w0; f[0].y *= w1; f[1].x *= w0; f[1].y *= w1;
+                f[2].x *= w2; f[2].y *= w3; f[3].x *= w2; f[3].y *= w3;
+                uint32_t ka[3][4];
+#pragma unroll
+                for (int m = 0; m < 3; ++m)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ka[m][e] = take(f[e].x, f[e].y);
+#pragma unroll
+                for (int p = 0; p < SN / 2; ++p)
+#pragma unroll
+                    for (int m = 0; m < IN; ++m) {
+                        uint32_t b[4];
+                        ldsm4t(b, sV + m * kChunk * LV + (ks + lane % 16) * LV + n0 + p * 16 + lane / 16 * 8);
+#pragma unroll
+                        for (int q = 0; q < 3; ++q)
+                            if (q + m <= 2) {
+                                mma(U[2 * p], ka[q], b[0], b[1]);
+                                mma(U[2 * p + 1], ka[q], b[2], b[3]);
+                            }
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < SN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    S[i][j][e] = fmaf(gc, S[i][j][e], U[j][e]);
+                    if (any && bad[n0 + j * 8 + t2 + e % 2] < kChunk) S[i][j][e] = __int_as_float(0x7FC00000);
+                }
+        }
+        zero = false;
+        __syncthreads();                                    // the tiles are rewritten
+        if (any) {
+            if (tid < DV) bad[tid] = kChunk;
+            __syncthreads();
+        }
+    }
+
+    float* to = nullptr;
+    if (!OUT) to = seg_state + (static_cast<size_t>(blockIdx.z) * a.heads + h) * head_state;
+    else if (seg == nseg - 1 && slot >= 0 && last > first)
+        to = a.state + (static_cast<size_t>(slot) * a.heads + h) * head_state;
+    if (to)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < SN; ++j) {
+                const int r = m0 + i * 16 + g8, c = c0 + n0 + j * 8 + t2;
+                state_store2(to, r, c, a.dk, a.dv, S[i][j][0], S[i][j][1]);
+                state_store2(to, r + 8, c, a.dk, a.dv, S[i][j][2], S[i][j][3]);
+            }
+    if (!OUT && blockIdx.x == 0 && tid == 0) seg_decay[static_cast<size_t>(blockIdx.z) * a.heads + h] = total;
+}
+
+// Chains a sequence's segments: segment i's place in the workspace becomes
+// the state after it.  One thread per state element.
+__global__ void __launch_bounds__(256)
+k_chunk_join(LinArgs a, const __grid_constant__ Table tab, float* seg_state, const double* seg_decay) {
+    const int seq = blockIdx.z, h = blockIdx.y;
+    const int s0 = tab.seg0[seq], s1 = tab.seg0[seq + 1] - 1;
+    const int e = blockIdx.x * 256 + threadIdx.x;
+    if (s0 >= s1 || e >= a.dk * a.dv) return;
+    const size_t head_state = static_cast<size_t>(a.dk) * a.dv;
+    const int slot = tab.slot[seq];
+    float run = slot >= 0 ? a.state[(static_cast<size_t>(slot) * a.heads + h) * head_state + e] : 0.0f;
+    for (int s = s0; s < s1; ++s) {
+        float* p = seg_state + (static_cast<size_t>(s) * a.heads + h) * head_state + e;
+        run = fmaf(exp2f(static_cast<float>(seg_decay[static_cast<size_t>(s) * a.heads + h])), run, *p);
+        *p = run;
+    }
+}
+
+// ---- host ------------------------------------------------------------------
+struct Shape {
+    int dk, dv, ctas;               // tile and resident CTAs per SM
+};
+
+template <typename F> auto with_shape(int dtype, int dk, int dv, F&& f) {
+    auto by_dk = [&](auto t, auto v) {
+        using std::integral_constant;
+        if (dk <= 32) return f(t, integral_constant<int, 32>(), v);
+        if (dk <= 64) return f(t, integral_constant<int, 64>(), v);
+        return f(t, integral_constant<int, 128>(), v);
+    };
+    auto by_dv = [&](auto t) {
+        return dv <= 32 ? by_dk(t, std::integral_constant<int, 32>()) : by_dk(t, std::integral_constant<int, 64>());
+    };
+    return dtype == SSLA_DT_F32 ? by_dv(float()) : dtype == SSLA_DT_BF16 ? by_dv(__nv_bfloat16()) : by_dv(__half());
+}
+
+Shape shape_of(int dtype, int dk, int dv) {
+    return with_shape(dtype, dk, dv, [](auto t, auto k, auto v) {
+        constexpr int K = decltype(k)::value, V = decltype(v)::value;
+        const int bytes = Tile<decltype(t), K, V>::bytes;
+        return Shape{K, V, std::max(1, std::min(K * V >= 128 * 64 ? 2 : 4, (227 * 1024) / (bytes + 1024)))};
+    });
+}
+
+// Tokens of a segment for sequences [i0, i1): whole sequences where they fill
+// the GPU, else segments such that all resident CTAs have one.  A divided
+// sequence costs its keys and values a second pass (about 0.45 of the work).
+int segment_tokens(const LinArgs& a, const Shape& sh, const std::vector<Seq>& seqs, size_t i0, size_t i1) {
+    long long chunks = 0, longest = 0, per = static_cast<long long>(a.heads) * ((a.dv + sh.dv - 1) / sh.dv);
+    for (size_t i = i0; i < i1; ++i) {
+        const long long n = (seqs[i].len + kChunk - 1LL) / kChunk;
+        chunks += n;
+        longest = std::max(longest, n);
+    }
+    const long long slots = 148LL * sh.ctas;
+    const long long whole = std::max(longest, (chunks * per + slots - 1) / slots);
+    const long long step = std::max(4LL, (chunks * per + slots - 1) / slots);
+    if (whole * 100 <= step * 145 || step >= longest) return INT_MAX / 2 / kChunk * kChunk;
+    return static_cast<int>(step * kChunk);
+}
+
+int segments(const Seq& s, int tokens) { return s.len ? (s.len - 1) / tokens + 1 : 0; }
+
+// Ends of the launch groups: at most kTable sequences and 65535 segments.
+size_t group_end(const std::vector<Seq>& seqs, size_t i0) { return std::min(seqs.size(), i0 + kTable); }
+
+}  // namespace
+
+size_t chunk_workspace(const LinArgs& a, int dtype, const std::vector<Seq>& seqs) {
+    const Shape sh = shape_of(dtype, a.dk, a.dv);
+    size_t most = 0;
+    for (size_t i0 = 0; i0 < seqs.size(); i0 = group_end(seqs, i0)) {
+        const size_t i1 = group_end(seqs, i0);
+        const int tokens = segment_tokens(a, sh, seqs, i0, i1);
+        size_t n = 0;
+        bool divided = false;
+        for (size_t i = i0; i < i1; ++i) {
+            n += segments(seqs[i], tokens);
+            divided |= segments(seqs[i], tokens) > 1;
+        }
+        if (divided) most = std::max(most, n * a.heads * (8 + 4 * static_cast<size_t>(a.dk) * a.dv));
+    }
+    return most;
+}
+
+int chunk_launch(const LinArgs& a, int dtype, const std::vector<Seq>& seqs, void* workspace, cudaStream_t st) {
+    const Shape sh = shape_of(dtype, a.dk, a.dv);
+    const int esz = dtype_size(dtype), lanes = 16 / esz;
+    auto wide = [&](const void* p, long long row, long long head) {
+        return aligned(p, 16) && row % lanes == 0 && head % lanes == 0;
+    };
+    const int wides = (wide(a.q, a.q_row, a.q_head) ? 1 : 0) | (wide(a.k, a.k_row, a.k_head) ? 2 : 0) |
+                      (wide(a.v, a.v_row, a.v_head) ? 4 : 0);
+    for (size_t i0 = 0; i0 < seqs.size(); i0 = group_end(seqs, i0)) {
+        const size_t i1 = group_end(seqs, i0);
+        const int tokens = segment_tokens(a, sh, seqs, i0, i1);
+        Table tab;
+        tab.n = 0;
+        tab.seg0[0] = 0;
+        bool divided = false;
+        for (size_t i = i0; i < i1; ++i) {
+            if (!seqs[i].len) continue;
+            const int n = segments(seqs[i], tokens), k = tab.n++;
+            tab.start[k] = seqs[i].start;
+            tab.len[k] = seqs[i].len;
+            tab.slot[k] = seqs[i].slot;
+            tab.step[k] = tokens;
+            tab.seg0[k + 1] = tab.seg0[k] + n;
+            divided |= n > 1;
+        }
+        if (!tab.n) continue;
+        const int nseg = tab.seg0[tab.n];
+        double* decays = static_cast<double*>(workspace);
+        float* states = reinterpret_cast<float*>(decays + static_cast<size_t>(nseg) * a.heads);
+        const int rc = with_shape(dtype, a.dk, a.dv, [&](auto t, auto k, auto v) {
+            using T = decltype(t);
+            constexpr int K = decltype(k)::value, V = decltype(v)::value, bytes = Tile<T, K, V>::bytes;
+            cudaFuncSetAttribute(k_chunk<T, K, V, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            const dim3 grid((a.dv + V - 1) / V, a.heads, nseg);
+            if (divided) {
+                cudaFuncSetAttribute(k_chunk<T, K, V, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+                k_chunk<T, K, V, false><<<grid, kThreads, bytes, st>>>(a, tab, states, decays, wides);
+                k_chunk_join<<<dim3((a.dk * a.dv + 255) / 256, a.heads, tab.n), 256, 0, st>>>(a, tab, states, decays);
+            }
+            k_chunk<T, K, V, true><<<grid, kThreads, bytes, st>>>(a, tab, states, decays, wides);
+            return launched("k_chunk");
+        });
+        if (rc != SSLA_OK) return rc;
+    }
+    return SSLA_OK;
+}
+
+}  // namespace ops
+}  // namespace ssla
