@@ -5,14 +5,17 @@
 // times the channels of one group.
 //   - small slabs (k_gn_slab): a few lanes or one CTA hold a slab in
 //     registers; one read, two-pass statistics, one write;
+//   - slabs that fit the shared memory of a cluster of up to eight CTAs
+//     (k_gn_cluster): one read, one write;
 //   - others: k_gn_sums leaves every slab's shifted sums per slice of the
 //     positions in the workspace, k_gn_apply joins them (in 64 bits) and
-//     writes the outputs.
+//     writes the outputs; the second read mostly comes from L2.
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <numeric>
 
 #include "ssla_ops.cuh"
 
@@ -27,21 +30,96 @@ struct GnArgs {
     long long x_sample, x_pos, y_sample, y_pos;
     int n, positions, channels, groups, width;     // width: channels of a group
     int act;
+    int wide;                                      // weight and bias are 16-byte aligned
+    float* shift;                                  // large slabs: what their sums are shifted by
     float eps;
 };
 
-// y / (1 + e^-y); where e^-y overflows the limit is -0.  16-bit outputs take
-// the fast exponential and quotient (their errors, about 2^-21 here, are far
-// below half a step of the output, 2^-9 or 2^-12), 32-bit ones do not.
-template <typename T> __device__ __forceinline__ float silu(float y) {
-    if constexpr (sizeof(T) == 2) return __fdividef(y, 1.0f + __expf(-y));
-    else return y / (1.0f + expf(-y));
+// A vector's elements two at a time (packed 32-bit arithmetic); each
+// component is the ordinary operation.
+template <int VEC> __device__ __forceinline__ float add_up(const float (&x)[VEC]) {
+    if constexpr (VEC == 1) return x[0];
+    else {
+        float2 s = make_float2(x[0], x[1]);
+#pragma unroll
+        for (int j = 2; j < VEC; j += 2) s = __fadd2_rn(s, make_float2(x[j], x[j + 1]));
+        return s.x + s.y;
+    }
+}
+// s1 += sum of (x - shift), s2 += sum of their squares.
+template <int VEC> __device__ __forceinline__ void moments(const float (&x)[VEC], float shift, float2& s1, float2& s2) {
+    if constexpr (VEC == 1) {
+        const float d = x[0] - shift;
+        s1.x += d;
+        s2.x = fmaf(d, d, s2.x);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const float2 d = __fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-shift, -shift));
+            s1 = __fadd2_rn(s1, d);
+            s2 = __ffma2_rn(d, d, s2);
+        }
+    }
 }
 
-template <typename T>
-__device__ __forceinline__ float gn_finish(float x, float mean, float rstd, float w, float b, int act) {
-    const float y = fmaf((x - mean) * rstd, w, b);
-    return act == SSLA_ACT_SILU ? silu<T>(y) : y;
+// y / (1 + e^-y) with the hardware's exponential and reciprocal: relative
+// errors of 2^-22 each and |y| 2^-24 from rounding the exponent, which is
+// below 2^-20 where the value counts and below half a step of 16-bit outputs
+// everywhere.  Where e^-y overflows the limit is -0.
+__device__ __forceinline__ float sigmoid_of(float neg_y_log2e) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(neg_y_log2e));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+}
+
+// x <- act((x - mean) * rstd * w + b)
+template <int VEC>
+__device__ __forceinline__ void gn_finish(float (&x)[VEC], float mean, float rstd, const float (&w)[VEC], const float (&b)[VEC],
+                                          int act) {
+    if constexpr (VEC == 1) {
+        x[0] = fmaf((x[0] - mean) * rstd, w[0], b[0]);
+        if (act == SSLA_ACT_SILU) x[0] *= sigmoid_of(x[0] * -1.44269504f);
+    } else {
+        const float2 m = make_float2(-mean, -mean), r = make_float2(rstd, rstd);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const float2 y = __ffma2_rn(__fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), m), r), make_float2(w[j], w[j + 1]),
+                                        make_float2(b[j], b[j + 1]));
+            x[j] = y.x;
+            x[j + 1] = y.y;
+        }
+        if (act == SSLA_ACT_SILU) {
+#pragma unroll
+            for (int j = 0; j < VEC; j += 2) {
+                const float2 y = make_float2(x[j], x[j + 1]);
+                const float2 t = __fmul2_rn(y, make_float2(-1.44269504f, -1.44269504f));
+                const float2 o = __fmul2_rn(y, make_float2(sigmoid_of(t.x), sigmoid_of(t.y)));
+                x[j] = o.x;
+                x[j + 1] = o.y;
+            }
+        }
+    }
+}
+
+// VEC weights (or the given constant) from channel c on.
+template <int VEC>
+__device__ __forceinline__ void channel_params(const float* p, int c, float none, bool wide, float (&x)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = none;
+    if (!p) return;
+    if constexpr (VEC >= 4) {
+        if (wide) {
+#pragma unroll
+            for (int j = 0; j < VEC; j += 4) {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(p + c + j));
+                x[j] = f.x; x[j + 1] = f.y; x[j + 2] = f.z; x[j + 3] = f.w;
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = __ldg(p + c + j);
 }
 
 // ---- small slabs: LPS threads each hold EPT vectors of a slab -------------
@@ -59,52 +137,92 @@ template <int LPS> __device__ __forceinline__ float slab_sum(float v, float* red
     return v;
 }
 
-template <typename T, int VEC, int LPS, int EPT>
-__global__ void __launch_bounds__(kGnThreads) k_gn_slab(GnArgs a, const T* x, T* y) {
+constexpr int kGnSlabCtas = 4;     // resident CTAs per SM that the one-vector forms are built for
+
+// A thread takes UNR slabs at a time, gridDim.x * (slabs of a CTA) apart:
+// the launch makes that a multiple of the groups where it can, so that a
+// thread's channels, and the weights it keeps, stay the same.
+template <typename T, int VEC, int LPS, int EPT, int UNR>
+__global__ void __launch_bounds__(kGnThreads, LPS <= 32 && EPT == 1 ? kGnSlabCtas : 1) k_gn_slab(GnArgs a, const T* x, T* y) {
     __shared__ float red[kGnThreads / 32];
+    constexpr int kPer = kGnThreads / LPS;
     const int lane = threadIdx.x % LPS;
-    const long long slab = static_cast<long long>(blockIdx.x) * (kGnThreads / LPS) + threadIdx.x / LPS;
-    const bool on = slab < static_cast<long long>(a.n) * a.groups;
-    const int n = on ? static_cast<int>(slab / a.groups) : 0, g = on ? static_cast<int>(slab % a.groups) : 0;
+    const unsigned slabs = static_cast<unsigned>(a.n) * a.groups, stride = gridDim.x * kPer;   // below 2^31 (check_gn)
     const int wv = a.width / VEC, vecs = a.positions * wv;
-    const T* xp = x + n * a.x_sample + g * a.width;
-    float v[EPT][VEC];
-    float sum = 0.0f;
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-        const int k = e * LPS + lane;
-        if (on && k < vecs) {
-            const int p = k / wv;
-            load_vec<T, VEC>(xp + p * a.x_pos + (k - p * wv) * VEC, v[e]);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) sum += v[e][j];
-        }
-    }
     const float inv = 1.0f / (static_cast<float>(a.positions) * static_cast<float>(a.width));
-    const float mean = slab_sum<LPS>(sum, red) * inv;
-    float sq = 0.0f;
+    const bool wide = VEC >= 4 && a.wide;
+    float w[EPT][VEC], b[EPT][VEC];
+    int kept = -1;
+    // a multiple of the groups apart, a thread's slabs need no division
+    const unsigned groups = a.groups, turn = stride / groups, first = blockIdx.x * kPer + threadIdx.x / LPS;
+    const bool steady = turn * groups == stride;
+    const unsigned n_first = first / groups, g_first = first - n_first * groups;
+    unsigned round = 0;
+    auto params = [&](int g) {
 #pragma unroll
-    for (int e = 0; e < EPT; ++e)
-        if (on && e * LPS + lane < vecs)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float d = v[e][j] - mean;
-                sq = fmaf(d, d, sq);
+        for (int e = 0; e < EPT; ++e) {
+            const int k = e * LPS + lane;
+            if (k < vecs) {
+                const int c = (a.positions == 1 ? k : k % wv) * VEC;
+                channel_params<VEC>(a.weight, g * a.width + c, 1.0f, wide, w[e]);
+                channel_params<VEC>(a.bias, g * a.width + c, 0.0f, wide, b[e]);
             }
-    const float rstd = 1.0f / sqrtf(slab_sum<LPS>(sq, red) * inv + a.eps);
-    T* yp = y + n * a.y_sample + g * a.width;
+        }
+        kept = g;
+    };
+    if (first < slabs) params(g_first);             // in flight with the first values
+    // all threads of a CTA run the same rounds (wide slabs meet at barriers)
+    for (unsigned base = blockIdx.x * kPer; base < slabs; base += UNR * stride, round += UNR) {
+        float v[UNR][EPT][VEC], mean[UNR], rstd[UNR];
+        int n[UNR], g[UNR];
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-        const int k = e * LPS + lane;
-        if (on && k < vecs) {
-            const int p = k / wv, c = (k - p * wv) * VEC;
+        for (int u = 0; u < UNR; ++u) {
+            const unsigned slab = base + u * stride + threadIdx.x / LPS;
+            const unsigned nn = steady ? n_first + (round + u) * turn : slab / groups;
+            n[u] = slab < slabs ? static_cast<int>(nn) : -1;
+            g[u] = slab < slabs ? static_cast<int>(steady ? g_first : slab - nn * groups) : 0;
+            const T* xp = x + (n[u] >= 0 ? n[u] * a.x_sample + static_cast<long long>(g[u]) * a.width : 0);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const int ch = g * a.width + c + j;
-                v[e][j] = gn_finish<T>(v[e][j], mean, rstd, a.weight ? __ldg(a.weight + ch) : 1.0f,
-                                       a.bias ? __ldg(a.bias + ch) : 0.0f, a.act);
+            for (int e = 0; e < EPT; ++e) {
+                const int k = e * LPS + lane;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[u][e][j] = 0.0f;
+                if (n[u] >= 0 && k < vecs) {
+                    const int p = a.positions == 1 ? 0 : k / wv;
+                    load_vec<T, VEC>(xp + p * a.x_pos + (k - p * wv) * VEC, v[u][e]);
+                }
             }
-            store_vec<T, VEC>(yp + p * a.y_pos + c, v[e]);
+        }
+#pragma unroll
+        for (int u = 0; u < UNR; ++u) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < EPT; ++e) sum += add_up<VEC>(v[u][e]);
+            mean[u] = slab_sum<LPS>(sum, red) * inv;
+        }
+#pragma unroll
+        for (int u = 0; u < UNR; ++u) {
+            float2 none = make_float2(0.0f, 0.0f), sq = none;
+#pragma unroll
+            for (int e = 0; e < EPT; ++e)
+                if (e * LPS + lane < vecs) moments<VEC>(v[u][e], mean[u], none, sq);
+            const float var = slab_sum<LPS>(sq.x + sq.y, red) * inv + a.eps;
+            rstd[u] = sizeof(T) == 2 ? rsqrtf(var) : 1.0f / sqrtf(var);
+        }
+#pragma unroll
+        for (int u = 0; u < UNR; ++u) {
+            if (n[u] < 0) continue;
+            T* yp = y + n[u] * a.y_sample + static_cast<long long>(g[u]) * a.width;
+            if (g[u] != kept) params(g[u]);
+#pragma unroll
+            for (int e = 0; e < EPT; ++e) {
+                const int k = e * LPS + lane;
+                if (k < vecs) {
+                    const int p = a.positions == 1 ? 0 : k / wv, c = (k - p * wv) * VEC;
+                    gn_finish<VEC>(v[u][e], mean[u], rstd[u], w[e], b[e], a.act);
+                    store_vec<T, VEC>(yp + p * a.y_pos + c, v[u][e]);
+                }
+            }
         }
     }
 }
@@ -128,7 +246,7 @@ __global__ void __launch_bounds__(kGnThreads) k_gn_sums(GnArgs a, GnSplit s, con
     const int p1 = static_cast<int>(static_cast<long long>(a.positions) * (blockIdx.x + 1) / s.splits);
     const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx;
     const T* xn = x + n * a.x_sample + static_cast<long long>(g0) * a.width;
-    float s1 = 0.0f, s2 = 0.0f;
+    float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
     if (ty < s.ty)
         for (int c = tx; c < cv; c += s.tx) {
             // the first position's first channel of the group as the shift
@@ -138,15 +256,10 @@ __global__ void __launch_bounds__(kGnThreads) k_gn_sums(GnArgs a, GnSplit s, con
             for (int p = p0 + ty; p < p1; p += s.ty) {
                 float v[VEC];
                 load_vec<T, VEC>(xp + p * a.x_pos, v);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float d = v[j] - shift;
-                    s1 += d;
-                    s2 = fmaf(d, d, s2);
-                }
+                moments<VEC>(v, shift, s1, s2);
             }
         }
-    red[threadIdx.x] = make_float2(s1, s2);
+    red[threadIdx.x] = make_float2(s1.x + s1.y, s2.x + s2.y);
     __syncthreads();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     for (int g = warp; g < ng; g += kGnThreads / 32) {
@@ -162,63 +275,177 @@ __global__ void __launch_bounds__(kGnThreads) k_gn_sums(GnArgs a, GnSplit s, con
             a1 += __shfl_xor_sync(0xFFFFFFFFu, a1, m);
             a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
         }
-        if (lane == 0) part[(static_cast<size_t>(n) * a.groups + g0 + g) * s.splits + blockIdx.x] = make_float2(a1, a2);
+        if (lane == 0) {
+            const size_t slab = static_cast<size_t>(n) * a.groups + g0 + g;
+            part[slab * s.splits + blockIdx.x] = make_float2(a1, a2);
+            // (an output written in place has replaced the value itself by then)
+            if (blockIdx.x == 0) a.shift[slab] = to_f<T>(xn[g * a.width]);
+        }
     }
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kGnThreads) k_gn_stats(GnArgs a, int splits, const T* x, const float2* part, float2* stat) {
-    // one warp per slab: joins the slices' sums in 64 bits
-    const long long slab = static_cast<long long>(blockIdx.x) * (kGnThreads / 32) + threadIdx.x / 32;
-    if (slab >= static_cast<long long>(a.n) * a.groups) return;
-    const int lane = threadIdx.x % 32;
-    double a1 = 0.0, a2 = 0.0;
-    for (int k = lane; k < splits; k += 32) {
-        const float2 r = part[slab * splits + k];
-        a1 += r.x;
-        a2 += r.y;
-    }
-#pragma unroll
-    for (int m = 16; m; m >>= 1) {
-        a1 += __shfl_xor_sync(0xFFFFFFFFu, a1, m);
-        a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
-    }
-    if (lane == 0) {
-        const double inv = 1.0 / (static_cast<double>(a.positions) * a.width);
-        const float shift = gn_shift(to_f<T>(x[slab / a.groups * a.x_sample + slab % a.groups * a.width]));
-        const double m = a1 * inv, var = a2 * inv - m * m;   // a non-finite value: NaN
-        stat[slab] = make_float2(static_cast<float>(shift + m), static_cast<float>(1.0 / sqrt((var < 0.0 ? 0.0 : var) + a.eps)));
-    }
-}
-
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kGnThreads) k_gn_apply(GnArgs a, GnSplit s, const T* x, T* y, const float2* stat) {
+__global__ void __launch_bounds__(kGnThreads)
+k_gn_apply(GnArgs a, GnSplit s, const T* x, T* y, const float2* part) {
+    extern __shared__ float2 stat[];               // (mean, 1 / deviation) of the CTA's groups
     const int n = blockIdx.z, g0 = blockIdx.y * s.gpc, ng = min(s.gpc, a.groups - g0);
     const int wv = a.width / VEC, cv = ng * wv;
     const int p0 = static_cast<int>(static_cast<long long>(a.positions) * blockIdx.x / s.splits);
     const int p1 = static_cast<int>(static_cast<long long>(a.positions) * (blockIdx.x + 1) / s.splits);
     const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx;
-    if (ty >= s.ty) return;
     const int ch0 = g0 * a.width;
-    for (int c = tx; c < cv; c += s.tx) {
-        const float2 st = stat[static_cast<size_t>(n) * a.groups + g0 + c / wv];
-        float w[VEC], b[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            w[j] = a.weight ? __ldg(a.weight + ch0 + c * VEC + j) : 1.0f;
-            b[j] = a.bias ? __ldg(a.bias + ch0 + c * VEC + j) : 0.0f;
+    const T* xn = x + n * a.x_sample + ch0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the sums of the kernel before
+    // one warp a slab joins the slices' sums, in 64 bits
+    for (int g = threadIdx.x / 32; g < ng; g += kGnThreads / 32) {
+        double a1 = 0.0, a2 = 0.0;
+        for (int k = threadIdx.x % 32; k < s.splits; k += 32) {
+            const float2 r = part[(static_cast<size_t>(n) * a.groups + g0 + g) * s.splits + k];
+            a1 += r.x;
+            a2 += r.y;
         }
-        const T* xp = x + n * a.x_sample + ch0 + c * VEC;
+#pragma unroll
+        for (int m = 16; m; m >>= 1) {
+            a1 += __shfl_xor_sync(0xFFFFFFFFu, a1, m);
+            a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
+        }
+        if (threadIdx.x % 32 == 0) {
+            const double inv = 1.0 / (static_cast<double>(a.positions) * a.width);
+            const float shift = gn_shift(a.shift[static_cast<size_t>(n) * a.groups + g0 + g]);
+            const double m = a1 * inv, var = a2 * inv - m * m;   // a non-finite value: NaN
+            stat[g] = make_float2(static_cast<float>(shift + m), static_cast<float>(1.0 / sqrt((var < 0.0 ? 0.0 : var) + a.eps)));
+        }
+    }
+    __syncthreads();
+    if (ty >= s.ty) return;
+    for (int c = tx; c < cv; c += s.tx) {
+        const float2 st = stat[c / wv];
+        float w[VEC], b[VEC];
+        channel_params<VEC>(a.weight, ch0 + c * VEC, 1.0f, VEC >= 4 && a.wide, w);
+        channel_params<VEC>(a.bias, ch0 + c * VEC, 0.0f, VEC >= 4 && a.wide, b);
+        const T* xp = xn + c * VEC;
         T* yp = y + n * a.y_sample + ch0 + c * VEC;
 #pragma unroll 4
         for (int p = p0 + ty; p < p1; p += s.ty) {
             float v[VEC];
             load_vec<T, VEC>(xp + p * a.x_pos, v);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = gn_finish<T>(v[j], st.x, st.y, w[j], b[j], a.act);
+            gn_finish<VEC>(v, st.x, st.y, w, b, a.act);
             store_vec<T, VEC>(yp + p * a.y_pos, v);
         }
     }
+}
+
+// ---- slabs that fit the shared memory of a cluster -----------------------------
+// One read: each CTA of a cluster keeps its slice of the positions (of `gpc`
+// whole groups of one sample) in shared memory -- every thread its own
+// vectors, in its own places --, the CTAs read one another's sums through
+// distributed shared memory, and each writes its slice's outputs.
+constexpr int kGnClusterThreads = 1024;
+constexpr int kGnClusterBytes = 192 * 1024;
+
+struct GnCluster {
+    int ctas, chunks, gpc, tx, ty, rounds;         // rounds: position steps of a thread
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCluster s, const T* x, T* y) {
+    extern __shared__ __align__(16) uint8_t gn_smem[];
+    __shared__ float2 red[kGnClusterThreads];
+    Pack<T, VEC>* tile = reinterpret_cast<Pack<T, VEC>*>(gn_smem);
+    float2* sums = reinterpret_cast<float2*>(gn_smem + static_cast<size_t>(s.rounds) * kGnClusterThreads * sizeof(Pack<T, VEC>));
+    float2* stat = sums + s.gpc;
+    float* shifts = reinterpret_cast<float*>(stat + s.gpc);
+    const int rank = blockIdx.x, n = blockIdx.z, g0 = blockIdx.y * s.gpc, ng = min(s.gpc, a.groups - g0);
+    const int wv = a.width / VEC, cv = ng * wv;
+    const int p0 = static_cast<int>(static_cast<long long>(a.positions) * rank / s.ctas);
+    const int p1 = static_cast<int>(static_cast<long long>(a.positions) * (rank + 1) / s.ctas);
+    const int tid = threadIdx.x, tx = tid % s.tx, ty = tid / s.tx, ch0 = g0 * a.width;
+    const bool on = ty < s.ty && tx < cv;
+    const int g = on ? tx / wv : 0;
+    const T* xn = x + n * a.x_sample + ch0;
+    float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
+    const float shift = gn_shift(to_f<T>(xn[g * a.width]));
+    float w[VEC], b[VEC];
+    if (on) {
+        const T* xp = xn + tx * VEC;
+        constexpr int kBatch = 8;                  // loads in flight
+        for (int r0 = 0; r0 < s.rounds; r0 += kBatch) {
+            Pack<T, VEC> k[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int p = p0 + ty + (r0 + i) * s.ty;
+                if (p < p1) k[i] = *reinterpret_cast<const Pack<T, VEC>*>(xp + p * a.x_pos);
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                if (p0 + ty + (r0 + i) * s.ty >= p1) break;
+                tile[(r0 + i) * kGnClusterThreads + tid] = k[i];
+                float v[VEC];
+                unpack_vec<T, VEC>(k[i], v);
+                moments<VEC>(v, shift, s1, s2);
+            }
+        }
+    }
+    if (on) {
+        channel_params<VEC>(a.weight, ch0 + tx * VEC, 1.0f, VEC >= 4 && a.wide, w);
+        channel_params<VEC>(a.bias, ch0 + tx * VEC, 0.0f, VEC >= 4 && a.wide, b);
+        if (ty == 0 && tx == g * wv) shifts[g] = shift;
+    }
+    red[tid] = make_float2(s1.x + s1.y, s2.x + s2.y);
+    __syncthreads();
+    const int warp = tid / 32, lane = tid % 32;
+    for (int i = warp; i < ng; i += kGnClusterThreads / 32) {
+        float a1 = 0.0f, a2 = 0.0f;
+        const int t0 = wv < 32 ? lane : 0, dt = wv < 32 ? 32 : 1, q0 = wv < 32 ? 0 : lane, dq = wv < 32 ? 1 : 32;
+        for (int t = t0; t < s.ty; t += dt)
+            for (int q = q0; q < wv; q += dq) {
+                const float2 r = red[t * s.tx + i * wv + q];
+                a1 += r.x;
+                a2 += r.y;
+            }
+#pragma unroll
+        for (int m = 16; m; m >>= 1) {
+            a1 += __shfl_xor_sync(0xFFFFFFFFu, a1, m);
+            a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
+        }
+        if (lane == 0) sums[i] = make_float2(a1, a2);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int i = warp; i < ng; i += kGnClusterThreads / 32) {   // lane c: CTA c's sums
+        float u = 0.0f, v = 0.0f;
+        if (lane < s.ctas) {
+            uint32_t there;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                         : "=r"(there) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(sums + i))), "r"(lane));
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(u), "=f"(v) : "r"(there) : "memory");
+        }
+        double a1 = u, a2 = v;
+#pragma unroll
+        for (int m = 4; m; m >>= 1) {
+            a1 += __shfl_xor_sync(0xFFFFFFFFu, a1, m);
+            a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
+        }
+        if (lane == 0) {
+            const double inv = 1.0 / (static_cast<double>(a.positions) * a.width);
+            const double m = a1 * inv, var = a2 * inv - m * m;   // a non-finite value: NaN
+            stat[i] = make_float2(static_cast<float>(shifts[i] + m), 1.0f / sqrtf(static_cast<float>((var < 0.0 ? 0.0 : var) + a.eps)));
+        }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this CTA has read its peers' sums
+    __syncthreads();
+    const float2 st = stat[g];
+    T* yp = y + n * a.y_sample + ch0 + tx * VEC;
+    if (on)
+#pragma unroll 4
+        for (int r = 0; r < s.rounds; ++r) {
+            const int p = p0 + ty + r * s.ty;
+            if (p >= p1) break;
+            float v[VEC];
+            unpack_vec<T, VEC>(tile[r * kGnClusterThreads + tid], v);
+            gn_finish<VEC>(v, st.x, st.y, w, b, a.act);
+            store_vec<T, VEC>(yp + p * a.y_pos, v);
+        }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // no CTA leaves while a peer may read it
 }
 
 // ---- host ----------------------------------------------------------------
@@ -282,6 +509,36 @@ bool gn_small(const SslaGroupNorm* a, int vec, int* lps, int* ept) {
     return true;
 }
 
+size_t gn_cluster_bytes(const GnCluster& c, int vec, int sz) {
+    return static_cast<size_t>(c.rounds) * kGnClusterThreads * vec * sz + c.gpc * 5 * sizeof(float);
+}
+
+// The smallest cluster, of whole groups of at least 128 contiguous bytes,
+// whose slices fit and that gives (nearly) every SM a CTA; the widest that
+// fits where none does; false: a slab does not fit.
+bool gn_cluster(const SslaGroupNorm* a, int vec, GnCluster* c) {
+    const int wv = a->channels / a->groups / vec, sz = dtype_size(a->dtype);
+    if (wv > kGnClusterThreads || a->n > 65535) return false;
+    bool found = false;
+    for (int ctas = 1; ctas <= 8; ctas *= 2)
+        for (int parts = 1; parts <= 8; parts *= 2) {
+            GnCluster k;
+            k.ctas = ctas;
+            k.gpc = std::min((a->groups + parts - 1) / parts, kGnClusterThreads / wv);
+            if (parts > 1 && static_cast<long long>(k.gpc) * wv * vec * sz < 128) continue;
+            k.chunks = (a->groups + k.gpc - 1) / k.gpc;
+            if (k.chunks > 65535) continue;
+            k.tx = k.gpc * wv;
+            k.ty = kGnClusterThreads / k.tx;
+            k.rounds = ((a->positions + ctas - 1) / ctas + k.ty - 1) / k.ty;
+            if (k.rounds > kGnClusterBytes / (kGnClusterThreads * vec * sz)) continue;
+            found = true;
+            *c = k;
+            if (static_cast<long long>(a->n) * k.chunks * ctas >= 128 || k.rounds <= 2) return true;
+        }
+    return found;
+}
+
 GnSplit gn_split(const SslaGroupNorm* a, int vec) {
     GnSplit s;
     const int wv = a->channels / a->groups / vec;
@@ -300,8 +557,9 @@ size_t gn_bytes(const SslaGroupNorm* a) {
     if (a->n == 0 || a->positions == 0 || a->channels == 0) return 0;
     const int vec = gn_vec(a);
     int lps, ept;
-    if (gn_small(a, vec, &lps, &ept)) return 0;
-    return static_cast<size_t>(a->n) * a->groups * (gn_split(a, vec).splits + 1) * sizeof(float2);
+    GnCluster c;
+    if (gn_small(a, vec, &lps, &ept) || gn_cluster(a, vec, &c)) return 0;
+    return static_cast<size_t>(a->n) * a->groups * (gn_split(a, vec).splits * sizeof(float2) + sizeof(float));
 }
 
 }  // namespace
@@ -334,6 +592,8 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
     d.n = a->n; d.positions = a->positions; d.channels = a->channels; d.groups = a->groups;
     d.width = a->channels / a->groups;
     d.act = a->activation; d.eps = a->eps;
+    d.wide = aligned(a->weight, 16) && aligned(a->bias, 16);
+    d.shift = nullptr;
     const int vec = gn_vec(a);
     auto run = [&](auto t, auto v) {
         using T = decltype(t);
@@ -343,29 +603,65 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
         int lps, ept;
         const long long slabs = static_cast<long long>(a->n) * a->groups;
         if (gn_small(a, vec, &lps, &ept)) {
-            const unsigned grid = static_cast<unsigned>((slabs + kGnThreads / lps - 1) / (kGnThreads / lps));
-            auto go = [&](auto l, auto e) {
-                k_gn_slab<T, V, decltype(l)::value, decltype(e)::value><<<grid, kGnThreads, 0, st>>>(d, x, y);
+            auto go = [&](auto l, auto e, auto un) {
+                constexpr int LPS = decltype(l)::value, UNR = decltype(un)::value, kPer = kGnThreads / LPS;
+                // the resident CTAs, a multiple of what keeps a thread's group
+                const long long all = (slabs + kPer * UNR - 1) / (kPer * UNR);
+                const int turn = a->groups / std::gcd(a->groups, kPer);
+                long long grid = std::min<long long>(all, 148 * (LPS <= 32 ? kGnSlabCtas : 8));
+                if (grid > turn) grid -= grid % turn;
+                k_gn_slab<T, V, LPS, decltype(e)::value, UNR><<<static_cast<unsigned>(grid), kGnThreads, 0, st>>>(d, x, y);
                 return launched("k_gn_slab");
             };
             using std::integral_constant;
-            if (lps == 8) return go(integral_constant<int, 8>(), integral_constant<int, 1>());
-            if (lps == 16) return go(integral_constant<int, 16>(), integral_constant<int, 1>());
-            if (lps == 32 && ept == 1) return go(integral_constant<int, 32>(), integral_constant<int, 1>());
-            if (lps == 32 && ept == 2) return go(integral_constant<int, 32>(), integral_constant<int, 2>());
-            if (lps == 32) return go(integral_constant<int, 32>(), integral_constant<int, 4>());
-            return go(integral_constant<int, kGnThreads>(), integral_constant<int, (V >= 8 ? 4 : 8)>());
+            constexpr integral_constant<int, 1> one;
+            constexpr integral_constant<int, 2> two;
+            constexpr integral_constant<int, 4> four;
+            constexpr integral_constant<int, 32> warp;
+            if (lps == 8) return go(integral_constant<int, 8>(), one, two);
+            if (lps == 16) return go(integral_constant<int, 16>(), one, two);
+            if (lps == 32 && ept == 1) return go(warp, one, two);
+            if (lps == 32 && ept == 2) return go(warp, two, two);
+            if (lps == 32) return go(warp, four, one);
+            return go(integral_constant<int, kGnThreads>(), integral_constant<int, (V >= 8 ? 4 : 8)>(), one);
+        }
+        GnCluster c;
+        if (gn_cluster(a, vec, &c)) {
+            const size_t bytes = gn_cluster_bytes(c, V, sizeof(T));
+            allow_smem<k_gn_cluster<T, V>>(kGnClusterBytes + 5 * kGnClusterThreads * static_cast<int>(sizeof(float)));
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute at;
+            at.id = cudaLaunchAttributeClusterDimension;
+            at.val.clusterDim.x = c.ctas;
+            at.val.clusterDim.y = at.val.clusterDim.z = 1;
+            cfg.gridDim = dim3(c.ctas, c.chunks, a->n);
+            cfg.blockDim = dim3(kGnClusterThreads);
+            cfg.dynamicSmemBytes = bytes;
+            cfg.stream = st;
+            cfg.attrs = &at;
+            cfg.numAttrs = 1;
+            cudaLaunchKernelEx(&cfg, k_gn_cluster<T, V>, d, c, x, y);
+            return launched("k_gn_cluster");
         }
         const GnSplit s = gn_split(a, vec);
-        float2* stat = static_cast<float2*>(workspace);
-        float2* part = stat + slabs;
-        if (s.chunks > 65535 || a->n > 65535) {
-            return fail(SSLA_ERR_ARG, "group norm: more than 65535 samples or groups of large slabs");
-        }
+        if (s.chunks > 65535 || a->n > 65535)
+            return fail(SSLA_ERR_ARG, "group norm: more than 65535 samples or group chunks of large slabs");
+        float2* part = static_cast<float2*>(workspace);
+        d.shift = reinterpret_cast<float*>(part + static_cast<size_t>(slabs) * s.splits);
         const dim3 grid(s.splits, s.chunks, a->n);
         k_gn_sums<T, V><<<grid, kGnThreads, 0, st>>>(d, s, x, part);
-        k_gn_stats<T, V><<<static_cast<unsigned>((slabs + 7) / 8), kGnThreads, 0, st>>>(d, s.splits, x, part, stat);
-        k_gn_apply<T, V><<<grid, kGnThreads, 0, st>>>(d, s, x, y, stat);
+        // the second launch's latency passes under the first kernel
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute at;
+        at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at.val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(kGnThreads);
+        cfg.dynamicSmemBytes = s.gpc * sizeof(float2);
+        cfg.stream = st;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, k_gn_apply<T, V>, d, s, x, y, static_cast<const float2*>(part));
         return launched("group norm");
     };
     auto by_vec = [&](auto t) {

@@ -574,10 +574,10 @@ int chunk_launch(const LinArgs& a, int dtype, const std::vector<Seq>& seqs, void
         const int rc = with_shape(dtype, a.dk, a.dv, [&](auto t, auto k, auto v) {
             using T = decltype(t);
             constexpr int K = decltype(k)::value, V = decltype(v)::value, bytes = Tile<T, K, V>::bytes;
-            cudaFuncSetAttribute(k_chunk<T, K, V, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            allow_smem<k_chunk<T, K, V, true>>(bytes);
             const dim3 grid((a.dv + V - 1) / V, a.heads, nseg);
             if (divided) {
-                cudaFuncSetAttribute(k_chunk<T, K, V, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+                allow_smem<k_chunk<T, K, V, false>>(bytes);
                 k_chunk<T, K, V, false><<<grid, kThreads, bytes, st>>>(a, tab, states, decays, wides);
                 k_chunk_join<<<dim3((a.dk * a.dv + 255) / 256, a.heads, tab.n), 256, 0, st>>>(a, tab, states, decays);
             }

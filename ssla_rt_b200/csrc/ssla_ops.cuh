@@ -6,9 +6,11 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <cstring>
 #include <string>
 
 #include "ssla_b200.h"
@@ -38,9 +40,12 @@ inline int fail(int code, const char* fmt, ...) noexcept {
 struct OnDevice {
     int prev = -1, err = SSLA_OK;
     explicit OnDevice(int dev) noexcept {
-        int n = 0;
-        if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
-            cudaGetLastError();
+        static const int n = [] {                  // fixed for the process
+            int c = 0;
+            if (cudaGetDeviceCount(&c) != cudaSuccess) cudaGetLastError(), c = 0;
+            return c;
+        }();
+        if (n == 0) {
             err = fail(SSLA_ERR_NO_DEVICE, "no CUDA device");
             return;
         }
@@ -63,6 +68,17 @@ struct OnDevice {
 inline int launched(const char* what) noexcept {
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? SSLA_OK : fail(SSLA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+// Raises a kernel's dynamic shared memory limit, once per device.
+template <auto K> inline void allow_smem(int bytes) noexcept {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return;
+    cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 inline bool dtype_ok(int dt) { return dt == SSLA_DT_F32 || dt == SSLA_DT_BF16 || dt == SSLA_DT_F16; }
@@ -88,17 +104,57 @@ template <> __device__ __forceinline__ __half from_f<__half>(float x) { return _
 // V consecutive values at p (aligned to V * sizeof(T)) as floats, and back.
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
+// Two 16-bit values as floats, and back (one rounding each).
+template <typename T> __device__ __forceinline__ float2 unpack16(uint32_t u);
+template <> __device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+}
+template <> __device__ __forceinline__ float2 unpack16<__half>(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack16(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <> __device__ __forceinline__ uint32_t pack16<__half>(float x, float y) {
+    const __half2 p = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack_vec(const Pack<T, V>& k, float (&x)[V]) {
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+        uint32_t u[V / 2];
+        memcpy(u, &k, sizeof u);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 f = unpack16<T>(u[i]);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = to_f<T>(k.v[i]);
+    }
+}
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(const T* p, float (&x)[V]) {
     const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = to_f<T>(k.v[i]);
+    unpack_vec<T, V>(k, x);
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[V]) {
     Pack<T, V> k;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+        uint32_t u[V / 2];
 #pragma unroll
-    for (int i = 0; i < V; ++i) k.v[i] = from_f<T>(x[i]);
+        for (int i = 0; i < V / 2; ++i) u[i] = pack16<T>(x[2 * i], x[2 * i + 1]);
+        memcpy(&k, u, sizeof u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) k.v[i] = from_f<T>(x[i]);
+    }
     *reinterpret_cast<Pack<T, V>*>(p) = k;
 }
 

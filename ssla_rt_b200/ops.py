@@ -28,15 +28,40 @@ _FORMATS = {torch.int8: abi.FMT_INT8, torch.float8_e4m3fn: abi.FMT_E4M3}
 _ACTIVATIONS = {"none": abi.ACT_NONE, None: abi.ACT_NONE, "silu": abi.ACT_SILU}
 
 
+# What a call's shapes, strides, types and device decide -- its checks and the
+# filled argument block -- is kept by exactly those, so that a repeated call
+# only sets its pointers (the C entry checks those every time).
+_PLANS: dict = {}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _sig(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _plan(key, make):
+    p = _PLANS.get(key)
+    if p is None:
+        p = make()
+        if len(_PLANS) >= 4096:
+            _PLANS.clear()
+        _PLANS[key] = p
+    return p
+
+
+def _no_grad(*tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("inference only: an input requires a gradient")
+
+
 def _device(first: torch.Tensor, **others) -> int:
     """The CUDA device index that every given tensor is on."""
     dev = first.device
     for name, t in others.items():
         if t is not None and t.device != dev:
             raise ValueError(f"{name} is on {t.device}, not {dev}")
-    if torch.is_grad_enabled() and (first.requires_grad or
-                                    any(t is not None and t.requires_grad for t in others.values())):
-        raise ValueError("inference only: an input requires a gradient")
     if dev.type != "cuda":
         raise ValueError(f"CUDA tensors are needed, got {dev}")
     return dev.index
@@ -45,6 +70,8 @@ def _device(first: torch.Tensor, **others) -> int:
 def _stream_of(stream, device: int):
     """(handle to launch on, torch stream to allocate and synchronise with, or None for the current one)."""
     if stream is None:
+        if _raw_stream is not None:
+            return _raw_stream(device), None
         return torch.cuda.current_stream(device).cuda_stream, None
     if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=device)
@@ -60,13 +87,20 @@ def _keep(ts, *tensors) -> None:
                 t.record_stream(ts)
 
 
-def _empty(shape, dtype, device: int, stream, zero: bool = False) -> torch.Tensor:
-    """A new tensor that belongs to the launch's stream."""
-    make = torch.zeros if zero else torch.empty
+def _like(x: torch.Tensor, stream, zero: bool = False) -> torch.Tensor:
+    """A new contiguous tensor of x's shape that belongs to the launch's stream."""
+    make = torch.zeros_like if zero else torch.empty_like
     if stream is None:
-        return make(shape, dtype=dtype, device=f"cuda:{device}")
+        return make(x, memory_format=torch.contiguous_format)
     with torch.cuda.stream(stream):
-        return make(shape, dtype=dtype, device=f"cuda:{device}")
+        return make(x, memory_format=torch.contiguous_format)
+
+
+def _new(x: torch.Tensor, shape, dtype, stream) -> torch.Tensor:
+    if stream is None:
+        return x.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        return x.new_empty(shape, dtype=dtype)
 
 
 def _rows_heads(name: str, t: torch.Tensor, dtype=None) -> None:
@@ -84,6 +118,8 @@ def _host_ints(name: str, x) -> np.ndarray:
         if x.device.type != "cpu":
             raise ValueError(f"{name} is a host array")
         x = x.numpy()
+    if type(x) is np.ndarray and x.dtype == np.int32 and x.ndim == 1 and x.flags.c_contiguous:
+        return x
     a = np.asarray(x)
     if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
         raise ValueError(f"{name} is a one-dimensional array of integers")
@@ -103,8 +139,8 @@ def _device_slots(slots: Optional[torch.Tensor], n: int) -> None:
         raise ValueError(f"slots has shape {tuple(slots.shape)}: {n} contiguous entries are needed")
 
 
-def _linattn(q, k, v, decay, state, scale, out):
-    """Checks what both forms share; the filled argument block without out, and the device."""
+def _linattn_block(q, k, v, decay, state, scale, out, step_slots=None):
+    """Checks what both forms share; the argument block without its pointers."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         _rows_heads(name, t, v.dtype)
     if v.dtype not in _DTYPES:
@@ -121,14 +157,16 @@ def _linattn(q, k, v, decay, state, scale, out):
             raise ValueError(f"state is {state.dtype} {tuple(state.shape)}: float32 (slots, {heads}, {dk}, {dv}) is needed")
         if not state.is_contiguous():
             raise ValueError("state is not contiguous")
-        a.state = state.data_ptr()
         a.n_slots = state.shape[0]
     if out is not None:
         _rows_heads("out", out, v.dtype)
         if out.shape != v.shape:
             raise ValueError(f"out has shape {tuple(out.shape)}, not {tuple(v.shape)}")
-    a.device = _device(q, k=k, v=v, decay=decay, state=state, out=out)
-    a.q, a.k, a.v, a.decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr()
+        a.out_row, a.out_head, _ = out.stride()
+    else:
+        a.out_row, a.out_head = heads * dv, dv
+    _device_slots(step_slots, n)
+    a.device = _device(q, k=k, v=v, decay=decay, state=state, out=out, slots=step_slots)
     a.q_row, a.q_head, _ = q.stride()
     a.k_row, a.k_head, _ = k.stride()
     a.v_row, a.v_head, _ = v.stride()
@@ -142,9 +180,18 @@ def _linattn(q, k, v, decay, state, scale, out):
     return a
 
 
-def _set_out(a: "abi.SslaLinAttn", out: torch.Tensor) -> None:
-    a.out = out.data_ptr()
-    a.out_row, a.out_head, _ = out.stride()
+def _linattn(q, k, v, decay, state, scale, out, slots=None):
+    """The checked argument block of a call with every pointer but out's."""
+    _no_grad(q, k, v, decay, state)
+    key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(),
+           v.shape, v.stride(), v.dtype, v.get_device(), decay.shape, decay.stride(), decay.dtype, decay.get_device(),
+           scale, _sig(state), _sig(out), _sig(slots))
+    a = abi.SslaLinAttn.from_buffer_copy(
+        _plan(key, lambda: _linattn_block(q, k, v, decay, state, scale, out, slots)))
+    a.q, a.k, a.v, a.decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr()
+    if state is not None:
+        a.state = state.data_ptr()
+    return a
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, *,
@@ -192,16 +239,17 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     a = _linattn(q, k, v, decay, state, scale, out)
     handle, ts = _stream_of(stream, a.device)
     if out is None:
-        out = _empty(v.shape, v.dtype, a.device, ts, zero=gaps)
-    _set_out(a, out)
+        out = _like(v, ts, zero=gaps)
+    a.out = out.data_ptr()
     lib = load_library()
     po, pl = off.ctypes.data, lengths.ctypes.data if lengths is not None else None
     need = C.c_size_t()
     _check(lib.ssla_linattn_chunk_workspace(C.byref(a), po, pl, n_seq, C.byref(need)))
-    ws = _empty((need.value,), torch.uint8, a.device, ts) if need.value else None
+    ws = _new(v, (need.value,), torch.uint8, ts) if need.value else None
     _check(lib.ssla_linattn_chunk(C.byref(a), po, pl, slots.ctypes.data if slots is not None else None, n_seq,
                                   ws.data_ptr() if ws is not None else None, need.value, handle))
-    _keep(ts, q, k, v, decay, state, out)
+    if ts is not None:
+        _keep(ts, q, k, v, decay, state, out)
     return out
 
 
@@ -216,18 +264,18 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dec
     Rows that name the same slot are applied in row order; a slot outside the
     state marks a padding row: zero output, no state touched.
     """
-    _device_slots(slots, v.shape[0])
     if state is None:
         raise ValueError("state is needed")
-    a = _linattn(q, k, v, decay, state, scale, out)
-    if slots is not None and slots.device != v.device:
-        raise ValueError(f"slots is on {slots.device}, not {v.device}")
+    if slots is not None and not isinstance(slots, torch.Tensor):
+        raise ValueError("slots is a one-dimensional int32 tensor")
+    a = _linattn(q, k, v, decay, state, scale, out, slots)
     handle, ts = _stream_of(stream, a.device)
     if out is None:
-        out = _empty(v.shape, v.dtype, a.device, ts)
-    _set_out(a, out)
+        out = _like(v, ts)
+    a.out = out.data_ptr()
     _check(load_library().ssla_linattn_step(C.byref(a), slots.data_ptr() if slots is not None else None, handle))
-    _keep(ts, q, k, v, decay, state, slots, out)
+    if ts is not None:
+        _keep(ts, q, k, v, decay, state, slots, out)
     return out
 
 
@@ -242,7 +290,8 @@ def state_cache(n_slots: int, rows: int, cols: int, *, block: int = 64, dtype: t
     return codes, torch.zeros((n_slots, rows, -(-cols // block)), dtype=torch.float32, device=device)
 
 
-def _cache(codes, scales, block, slots, n):
+def _cache_block(codes, scales, block, slots, n, name, x, dtype):
+    """Checks a store or load; the argument block without its pointers."""
     if codes.dtype not in _FORMATS or codes.dim() != 3 or not codes.is_contiguous():
         raise ValueError("codes is a contiguous (slots, rows, cols) tensor of int8 or float8_e4m3fn")
     if not 1 <= block <= 256:
@@ -254,22 +303,35 @@ def _cache(codes, scales, block, slots, n):
                          f"({n_slots}, {rows}, {-(-cols // block)}) is needed")
     _device_slots(slots, n)
     c = abi.SslaStateCache()
-    c.codes, c.scales = codes.data_ptr(), scales.data_ptr()
-    if slots is not None:
-        c.slots = slots.data_ptr()
     c.n, c.n_slots, c.rows, c.cols, c.block = n, n_slots, rows, cols, block
     c.format = _FORMATS[codes.dtype]
+    if x is not None:
+        if x.dtype not in _DTYPES or x.dim() != 3 or tuple(x.shape[1:]) != (rows, cols):
+            raise ValueError(f"{name} is {x.dtype} {tuple(x.shape)}: (states, {rows}, {cols}) of float32, bfloat16 "
+                             f"or float16 is needed")
+        if cols > 1 and x.stride(2) != 1:
+            raise ValueError(f"{name}'s last dimension is not contiguous")
+        c.x_state, c.x_row, _ = x.stride()
+    else:
+        c.x_state, c.x_row = rows * cols, cols
+    if dtype not in _DTYPES:
+        raise ValueError(f"{dtype} is not supported: float32, bfloat16 or float16")
+    c.dtype = _DTYPES[dtype]
+    c.device = _device(codes, scales=scales, slots=slots, **{name: x})
     return c
 
 
-def _cache_x(c: "abi.SslaStateCache", name: str, x: torch.Tensor) -> None:
-    if x.dtype not in _DTYPES or x.dim() != 3 or tuple(x.shape[1:]) != (c.rows, c.cols):
-        raise ValueError(f"{name} is {x.dtype} {tuple(x.shape)}: (states, {c.rows}, {c.cols}) of float32, bfloat16 "
-                         f"or float16 is needed")
-    if c.cols > 1 and x.stride(2) != 1:
-        raise ValueError(f"{name}'s last dimension is not contiguous")
-    c.dtype = _DTYPES[x.dtype]
-    c.x_state, c.x_row, _ = x.stride()
+def _cache(codes, scales, block, slots, n, name, x, dtype):
+    if slots is not None and not isinstance(slots, torch.Tensor):
+        raise ValueError("slots is a one-dimensional int32 tensor")
+    _no_grad(x, scales)
+    key = ("cache", _sig(codes), _sig(scales), block, _sig(slots), n, name, _sig(x), dtype)
+    c = abi.SslaStateCache.from_buffer_copy(
+        _plan(key, lambda: _cache_block(codes, scales, block, slots, n, name, x, dtype)))
+    c.codes, c.scales = codes.data_ptr(), scales.data_ptr()
+    if slots is not None:
+        c.slots = slots.data_ptr()
+    return c
 
 
 def state_store(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, block: int = 64,
@@ -284,12 +346,11 @@ def state_store(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, b
     is named twice the last state is kept; other slots stay as they were.  A
     block with a non-finite value reads back as NaN.
     """
-    c = _cache(codes, scales, block, slots, x.shape[0])
-    _cache_x(c, "x", x)
-    c.device = _device(x, codes=codes, scales=scales, slots=slots)
+    c = _cache(codes, scales, block, slots, x.shape[0], "x", x, x.dtype)
     handle, ts = _stream_of(stream, c.device)
     _check(load_library().ssla_state_store(C.byref(c), x.data_ptr(), handle))
-    _keep(ts, x, codes, scales, slots)
+    if ts is not None:
+        _keep(ts, x, codes, scales, slots)
 
 
 def state_load(codes: torch.Tensor, scales: torch.Tensor, *, block: int = 64, slots: Optional[torch.Tensor] = None,
@@ -301,36 +362,17 @@ def state_load(codes: torch.Tensor, scales: torch.Tensor, *, block: int = 64, sl
         n, dtype = out.shape[0], out.dtype
     else:
         n = slots.shape[0] if slots is not None else codes.shape[0]
-    if dtype not in _DTYPES:
-        raise ValueError(f"{dtype} is not supported: float32, bfloat16 or float16")
-    c = _cache(codes, scales, block, slots, n)
-    if out is not None:
-        _cache_x(c, "out", out)
-    c.device = _device(codes, scales=scales, slots=slots, out=out)
+    c = _cache(codes, scales, block, slots, n, "out", out, dtype)
     handle, ts = _stream_of(stream, c.device)
     if out is None:
-        out = _empty((n, c.rows, c.cols), dtype, c.device, ts)
-        _cache_x(c, "out", out)
+        out = _new(codes, (n, c.rows, c.cols), dtype, ts)
     _check(load_library().ssla_state_load(C.byref(c), out.data_ptr(), handle))
-    _keep(ts, codes, scales, slots, out)
+    if ts is not None:
+        _keep(ts, codes, scales, slots, out)
     return out
 
 
-def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None,
-               bias: Optional[torch.Tensor] = None, *, eps: float = 1e-5, activation: Optional[str] = "silu",
-               out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
-    """Group norm with an activation, channels last.
-
-    x: (samples, positions, channels), channels contiguous, any other strides;
-    (rows, channels) is rows of one position each, so that with one group per
-    head it normalises linear_attention's output rows.  Statistics over a
-    sample's positions and the channels of a group; weight, bias: (channels,)
-    float32.  activation: "silu" or "none".  ``out`` may be x.
-    """
-    if x.dim() == 2:
-        y = group_norm(x[:, None], groups, weight, bias, eps=eps, activation=activation,
-                       out=None if out is None else out[:, None], stream=stream)
-        return y[:, 0] if out is None else out
+def _norm_block(x, groups, weight, bias, eps, activation, out):
     if x.dtype not in _DTYPES or x.dim() != 3:
         raise ValueError(f"x is {x.dtype} {tuple(x.shape)}: (samples, positions, channels) or (rows, channels) of "
                          f"float32, bfloat16 or float16 is needed")
@@ -349,20 +391,48 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, x {x.dtype} {tuple(x.shape)}")
     a = abi.SslaGroupNorm()
     a.device = _device(x, weight=weight, bias=bias, out=out)
-    handle, ts = _stream_of(stream, a.device)
-    if out is None:
-        out = _empty(x.shape, x.dtype, a.device, ts)
-    a.x, a.y = x.data_ptr(), out.data_ptr()
-    a.weight = weight.data_ptr() if weight is not None else None
-    a.bias = bias.data_ptr() if bias is not None else None
     a.x_sample, a.x_pos, _ = x.stride()
-    a.y_sample, a.y_pos, _ = out.stride()
+    if out is not None:
+        a.y_sample, a.y_pos, _ = out.stride()
+    else:
+        a.y_sample, a.y_pos = positions * channels, channels
     a.n, a.positions, a.channels, a.groups = n, positions, channels, groups
     a.dtype, a.activation, a.eps = _DTYPES[x.dtype], _ACTIVATIONS[activation], eps
+    return a
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, *, eps: float = 1e-5, activation: Optional[str] = "silu",
+               out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """Group norm with an activation, channels last.
+
+    x: (samples, positions, channels), channels contiguous, any other strides;
+    (rows, channels) is rows of one position each, so that with one group per
+    head it normalises linear_attention's output rows.  Statistics over a
+    sample's positions and the channels of a group; weight, bias: (channels,)
+    float32.  activation: "silu" or "none".  ``out`` may be x.
+    """
+    if x.dim() == 2:
+        y = group_norm(x[:, None], groups, weight, bias, eps=eps, activation=activation,
+                       out=None if out is None else out[:, None], stream=stream)
+        return y[:, 0] if out is None else out
+    _no_grad(x, weight, bias)
+    key = ("norm", _sig(x), groups, _sig(weight), _sig(bias), eps, activation, _sig(out))
+    a = abi.SslaGroupNorm.from_buffer_copy(
+        _plan(key, lambda: _norm_block(x, groups, weight, bias, eps, activation, out)))
+    handle, ts = _stream_of(stream, a.device)
+    if out is None:
+        out = _like(x, ts)
+    a.x, a.y = x.data_ptr(), out.data_ptr()
+    if weight is not None:
+        a.weight = weight.data_ptr()
+    if bias is not None:
+        a.bias = bias.data_ptr()
     lib = load_library()
     need = C.c_size_t()
     _check(lib.ssla_group_norm_workspace(C.byref(a), C.byref(need)))
-    ws = _empty((need.value,), torch.uint8, a.device, ts) if need.value else None
+    ws = _new(x, (need.value,), torch.uint8, ts) if need.value else None
     _check(lib.ssla_group_norm(C.byref(a), ws.data_ptr() if ws is not None else None, need.value, handle))
-    _keep(ts, x, weight, bias, out)
+    if ts is not None:
+        _keep(ts, x, weight, bias, out)
     return out
