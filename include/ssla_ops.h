@@ -64,6 +64,12 @@ int ssla_linattn_chunk(const SslaLinAttn* a, const int* offsets, const int* leng
 int ssla_linattn_chunk_workspace(const SslaLinAttn* a, const int* offsets, const int* lengths, int n_seq,
                                  size_t* bytes);
 
+/* Status bits of the chunked form's kernels on `device` since the last call
+ * (0: fine).  SSLA_LINATTN_TIMED_OUT: a bounded wait inside a kernel ran out,
+ * and what the calls since wrote is not valid.  Synchronises the device. */
+enum { SSLA_LINATTN_TIMED_OUT = 1 };
+int ssla_linattn_status(int device, unsigned* status);
+
 /* Recurrent form: one token per row.  Row r updates state slot slots[r]
  * (device array; NULL: slot r, n_rows <= n_slots).  Rows that name the same
  * slot are applied in row order.  A slot outside [0, n_slots) marks a padding

@@ -155,7 +155,7 @@ class SslaGroupNorm(C.Structure):
 
 # Every symbol include/ssla_ops.h declares.
 OPS_EXPORTED = (
-    "ssla_linattn_chunk", "ssla_linattn_chunk_workspace", "ssla_linattn_step",
+    "ssla_linattn_chunk", "ssla_linattn_chunk_workspace", "ssla_linattn_step", "ssla_linattn_status",
     "ssla_state_store", "ssla_state_load", "ssla_group_norm", "ssla_group_norm_workspace",
 )
 DT_F32, DT_BF16, DT_F16 = range(3)

@@ -322,4 +322,11 @@ int ssla_linattn_chunk(const SslaLinAttn* a, const int* offsets, const int* leng
     }
 }
 
+int ssla_linattn_status(int device, unsigned* status) {
+    if (!status) return fail(SSLA_ERR_ARG, "linear attention status: null argument");
+    OnDevice dev(device);
+    if (dev.err != SSLA_OK) return dev.err;
+    return chunk_status(status);
+}
+
 }  // extern "C"

@@ -27,5 +27,7 @@ struct Seq {
 size_t chunk_workspace(const LinArgs& a, int dtype, const std::vector<Seq>& seqs);
 int chunk_launch(const LinArgs& a, int dtype, const std::vector<Seq>& seqs, void* workspace, cudaStream_t st);
 
+int chunk_status(unsigned* bits);
+
 }  // namespace ops
 }  // namespace ssla

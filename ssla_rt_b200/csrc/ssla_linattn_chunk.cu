@@ -164,6 +164,46 @@ __device__ __forceinline__ void state_store2(float* p, int r, int c, int dk, int
     }
 }
 
+// The log decays of tokens 2 lane and 2 lane + 1 of a chunk (0 from token n on).
+__device__ __forceinline__ float2 chunk_decay_values(const LinArgs& a, long long row, int n, int h, int lane) {
+    const float* p = a.decay + row * a.decay_row + h * a.decay_head;
+    const int t = 2 * lane;
+    return make_float2(t < n ? p[t * a.decay_row] : 0.0f, t + 1 < n ? p[(t + 1) * a.decay_row] : 0.0f);
+}
+
+// A chunk's decay sums, by one warp: G_t = sum of the log2 decays up to token
+// t as (hi, lo), 2^{G_t}, 2^{G_C - G_t}, 2^{G_C}.  The sums are taken in 64
+// bits: differences of them are exponents below.  Returns G_C.
+__device__ __forceinline__ double chunk_decays(float2 g, int lane, float* ghi, float* glo, float* eg, float* wk, float* gam) {
+    double s[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        float x = j ? g.y : g.x;
+        if (x < -1e5f) x = -1e5f;                           // e^-1e5 is 0 as well, and -inf - -inf is not
+        s[j] = x * 1.4426950408889634;
+    }
+    s[1] += s[0];
+    double run = s[1];
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        const double o = __shfl_up_sync(0xFFFFFFFFu, run, m);
+        if (lane >= m) run += o;
+    }
+    const double all = __shfl_sync(0xFFFFFFFFu, run, 31), before = run - s[1];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int t = 2 * lane + j;
+        const double G = j ? run : before + s[0];
+        const float x = static_cast<float>(G);
+        ghi[t] = x;
+        glo[t] = static_cast<float>(G - x);
+        eg[t] = exp2f(x);
+        wk[t] = exp2f(static_cast<float>(all - G));
+    }
+    if (lane == 0) gam[0] = exp2f(static_cast<float>(all));
+    return all;
+}
+
 // Segment states: [segment][head][dk][dv]; segment decays: [segment][head].
 template <typename T, int DK, int DV, bool OUT>
 __global__ void __launch_bounds__(kThreads)
@@ -242,35 +282,7 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
                 }
         }
         if (warp == 0) {
-            // inclusive sums of the log2 decays, in 64 bits: differences of them are exponents below
-            double s[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int t = 2 * lane + j;
-                float x = t < n ? a.decay[(row + t) * a.decay_row + h * a.decay_head] : 0.0f;
-                if (x < -1e5f) x = -1e5f;                   // e^-1e5 is 0 as well, and -inf - -inf is not
-                s[j] = x * 1.4426950408889634;
-            }
-            s[1] += s[0];
-            double run = s[1];
-#pragma unroll
-            for (int m = 1; m < 32; m <<= 1) {
-                const double o = __shfl_up_sync(0xFFFFFFFFu, run, m);
-                if (lane >= m) run += o;
-            }
-            const double all = __shfl_sync(0xFFFFFFFFu, run, 31), before = run - s[1];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int t = 2 * lane + j;
-                const double G = j ? run : before + s[0];
-                const float x = static_cast<float>(G);
-                ghi[t] = x;
-                glo[t] = static_cast<float>(G - x);
-                eg[t] = exp2f(x);
-                wk[t] = exp2f(static_cast<float>(all - G));
-            }
-            if (lane == 0) gam[0] = exp2f(static_cast<float>(all));
-            total += all;
+            total += chunk_decays(chunk_decay_values(a, row, n, h, lane), lane, ghi, glo, eg, wk, gam);
         }
         any = __syncthreads_or(any);
 
@@ -457,6 +469,8 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
     if (!OUT && blockIdx.x == 0 && tid == 0) seg_decay[static_cast<size_t>(blockIdx.z) * a.heads + h] = total;
 }
 
+#include "ssla_linattn_tc.cuh"
+
 // Chains a sequence's segments: segment i's place in the workspace becomes
 // the state after it.  One thread per state element.
 __global__ void __launch_bounds__(256)
@@ -468,16 +482,28 @@ k_chunk_join(LinArgs a, const __grid_constant__ Table tab, float* seg_state, con
     const size_t head_state = static_cast<size_t>(a.dk) * a.dv;
     const int slot = tab.slot[seq];
     float run = slot >= 0 ? a.state[(static_cast<size_t>(slot) * a.heads + h) * head_state + e] : 0.0f;
-    for (int s = s0; s < s1; ++s) {
-        float* p = seg_state + (static_cast<size_t>(s) * a.heads + h) * head_state + e;
-        run = fmaf(exp2f(static_cast<float>(seg_decay[static_cast<size_t>(s) * a.heads + h])), run, *p);
-        *p = run;
+    for (int s = s0; s < s1; s += 8) {
+        float x[8], g[8];                                   // loads of eight segments in flight
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (s + i < s1) {
+                x[i] = seg_state[(static_cast<size_t>(s + i) * a.heads + h) * head_state + e];
+                g[i] = exp2f(static_cast<float>(seg_decay[static_cast<size_t>(s + i) * a.heads + h]));
+            }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (s + i < s1) {
+                run = fmaf(g[i], run, x[i]);
+                seg_state[(static_cast<size_t>(s + i) * a.heads + h) * head_state + e] = run;
+            }
     }
 }
 
 // ---- host ------------------------------------------------------------------
 struct Shape {
     int dk, dv, ctas;               // tile and resident CTAs per SM
+    bool tc;                        // the tcgen05 form
+    int cost;                       // a divided sequence's time over a whole one's, percent
 };
 
 template <typename F> auto with_shape(int dtype, int dk, int dv, F&& f) {
@@ -493,29 +519,49 @@ template <typename F> auto with_shape(int dtype, int dk, int dv, F&& f) {
     return dtype == SSLA_DT_F32 ? by_dv(float()) : dtype == SSLA_DT_BF16 ? by_dv(__nv_bfloat16()) : by_dv(__half());
 }
 
-Shape shape_of(int dtype, int dk, int dv) {
-    return with_shape(dtype, dk, dv, [](auto t, auto k, auto v) {
+// Which inputs allow 16-byte loads: bits 1 q, 2 k, 4 v.
+int wide_inputs(const LinArgs& a, int dtype) {
+    const int lanes = 16 / dtype_size(dtype);
+    auto wide = [&](const void* p, long long row, long long head) {
+        return aligned(p, 16) && row % lanes == 0 && head % lanes == 0;
+    };
+    return (wide(a.q, a.q_row, a.q_head) ? 1 : 0) | (wide(a.k, a.k_row, a.k_head) ? 2 : 0) |
+           (wide(a.v, a.v_row, a.v_head) ? 4 : 0);
+}
+
+Shape shape_of(const LinArgs& a, int dtype) {
+    // bf16 with wide heads: the tcgen05 form, whose copies are 16 bytes wide
+    if (dtype == SSLA_DT_BF16 && a.dk > 32 && a.dv > 32 && wide_inputs(a, dtype) == 7)
+        return Shape{a.dk <= 64 ? 64 : 128, 128, 1, true, 155};
+    return with_shape(dtype, a.dk, a.dv, [](auto t, auto k, auto v) {
         constexpr int K = decltype(k)::value, V = decltype(v)::value;
         const int bytes = Tile<decltype(t), K, V>::bytes;
-        return Shape{K, V, std::max(1, std::min(K * V >= 128 * 64 ? 2 : 4, (227 * 1024) / (bytes + 1024)))};
+        return Shape{K, V, std::max(1, std::min(K * V >= 128 * 64 ? 2 : 4, (227 * 1024) / (bytes + 1024))), false, 145};
     });
 }
 
-// Tokens of a segment for sequences [i0, i1): whole sequences where they fill
-// the GPU, else segments such that all resident CTAs have one.  A divided
-// sequence costs its keys and values a second pass (about 0.45 of the work).
+// Tokens of a segment for sequences [i0, i1).  Undivided, the longest sequence
+// bounds the time; divided, all resident CTAs share the work, but keys and
+// values pass twice (`cost`) and a last round of CTAs is half empty.
 int segment_tokens(const LinArgs& a, const Shape& sh, const std::vector<Seq>& seqs, size_t i0, size_t i1) {
-    long long chunks = 0, longest = 0, per = static_cast<long long>(a.heads) * ((a.dv + sh.dv - 1) / sh.dv);
+    const long long per = static_cast<long long>(a.heads) * ((a.dv + sh.dv - 1) / sh.dv), slots = 148LL * sh.ctas;
+    long long longest = 0, all = 0;
     for (size_t i = i0; i < i1; ++i) {
         const long long n = (seqs[i].len + kChunk - 1LL) / kChunk;
-        chunks += n;
         longest = std::max(longest, n);
+        all += n;
     }
-    const long long slots = 148LL * sh.ctas;
-    const long long whole = std::max(longest, (chunks * per + slots - 1) / slots);
-    const long long step = std::max(4LL, (chunks * per + slots - 1) / slots);
-    if (whole * 100 <= step * 145 || step >= longest) return INT_MAX / 2 / kChunk * kChunk;
-    return static_cast<int>(step * kChunk);
+    const long long share = (all * per + slots - 1) / slots;
+    long long best = longest, best_time = std::max(longest, share) * 100;
+    for (int parts = 2; parts <= 512; parts += parts < 32 ? 1 : parts / 16) {
+        const long long step = (longest + parts - 1) / parts;
+        if (step < 4) break;
+        long long ctas = 0;
+        for (size_t i = i0; i < i1; ++i) ctas += ((seqs[i].len + kChunk - 1LL) / kChunk + step - 1) / step * per;
+        const long long time = (std::max(step, share) + (ctas > slots ? step / 2 : 0)) * sh.cost;
+        if (time < best_time) best = step, best_time = time;
+    }
+    return static_cast<int>(best == longest ? INT_MAX / 2 / kChunk * kChunk : best * kChunk);
 }
 
 int segments(const Seq& s, int tokens) { return s.len ? (s.len - 1) / tokens + 1 : 0; }
@@ -526,7 +572,7 @@ size_t group_end(const std::vector<Seq>& seqs, size_t i0) { return std::min(seqs
 }  // namespace
 
 size_t chunk_workspace(const LinArgs& a, int dtype, const std::vector<Seq>& seqs) {
-    const Shape sh = shape_of(dtype, a.dk, a.dv);
+    const Shape sh = shape_of(a, dtype);
     size_t most = 0;
     for (size_t i0 = 0; i0 < seqs.size(); i0 = group_end(seqs, i0)) {
         const size_t i1 = group_end(seqs, i0);
@@ -543,13 +589,8 @@ size_t chunk_workspace(const LinArgs& a, int dtype, const std::vector<Seq>& seqs
 }
 
 int chunk_launch(const LinArgs& a, int dtype, const std::vector<Seq>& seqs, void* workspace, cudaStream_t st) {
-    const Shape sh = shape_of(dtype, a.dk, a.dv);
-    const int esz = dtype_size(dtype), lanes = 16 / esz;
-    auto wide = [&](const void* p, long long row, long long head) {
-        return aligned(p, 16) && row % lanes == 0 && head % lanes == 0;
-    };
-    const int wides = (wide(a.q, a.q_row, a.q_head) ? 1 : 0) | (wide(a.k, a.k_row, a.k_head) ? 2 : 0) |
-                      (wide(a.v, a.v_row, a.v_head) ? 4 : 0);
+    const Shape sh = shape_of(a, dtype);
+    const int wides = wide_inputs(a, dtype);
     for (size_t i0 = 0; i0 < seqs.size(); i0 = group_end(seqs, i0)) {
         const size_t i1 = group_end(seqs, i0);
         const int tokens = segment_tokens(a, sh, seqs, i0, i1);
@@ -571,6 +612,26 @@ int chunk_launch(const LinArgs& a, int dtype, const std::vector<Seq>& seqs, void
         const int nseg = tab.seg0[tab.n];
         double* decays = static_cast<double*>(workspace);
         float* states = reinterpret_cast<float*>(decays + static_cast<size_t>(nseg) * a.heads);
+        auto join = [&]() {
+            k_chunk_join<<<dim3((a.dk * a.dv + 255) / 256, a.heads, tab.n), 256, 0, st>>>(a, tab, states, decays);
+        };
+        if (sh.tc) {
+            const dim3 grid((a.dv + 127) / 128, a.heads, nseg);
+            auto go = [&](auto k) {
+                constexpr int K = decltype(k)::value, bytes = tc::Plan<K>::bytes;
+                if (divided) {
+                    allow_smem<tc::k_chunk_tc<K, false>>(bytes);
+                    tc::k_chunk_tc<K, false><<<grid, tc::kTcThreads, bytes, st>>>(a, tab, states, decays);
+                    join();
+                }
+                allow_smem<tc::k_chunk_tc<K, true>>(bytes);
+                tc::k_chunk_tc<K, true><<<grid, tc::kTcThreads, bytes, st>>>(a, tab, states, decays);
+                return launched("k_chunk_tc");
+            };
+            const int rc = sh.dk == 64 ? go(std::integral_constant<int, 64>()) : go(std::integral_constant<int, 128>());
+            if (rc != SSLA_OK) return rc;
+            continue;
+        }
         const int rc = with_shape(dtype, a.dk, a.dv, [&](auto t, auto k, auto v) {
             using T = decltype(t);
             constexpr int K = decltype(k)::value, V = decltype(v)::value, bytes = Tile<T, K, V>::bytes;
@@ -579,7 +640,7 @@ int chunk_launch(const LinArgs& a, int dtype, const std::vector<Seq>& seqs, void
             if (divided) {
                 allow_smem<k_chunk<T, K, V, false>>(bytes);
                 k_chunk<T, K, V, false><<<grid, kThreads, bytes, st>>>(a, tab, states, decays, wides);
-                k_chunk_join<<<dim3((a.dk * a.dv + 255) / 256, a.heads, tab.n), 256, 0, st>>>(a, tab, states, decays);
+                join();
             }
             k_chunk<T, K, V, true><<<grid, kThreads, bytes, st>>>(a, tab, states, decays, wides);
             return launched("k_chunk");
@@ -587,6 +648,15 @@ int chunk_launch(const LinArgs& a, int dtype, const std::vector<Seq>& seqs, void
         if (rc != SSLA_OK) return rc;
     }
     return SSLA_OK;
+}
+
+// Bits of the tcgen05 form's bounded waits since the last call (1: one ran out).
+int chunk_status(unsigned* bits) {
+    unsigned zero = 0;
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(bits, tc::g_status, sizeof *bits);
+    if (e == cudaSuccess) e = cudaMemcpyToSymbol(tc::g_status, &zero, sizeof zero);
+    return e == cudaSuccess ? SSLA_OK : fail(SSLA_ERR_CUDA, "linear attention status: %s", cudaGetErrorString(e));
 }
 
 }  // namespace ops

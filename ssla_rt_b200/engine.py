@@ -81,6 +81,7 @@ def load_library() -> C.CDLL:
         "ssla_s2s3_gate_codes_noalloc": (i, [C.POINTER(abi.HybridS2S3Config), vp, vp, vp, vp]),
         "ssla_linattn_chunk": (i, [C.POINTER(abi.SslaLinAttn), vp, vp, vp, i, vp, C.c_size_t, vp]),
         "ssla_linattn_chunk_workspace": (i, [C.POINTER(abi.SslaLinAttn), vp, vp, i, C.POINTER(C.c_size_t)]),
+        "ssla_linattn_status": (i, [i, C.POINTER(C.c_uint)]),
         "ssla_linattn_step": (i, [C.POINTER(abi.SslaLinAttn), vp, vp]),
         "ssla_state_store": (i, [C.POINTER(abi.SslaStateCache), vp, vp]),
         "ssla_state_load": (i, [C.POINTER(abi.SslaStateCache), vp, vp]),

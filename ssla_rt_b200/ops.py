@@ -253,6 +253,15 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     return out
 
 
+def linear_attention_status(device: int = 0) -> int:
+    """Status bits of linear_attention's kernels on a device since the last
+    call (0: fine; 1: a bounded wait ran out and results since are not valid).
+    Synchronises the device."""
+    st = C.c_uint(0)
+    _check(load_library().ssla_linattn_status(device, C.byref(st)))
+    return st.value
+
+
 def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
                           state: torch.Tensor, *, slots: Optional[torch.Tensor] = None, scale: float = 1.0,
                           out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:

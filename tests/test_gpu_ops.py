@@ -161,6 +161,18 @@ def test_linear_attention_strides_and_padding(dtype):
 
 
 @pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dk,dv", [(100, 130), (50, 35), (71, 127), (33, 250)])
+def test_linear_attention_odd_widths_in_aligned_rows(dtype, dk, dv):
+    n, h = 150, 2
+    wide = lambda seed, w, std: rand(seed, n, h, -(-w // 8) * 8, dtype=DT[dtype], std=std)[:, :, :w]  # noqa: E731
+    q, k, v = wide(1, dk, dk ** -0.25), wide(2, dk, dk ** -0.25), wide(3, dv, 1.0)
+    d, state = -rand(4, n, h).abs() * 0.3, rand(5, 2, h, dk, dv)
+    before = state.clone()
+    out = ops.linear_attention(q, k, v, d, state=state, offsets=[0, 67, 150], scale=0.2)
+    check_attention(q, k, v, d, [(range(67), 0), (range(67, 150), 1)], before, 0.2, out, state)
+
+
+@pytest.mark.parametrize("dtype", DT)
 def test_linear_attention_heads_outermost(dtype):
     """(heads, rows, width) memory, expanded queries, and a decay for each head given with a stride of 0."""
     h, n, dk, dv = 3, 100, 24, 24
@@ -661,3 +673,7 @@ def test_on_other_streams():
 def test_a_stream_given_as_zero_is_the_legacy_default():
     x = rand(1, 4, 64)
     assert torch.equal(ops.group_norm(x, 4, stream=0), ops.group_norm(x, 4))
+
+
+def test_no_wait_ran_out():
+    assert ops.linear_attention_status() == 0

@@ -129,6 +129,7 @@ def test_linattn_null_arguments():
     lib = load_library()
     assert lib.ssla_linattn_chunk(None, None, None, None, 0, None, 0, None) == abi.SSLA_ERR_ARG
     assert lib.ssla_linattn_step(None, None, None) == abi.SSLA_ERR_ARG
+    assert lib.ssla_linattn_status(0, None) == abi.SSLA_ERR_ARG
     assert lib.ssla_linattn_chunk(C.byref(block()), None, None, None, 1, None, 0, None) == abi.SSLA_ERR_ARG
     assert lib.ssla_linattn_chunk_workspace(C.byref(block()), None, None, 0, None) == abi.SSLA_ERR_ARG
     # a state-less call that names slots
