@@ -29,6 +29,7 @@
 // before s, but 0 * inf in a masked place would take it there.  Masked scores
 // are replaced, not multiplied, and a non-finite v is taken out of the tile
 // and put back as NaN into its column from its own token on.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -171,10 +172,16 @@ __device__ __forceinline__ float2 chunk_decay_values(const LinArgs& a, long long
     return make_float2(t < n ? p[t * a.decay_row] : 0.0f, t + 1 < n ? p[(t + 1) * a.decay_row] : 0.0f);
 }
 
-// A chunk's decay sums, by one warp: G_t = sum of the log2 decays up to token
-// t as (hi, lo), 2^{G_t}, 2^{G_C - G_t}, 2^{G_C}.  The sums are taken in 64
-// bits: differences of them are exponents below.  Returns G_C.
-__device__ __forceinline__ double chunk_decays(float2 g, int lane, float* ghi, float* glo, float* eg, float* wk, float* gam) {
+// A chunk's decay sums, by one warp; a lane's for its two tokens: G_t = sum of
+// the log2 decays up to token t as (hi, lo), 2^{G_t}, 2^{G_C - G_t}, and for
+// the chunk 2^{G_C} and G_C.  The sums are taken in 64 bits: differences of
+// them are exponents.
+struct DecaySums {
+    float hi[2], lo[2], grown[2], left[2], whole;
+    double total;
+};
+__device__ __forceinline__ DecaySums chunk_decays(float2 g, int lane) {
+    DecaySums d;
     double s[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -189,19 +196,18 @@ __device__ __forceinline__ double chunk_decays(float2 g, int lane, float* ghi, f
         const double o = __shfl_up_sync(0xFFFFFFFFu, run, m);
         if (lane >= m) run += o;
     }
-    const double all = __shfl_sync(0xFFFFFFFFu, run, 31), before = run - s[1];
+    d.total = __shfl_sync(0xFFFFFFFFu, run, 31);
+    const double before = run - s[1];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const int t = 2 * lane + j;
         const double G = j ? run : before + s[0];
-        const float x = static_cast<float>(G);
-        ghi[t] = x;
-        glo[t] = static_cast<float>(G - x);
-        eg[t] = exp2f(x);
-        wk[t] = exp2f(static_cast<float>(all - G));
+        d.hi[j] = static_cast<float>(G);
+        d.lo[j] = static_cast<float>(G - d.hi[j]);
+        d.grown[j] = exp2f(d.hi[j]);
+        d.left[j] = exp2f(static_cast<float>(d.total - G));
     }
-    if (lane == 0) gam[0] = exp2f(static_cast<float>(all));
-    return all;
+    d.whole = exp2f(static_cast<float>(d.total));
+    return d;
 }
 
 // Segment states: [segment][head][dk][dv]; segment decays: [segment][head].
@@ -282,7 +288,17 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
                 }
         }
         if (warp == 0) {
-            total += chunk_decays(chunk_decay_values(a, row, n, h, lane), lane, ghi, glo, eg, wk, gam);
+            const DecaySums d = chunk_decays(chunk_decay_values(a, row, n, h, lane), lane);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int t = 2 * lane + j;
+                ghi[t] = d.hi[j];
+                glo[t] = d.lo[j];
+                eg[t] = d.grown[j];
+                wk[t] = d.left[j];
+            }
+            if (lane == 0) gam[0] = d.whole;
+            total += d.total;
         }
         any = __syncthreads_or(any);
 
@@ -531,7 +547,7 @@ int wide_inputs(const LinArgs& a, int dtype) {
 
 Shape shape_of(const LinArgs& a, int dtype) {
     // bf16 with wide heads: the tcgen05 form, whose copies are 16 bytes wide
-    if (dtype == SSLA_DT_BF16 && a.dk > 32 && a.dv > 32 && wide_inputs(a, dtype) == 7)
+    if (dtype == SSLA_DT_BF16 && a.dk > 32 && a.dv > 32 && wide_inputs(a, dtype) == 7 && a.out_row <= INT_MAX)
         return Shape{a.dk <= 64 ? 64 : 128, 128, 1, true, 155};
     return with_shape(dtype, a.dk, a.dv, [](auto t, auto k, auto v) {
         constexpr int K = decltype(k)::value, V = decltype(v)::value;
@@ -619,13 +635,18 @@ int chunk_launch(const LinArgs& a, int dtype, const std::vector<Seq>& seqs, void
             const dim3 grid((a.dv + 127) / 128, a.heads, nseg);
             auto go = [&](auto k) {
                 constexpr int K = decltype(k)::value, bytes = tc::Plan<K>::bytes;
+                tc::Maps maps;
+                const int tma =
+                    tc::tensor_map(&maps.q, a.q, a.dk, a.heads / a.q_share, a.n_rows, a.q_head, a.q_row) &&
+                    tc::tensor_map(&maps.k, a.k, a.dk, a.heads / a.k_share, a.n_rows, a.k_head, a.k_row) &&
+                    tc::tensor_map(&maps.v, a.v, a.dv, a.heads, a.n_rows, a.v_head, a.v_row);
                 if (divided) {
                     allow_smem<tc::k_chunk_tc<K, false>>(bytes);
-                    tc::k_chunk_tc<K, false><<<grid, tc::kTcThreads, bytes, st>>>(a, tab, states, decays);
+                    tc::k_chunk_tc<K, false><<<grid, tc::kTcThreads, bytes, st>>>(a, tab, maps, tma, states, decays);
                     join();
                 }
                 allow_smem<tc::k_chunk_tc<K, true>>(bytes);
-                tc::k_chunk_tc<K, true><<<grid, tc::kTcThreads, bytes, st>>>(a, tab, states, decays);
+                tc::k_chunk_tc<K, true><<<grid, tc::kTcThreads, bytes, st>>>(a, tab, maps, tma, states, decays);
                 return launched("k_chunk_tc");
             };
             const int rc = sh.dk == 64 ? go(std::integral_constant<int, 64>()) : go(std::integral_constant<int, 128>());

@@ -13,13 +13,15 @@
 //     inner   [dv, T]   = V^T P^T              two pieces of the decayed scores P
 // and, in registers, S <- e^{G_C} S + update, out = scale (e^{G_t} carried + inner).
 //
-// Roles (16 warps, one CTA per SM):
-//     warps 0-3    scores -> P (pieces to shared memory); carried, inner -> out
+// Roles (20 warps, one CTA per SM):
+//     warps 0-3    scores -> P: pieces to shared memory
 //     warps 4-11   the state, half of dk each group: wK pieces to shared memory,
 //                  update -> S, pieces of S to tensor memory
-//     warps 12-13  tiles into shared memory (three stages), non-finite v
-//     warp 14      decay sums
-//     warp 15      issues the matrix instructions
+//     warps 12-15  carried, inner -> out
+//     warps 16, 19 tiles into shared memory (three stages): whole chunks by TMA,
+//                  a sequence's last, partial one by 16-byte copies with zeros
+//     warp 17      decay sums
+//     warp 18      issues the matrix instructions
 // They meet at mbarriers only.  Every wait is bounded: one that runs out sets
 // the abort flag and a bit of the device's status word, all roles leave, and
 // the tensor memory is freed.
@@ -27,8 +29,8 @@
 
 namespace tc {
 
-constexpr int kTcThreads = 512;                    // 128 registers a thread
-constexpr int kCopyWarps = 2, kCopyThreads = 32 * kCopyWarps;
+constexpr int kTcThreads = 640;
+constexpr int kCopyThreads = 64;
 constexpr int kStages = 3;                        // chunks whose tiles are in shared memory
 constexpr int kSwRow = 128;                       // bytes of a swizzled row (64 values)
 constexpr int kBlk = kChunk * kSwRow;             // a 64-token tile of 64 columns
@@ -57,43 +59,38 @@ struct Turn {
 };
 
 struct Side {                                     // what the roles share besides the tiles
-    float ghi[kStages][kChunk], glo[kStages][kChunk], eg[kStages][kChunk], wk[kStages][kChunk], gam[kStages];
-    int bad[kStages][kCopyWarps][128], any[kStages][kCopyWarps];                // first non-finite row by column, as each copying warp saw it
-    uint64_t full[kStages], empty[kStages], sc_full, sc_free, p_full, o_full, o_free, wk_full, u_full, u_free, s_full, qs_full;
+    alignas(16) float2 g[kStages][kChunk];        // decay sums as (hi, lo)
+    alignas(16) float eg[kStages][kChunk], wk[kStages][kChunk], gam[kStages];   // eg: times scale
+    int odd[kStages];                             // an update was not finite
+    uint64_t full[kStages], empty[kStages], checked[kStages];
+    uint64_t sc_full, sc_free, p_full, o_full, o_free, wk_full, u_full, u_free, s_full, qs_full;
     uint32_t tmem;
     int abort;
-
-    __device__ bool any_bad(int st) const { return (any[st][0] | any[st][1]) != 0; }
-    __device__ int first_bad(int st, int d) const {
-        return min(bad[st][0][d], bad[st][1][d]);
-    }
 };
 
-__device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
-    // 128-byte swizzle, version 1
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | static_cast<uint64_t>((lead >> 4) & 0x3FFFu) << 16 |
-           static_cast<uint64_t>((stride >> 4) & 0x3FFFu) << 32 | 1ull << 46 | 2ull << 61;
-}
-// 64-column blocks of rows one after the other: columns are the contracted
-// index (K-major), or the rows are (MN-major, blocks kBlk apart).
-__device__ __forceinline__ uint64_t k_major(uint32_t tile, int ks) {
-    return umma_desc(tile + ks / 4 * kBlk + ks % 4 * 32, 16, 1024);
-}
-__device__ __forceinline__ uint64_t mn_major(uint32_t tile, int ks) { return umma_desc(tile + ks * 16 * kSwRow, kBlk, 1024); }
+// Shared memory descriptors (128-byte swizzle, version 1) of tiles made of
+// 64-column blocks, kBlk apart, of 128-byte rows.  Only the low word moves.
+// K-major: the columns are the contracted index.  MN-major: the rows are.
+constexpr uint32_t kDescHi = 1024u >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t k_major(uint32_t tile) { return tile >> 4 & 0x3FFFu | 1u << 16; }
+__device__ __forceinline__ uint32_t mn_major(uint32_t tile) { return tile >> 4 & 0x3FFFu | static_cast<uint32_t>(kBlk >> 4) << 16; }
+__host__ __device__ constexpr uint32_t k_step(int ks) { return (ks / 4 * kBlk + ks % 4 * 32) >> 4; }
+__host__ __device__ constexpr uint32_t mn_step(int ks) { return ks * 16 * kSwRow >> 4; }
 // D f32, A and B bf16; M x N, `at` / `bt`: operand is MN-major.
 __host__ __device__ constexpr uint32_t umma_idesc(int m, int n, int at, int bt) {
     return 1u << 4 | 1u << 7 | 1u << 10 | static_cast<uint32_t>(at) << 15 | static_cast<uint32_t>(bt) << 16 |
            static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(acc) : "memory");
+template <uint32_t ID> __device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, bool acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "r"(b), "n"(ID), "r"(static_cast<uint32_t>(acc)), "r"(kDescHi) : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 :: "r"(d), "r"(a), "l"(b), "r"(id), "r"(acc) : "memory");
+template <uint32_t ID> __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, bool acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "r"(b), "n"(ID), "r"(static_cast<uint32_t>(acc)), "r"(kDescHi) : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
@@ -121,19 +118,23 @@ __device__ __forceinline__ unsigned long long now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// Waits for a phase, two seconds at most; false: give up.
+// Waits for a phase, two seconds at most; false: give up.  (A try suspends
+// the thread for a while by itself.)
 __device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity, Side* s) {
     if (bar_try(bar, parity)) return true;
-    const unsigned long long t0 = now_ns();
-    while (!bar_try(bar, parity)) {
+    unsigned long long t0 = 0;
+    for (unsigned i = 1;; ++i) {
+        if (bar_try(bar, parity)) return true;
+        if (i % 16) continue;
         if (*reinterpret_cast<volatile int*>(&s->abort)) return false;
-        if (now_ns() - t0 > 2000000000ull) {
+        const unsigned long long t = now_ns();
+        if (!t0) t0 = t;
+        if (t - t0 > 2000000000ull) {
             *reinterpret_cast<volatile int*>(&s->abort) = 1;
             atomicOr(&g_status, kTimedOut);
             return false;
         }
     }
-    return true;
 }
 // The same for a whole warp, which goes on or gives up as one.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, Side* s) {
@@ -146,15 +147,12 @@ __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
     }
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr));
 }
 __device__ __forceinline__ void tmem_ld_frag(uint32_t addr, uint32_t (&r)[32]) {
@@ -177,18 +175,31 @@ __device__ __forceinline__ void ld_wait(uint32_t (&r)[32]) {
                    "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
                  :: "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-        :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
+__device__ __forceinline__ void ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :: "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 
 // 16-byte piece `ch` of row r in a tile of 64-column blocks.
 __device__ __forceinline__ uint32_t piece_at(int r, int ch) {
     return static_cast<uint32_t>(ch / 8 * kBlk + r * kSwRow + ((ch % 8 ^ r % 8) << 4));
+}
+// A 64-column, 64-row box of a [rows][heads][columns] tensor map.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 :: "r"(dst), "l"(map), "r"(x), "r"(head), "r"(row), "r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {     // 2^-22; results below 2^-126 become zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -211,9 +222,14 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const __nv_bfloat16* p, 
     }
 }
 
+struct Maps {
+    CUtensorMap q, k, v;
+};
+
 template <int DK, bool OUT>
 __global__ void __launch_bounds__(kTcThreads, 1)
-k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* seg_decay) {
+k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__ Maps maps, int use_tma, float* seg_state,
+           double* seg_decay) {
     using L = Plan<DK>;
     using T = __nv_bfloat16;
     constexpr int HC = DK / 2;                    // state columns of a state group
@@ -240,8 +256,9 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, float* seg_state, doubl
 
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
-            bar_init(&s.full[i], kCopyWarps + 1);
-            bar_init(&s.empty[i], OUT ? 13 : 9);  // the matrix unit, the state warps, the output warps
+            bar_init(&s.full[i], 3);              // two copying warps, the decay warp
+            bar_init(&s.empty[i], OUT ? 17 : 9);  // the matrix unit, the state warps, the P and output warps
+            bar_init(&s.checked[i], 8);
         }
         bar_init(&s.sc_full, 1); bar_init(&s.sc_free, 4); bar_init(&s.p_full, 4);
         bar_init(&s.o_full, 1); bar_init(&s.o_free, 4); bar_init(&s.wk_full, 8);
@@ -249,80 +266,70 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, float* seg_state, doubl
         s.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 15) {
+    if (warp == 18) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    // value columns from 64 on that no copy writes
+    if (width <= 64)
+        for (int i = tid; i < kStages * kBlk / 16; i += kTcThreads)
+            *reinterpret_cast<uint4*>(gen + i / (kBlk / 16) * L::kStage + 2 * L::kTile + kBlk + i % (kBlk / 16) * 16) =
+                make_uint4(0, 0, 0, 0);
+    to_async();
     before_sync();
     __syncthreads();
     after_sync();
     const uint32_t tm = s.tmem;
 
     if (warp < 4) {
-        // ---- scores -> P; carried, inner -> out ----
+        // ---- scores -> P ----
         if constexpr (OUT) {
             const int ra = warp * 16 + lane / 4, rb = ra + 8, t2 = lane % 4 * 2;
-            const int d = warp * 32 + lane;       // value column of the outputs
-            const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+            uint8_t* const pa = gen + L::kP + ra * kSwRow + t2 * 2;
+            uint8_t* const pb = pa + 8 * kSwRow;
             Turn at;
             for (int c = 0; c < chunks; ++c, at.next()) {
-                const int st = at.st, n = min(kChunk, count - c * kChunk);
+                const int st = at.st;
                 if (!bar_wait(&s.full[st], at.ph, &s)) break;
+                const float2 ga = s.g[st][ra], gb = s.g[st][rb];
                 if (!bar_wait(&s.sc_full, at.par, &s)) break;
                 after_sync();
                 uint32_t r[32];
-                tmem_ld_frag(tm + lanes + L::kSc, r);
-                const float ha = s.ghi[st][ra], la = s.glo[st][ra], hb = s.ghi[st][rb], lb = s.glo[st][rb];
+                tmem_ld_frag(tm + (static_cast<uint32_t>(warp * 32) << 16) + L::kSc, r);
                 ld_wait(r);
                 before_sync();
                 warp_arrive(&s.sc_free);
-                uint8_t* const pa = gen + L::kP + ra * kSwRow + t2 * 2;
-                uint8_t* const pb = pa + 8 * kSwRow;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    float x[4] = {};
-                    if (j * 8 <= warp * 16 + 15) {                // not wholly above the diagonal
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int col = j * 8 + t2 + e;
-                            const float hs = s.ghi[st][col], ls = s.glo[st][col];
-                            if (col <= ra) x[e] = __uint_as_float(r[j * 4 + e]) * exp2f((ha - hs) + (la - ls));
-                            if (col <= rb) x[2 + e] = __uint_as_float(r[j * 4 + 2 + e]) * exp2f((hb - hs) + (lb - ls));
-                        }
+                    if (j * 8 > warp * 16 + 15) {                 // wholly above the diagonal
+                        r[j * 4] = r[j * 4 + 1] = r[j * 4 + 2] = r[j * 4 + 3] = 0;
+                        continue;
                     }
+                    const float4 g = *reinterpret_cast<const float4*>(&s.g[st][j * 8 + t2]);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int col = j * 8 + t2 + e;
+                        const float hs = e ? g.z : g.x, ls = e ? g.w : g.y;
+                        const float xa = __uint_as_float(r[j * 4 + e]) * exp2_fast((ga.x - hs) + (ga.y - ls)) * a.scale;
+                        const float xb = __uint_as_float(r[j * 4 + 2 + e]) * exp2_fast((gb.x - hs) + (gb.y - ls)) * a.scale;
+                        r[j * 4 + e] = col <= ra ? __float_as_uint(xa) : 0u;
+                        r[j * 4 + 2 + e] = col <= rb ? __float_as_uint(xb) : 0u;
+                    }
+                }
+                // the chunk before has been read: by the matrix unit, and where v was not finite by the output warps
+                if (c && !bar_wait(&s.o_free, at.par ^ 1, &s)) break;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
                     const int ch = (j ^ ra % 8) << 4;             // (rb is the same row of its atom)
-                    *reinterpret_cast<uint32_t*>(pa + ch) = take(x[0], x[1]);
-                    *reinterpret_cast<uint32_t*>(pa + kBlk + ch) = take(x[0], x[1]);
-                    *reinterpret_cast<uint32_t*>(pb + ch) = take(x[2], x[3]);
-                    *reinterpret_cast<uint32_t*>(pb + kBlk + ch) = take(x[2], x[3]);
+                    float x0 = __uint_as_float(r[j * 4]), x1 = __uint_as_float(r[j * 4 + 1]);
+                    float y0 = __uint_as_float(r[j * 4 + 2]), y1 = __uint_as_float(r[j * 4 + 3]);
+                    *reinterpret_cast<uint32_t*>(pa + ch) = take(x0, x1);
+                    *reinterpret_cast<uint32_t*>(pa + kBlk + ch) = pack2(x0, x1);
+                    *reinterpret_cast<uint32_t*>(pb + ch) = take(y0, y1);
+                    *reinterpret_cast<uint32_t*>(pb + kBlk + ch) = pack2(y0, y1);
                 }
                 to_async();
                 warp_arrive(&s.p_full);
-                if (!bar_wait(&s.o_full, at.par, &s)) break;
-                after_sync();
-                const bool any = s.any_bad(st);
-                const int from = any ? s.first_bad(st, d) : kChunk;
-                T* p = static_cast<T*>(a.out) + (row0 + c * kChunk) * a.out_row + h * a.out_head + c0 + d;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t u[32];
-                    tmem_ld32(tm + lanes + L::kO1 + half * 32, r);
-                    tmem_ld32(tm + lanes + L::kO2 + half * 32, u);
-                    ld_wait(r);
-                    ld_wait(u);
-                    if (half == 1) {
-                        before_sync();
-                        warp_arrive(&s.o_free);
-                    }
-                    const int left = n - half * 32;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        float y = fmaf(s.eg[st][half * 32 + i], __uint_as_float(r[i]), __uint_as_float(u[i])) * a.scale;
-                        if (any && half * 32 + i >= from) y = __int_as_float(0x7FC00000);
-                        if (i < left && d < width) *p = __float2bfloat16_rn(y);
-                        p += a.out_row;
-                    }
-                }
                 warp_arrive(&s.empty[st]);
             }
         }
@@ -339,16 +346,16 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, float* seg_state, doubl
             S[i] = from && d < width && k0 + i < a.dk ? from[static_cast<size_t>(k0 + i) * a.dv + c0 + d] : 0.0f;
         auto put_pieces = [&]() {                  // S as two bf16 pieces, two columns a word
 #pragma unroll
-            for (int b = 0; b < HC / 32; ++b) {
-                uint32_t hi16[16], lo16[16];
+            for (int b = 0; b < HC / 16; ++b) {
+                uint32_t big[8], small[8];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float x = S[b * 32 + 2 * i], y = S[b * 32 + 2 * i + 1];
-                    hi16[i] = take(x, y);
-                    lo16[i] = pack2(x, y);
+                for (int i = 0; i < 8; ++i) {
+                    float x = S[b * 16 + 2 * i], y = S[b * 16 + 2 * i + 1];
+                    big[i] = take(x, y);
+                    small[i] = pack2(x, y);
                 }
-                tmem_st16(tm + lanes + L::kS + k0 / 2 + b * 16, hi16);
-                tmem_st16(tm + lanes + L::kS + DK / 2 + k0 / 2 + b * 16, lo16);
+                tmem_st8(tm + lanes + L::kS + k0 / 2 + b * 8, big);
+                tmem_st8(tm + lanes + L::kS + DK / 2 + k0 / 2 + b * 8, small);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             before_sync();
@@ -383,22 +390,26 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, float* seg_state, doubl
         for (int c = 0; ok && c < chunks; ++c) {
             const int st = at.st;
             const uint32_t par = at.par;
+            const float gam = s.gam[st];           // (its stage is full)
             if (!(ok = bar_wait(&s.u_full, par, &s))) break;
             after_sync();
-            const float gam = s.gam[st];
+            bool odd = false;
 #pragma unroll
-            for (int b = 0; b < HC / 32; ++b) {
-                uint32_t u[32];
-                tmem_ld32(tm + lanes + L::kU + k0 + b * 32, u);
+            for (int b = 0; b < HC / 16; ++b) {
+                uint32_t u[16];
+                tmem_ld16(tm + lanes + L::kU + k0 + b * 16, u);
                 ld_wait(u);
+                // every column of this lane has every v of value column d as a factor
+                if (b == 0) odd = (u[0] & 0x7F800000u) == 0x7F800000u;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) S[b * 32 + i] = fmaf(gam, S[b * 32 + i], __uint_as_float(u[i]));
+                for (int i = 0; i < 16; ++i) S[b * 16 + i] = fmaf(gam, S[b * 16 + i], __uint_as_float(u[i]));
             }
             before_sync();
             warp_arrive(&s.u_free);
-            if (s.any_bad(st) && s.first_bad(st, d) < kChunk)
-#pragma unroll
-                for (int i = 0; i < HC; ++i) S[i] = __int_as_float(0x7FC00000);
+            if (OUT) {
+                if (odd) s.odd[st] = 1;
+                warp_arrive(&s.checked[st]);
+            }
             warp_arrive(&s.empty[st]);
             at.next();
             if (c + 1 < chunks) {
@@ -418,59 +429,120 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, float* seg_state, doubl
 #pragma unroll
             for (int i = 0; i < HC; ++i)
                 if (k0 + i < a.dk) to[static_cast<size_t>(k0 + i) * a.dv + c0 + d] = S[i];
-    } else if (warp < 12 + kCopyWarps) {
-        // ---- tiles, non-finite values ----
-        const int t = tid - 384, w = warp - 12;
-        const T* Q = static_cast<const T*>(a.q) + (h / a.q_share) * a.q_head + row0 * a.q_row;
-        const T* K = static_cast<const T*>(a.k) + (h / a.k_share) * a.k_head + row0 * a.k_row;
+    } else if (warp < 16) {
+        // ---- carried, inner -> out: value column d, 64 tokens ----
+        if constexpr (OUT) {
+            const int d = (warp - 12) * 32 + lane;
+            const uint32_t lanes = static_cast<uint32_t>((warp - 12) * 32) << 16;
+            const int stride = static_cast<int>(a.out_row);
+            Turn at;
+            for (int c = 0; c < chunks; ++c, at.next()) {
+                const int st = at.st, n = min(kChunk, count - c * kChunk);
+                if (!bar_wait(&s.full[st], at.ph, &s)) break;
+                if (!bar_wait(&s.checked[st], at.ph, &s)) break;
+                const bool odd = s.odd[st] != 0;
+                if (!bar_wait(&s.o_full, at.par, &s)) break;
+                after_sync();
+                uint32_t y[kChunk / 2];            // outputs, two tokens a word
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t r[16], u[16];
+                    tmem_ld16(tm + lanes + L::kO1 + b * 16, r);
+                    tmem_ld16(tm + lanes + L::kO2 + b * 16, u);
+                    ld_wait(r);
+                    ld_wait(u);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 e = *reinterpret_cast<const float4*>(&s.eg[st][b * 16 + i]);
+                        y[b * 8 + i / 2] = pack2(fmaf(e.x, __uint_as_float(r[i]), __uint_as_float(u[i])),
+                                                 fmaf(e.y, __uint_as_float(r[i + 1]), __uint_as_float(u[i + 1])));
+                        y[b * 8 + i / 2 + 1] = pack2(fmaf(e.z, __uint_as_float(r[i + 2]), __uint_as_float(u[i + 2])),
+                                                     fmaf(e.w, __uint_as_float(r[i + 3]), __uint_as_float(u[i + 3])));
+                    }
+                }
+                T* const p = static_cast<T*>(a.out) + (row0 + static_cast<long long>(c) * kChunk) * a.out_row + h * a.out_head + c0 + d;
+                if (!odd) {
+                    before_sync();
+                    warp_arrive(&s.o_free);
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i)
+                        if (i < n && d < width)
+                            p[static_cast<long long>(i) * stride] =
+                                __ushort_as_bfloat16(static_cast<unsigned short>(i % 2 ? y[i / 2] >> 16 : y[i / 2] & 0xFFFFu));
+                } else {
+                    // A value in this chunk was not finite: if it is in this column, the product with
+                    // masked zeros has reached the tokens before it.  Their inner sums again, one by one.
+                    const uint8_t* V = gen + st * L::kStage + 2 * L::kTile;
+                    auto value = [&](int t) {
+                        return __bfloat162float(*reinterpret_cast<const T*>(V + piece_at(t, d / 8) + d % 8 * 2));
+                    };
+                    int bad = 0;
+                    while (bad < n && finite(value(bad))) ++bad;
+                    const uint8_t* P = gen + L::kP;
+                    for (int i = 0; i < n; ++i) {
+                        uint32_t o1, o2;
+                        __syncwarp();
+                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o1) : "r"(tm + lanes + L::kO1 + i));
+                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o2) : "r"(tm + lanes + L::kO2 + i));
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(o1), "+r"(o2) :: "memory");
+                        float inner = __uint_as_float(o2);
+                        if (bad < n) {
+                            inner = i < bad ? 0.0f : __int_as_float(0x7FC00000);
+                            if (i < bad)
+                                for (int t = 0; t <= i; ++t) {
+                                    const uint32_t at_p = piece_at(i, t / 8) + t % 8 * 2;
+                                    const float w = __bfloat162float(*reinterpret_cast<const T*>(P + at_p)) +
+                                                    __bfloat162float(*reinterpret_cast<const T*>(P + kBlk + at_p));
+                                    inner = fmaf(w, value(t), inner);
+                                }
+                        }
+                        if (d < width)
+                            p[static_cast<long long>(i) * stride] = __float2bfloat16_rn(fmaf(s.eg[st][i], __uint_as_float(o1), inner));
+                    }
+                    before_sync();
+                    warp_arrive(&s.o_free);
+                }
+                warp_arrive(&s.empty[st]);
+            }
+        }
+    } else if (warp == 16 || warp == 19) {
+        // ---- tiles ----
+        const int t = lane + (warp == 19 ? 32 : 0), hq = h / a.q_share, hk = h / a.k_share;
+        const T* Q = static_cast<const T*>(a.q) + hq * a.q_head + row0 * a.q_row;
+        const T* K = static_cast<const T*>(a.k) + hk * a.k_head + row0 * a.k_row;
         const T* V = static_cast<const T*>(a.v) + h * a.v_head + c0 + row0 * a.v_row;
-        Turn at, arrived;
-        bool ok = true;
-        // chunk c's copies start as soon as its stage is free; then chunk c - 1,
-        // whose copies started a chunk's time earlier, is handed over
-        for (int c = 0; ok && c <= chunks; ++c) {
-            if (c < chunks) {
-                const int n = min(kChunk, count - c * kChunk);
-                if (c >= kStages && !(ok = bar_wait(&s.empty[at.st], at.ph ^ 1, &s))) break;
-                const uint32_t to = base + at.st * L::kStage;
+        Turn at;
+        for (int c = 0; c < chunks; ++c, at.next()) {
+            const int n = min(kChunk, count - c * kChunk);
+            if (c >= kStages && !bar_wait(&s.empty[at.st], at.ph ^ 1, &s)) break;
+            uint64_t* const bar = &s.full[at.st];
+            const uint32_t to = base + at.st * L::kStage;
+            if (warp == 16 && lane == 0) s.odd[at.st] = 0;
+            if (use_tma && n == kChunk) {
+                if (warp == 16 && lane == 0) {
+                    const int row = static_cast<int>(row0) + c * kChunk;
+                    const uint32_t bytes = ((OUT ? 2 : 1) * (DK / 64) + (width > 64 ? 2 : 1)) * kBlk;
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+#pragma unroll
+                    for (int b = 0; b < DK / 64; ++b) tma_box(to + L::kTile + b * kBlk, &maps.k, b * 64, hk, row, bar);
+                    tma_box(to + 2 * L::kTile, &maps.v, c0, h, row, bar);
+                    if (width > 64) tma_box(to + 2 * L::kTile + kBlk, &maps.v, c0 + 64, h, row, bar);
+                    if (OUT)
+#pragma unroll
+                        for (int b = 0; b < DK / 64; ++b) tma_box(to + b * kBlk, &maps.q, b * 64, hq, row, bar);
+                }
+                if (warp == 19) warp_arrive(bar);
+            } else {
                 const long long row = static_cast<long long>(c) * kChunk;
                 copy_tile<DK>(to + L::kTile, K + row * a.k_row, a.k_row, n, a.dk, t);
                 copy_tile<128>(to + 2 * L::kTile, V + row * a.v_row, a.v_row, n, width, t);
                 if (OUT) copy_tile<DK>(to, Q + row * a.q_row, a.q_row, n, a.dk, t);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s.bad[at.st][w][lane + 32 * i] = kChunk;
-                if (lane == 0) s.any[at.st][w] = 0;
-                __syncwarp();
-                at.next();
+                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+                to_async();
+                warp_arrive(bar);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (c == 0) continue;
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            uint8_t* const tile = gen + arrived.st * L::kStage + 2 * L::kTile;
-            bool any = false;
-#pragma unroll
-            for (int i = 0; i < kChunk * 16 / kCopyThreads; ++i) {       // the pieces this thread has copied
-                const int r = t / 16 + i * (kCopyThreads / 16), ch = t % 16;
-                const uint4 u = *reinterpret_cast<const uint4*>(tile + piece_at(r, ch));
-                bool odd = false;
-                for (uint32_t x : {u.x, u.y, u.z, u.w}) odd |= (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
-                if (odd) {
-                    uint16_t* p = reinterpret_cast<uint16_t*>(tile + piece_at(r, ch));
-                    any = true;
-                    for (int j = 0; j < 8; ++j)
-                        if ((p[j] & 0x7F80u) == 0x7F80u) {
-                            p[j] = 0;
-                            atomicMin(&s.bad[arrived.st][w][ch * 8 + j], r);
-                        }
-                }
-            }
-            if (any) s.any[arrived.st][w] = 1;
-            to_async();
-            warp_arrive(&s.full[arrived.st]);
-            arrived.next();
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp == 14) {
+    } else if (warp == 17) {
         // ---- decay sums, the next chunk's values in flight ----
         double total = 0.0;
         Turn at;
@@ -481,7 +553,12 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, float* seg_state, doubl
                 ahead = chunk_decay_values(a, row0 + (c + 1LL) * kChunk, min(kChunk, count - (c + 1) * kChunk), h, lane);
             if (c >= kStages && !bar_wait(&s.empty[at.st], at.ph ^ 1, &s)) break;
             const int st = at.st;
-            total += chunk_decays(g, lane, s.ghi[st], s.glo[st], s.eg[st], s.wk[st], &s.gam[st]);
+            const DecaySums d = chunk_decays(g, lane);
+            total += d.total;
+            *reinterpret_cast<float4*>(&s.g[st][2 * lane]) = make_float4(d.hi[0], d.lo[0], d.hi[1], d.lo[1]);
+            *reinterpret_cast<float2*>(&s.eg[st][2 * lane]) = make_float2(d.grown[0] * a.scale, d.grown[1] * a.scale);
+            *reinterpret_cast<float2*>(&s.wk[st][2 * lane]) = make_float2(d.left[0], d.left[1]);
+            if (lane == 0) s.gam[st] = d.whole;
             warp_arrive(&s.full[st]);
             g = ahead;
         }
@@ -490,10 +567,11 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, float* seg_state, doubl
         // ---- matrix instructions ----
         constexpr uint32_t id_sc = umma_idesc(64, 64, 0, 0), id_u = umma_idesc(128, DK, 1, 1), id_q = umma_idesc(128, 64, 0, 0),
                            id_p = umma_idesc(128, 64, 1, 0);
-        const int ksteps = (a.dk + 15) / 16;       // of the contraction over dk
+        const uint32_t wk_desc = mn_major(base + L::kWk), p_desc = k_major(base + L::kP);
         auto scores = [&](int st) {
-            const uint32_t q = base + st * L::kStage;
-            for (int k = 0; k < ksteps; ++k) umma_ss(tm + L::kSc, k_major(q, k), k_major(q + L::kTile, k), id_sc, k > 0);
+            const uint32_t q = k_major(base + st * L::kStage), k = k_major(base + st * L::kStage + L::kTile);
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) umma_ss<id_sc>(tm + L::kSc, q + k_step(i), k + k_step(i), i > 0);
             commit(&s.sc_full);
         };
         bool ok = lane_wait(&s.full[0], 0, &s);
@@ -501,28 +579,35 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, float* seg_state, doubl
         if (OUT && ok) scores(0);
         Turn at;
         for (int c = 0; ok && c < chunks; ++c) {
-            const uint32_t par = at.par, prev = par ^ 1, tiles = base + at.st * L::kStage, v = tiles + 2 * L::kTile;
+            const uint32_t par = at.par, prev = par ^ 1, tiles = base + at.st * L::kStage;
+            const uint32_t q = k_major(tiles), v = mn_major(tiles + 2 * L::kTile);
             const int st = at.st;
             if (!(ok = lane_wait(&s.wk_full, par, &s))) break;
             if (c && !(ok = lane_wait(&s.u_free, prev, &s))) break;
             after_sync();
-            for (int k = 0; k < kChunk / 16; ++k)
+#pragma unroll
+            for (int i = 0; i < kChunk / 16; ++i)
+#pragma unroll
                 for (int m = 0; m < 3; ++m)
-                    umma_ss(tm + L::kU, mn_major(v, k), mn_major(base + L::kWk + m * L::kTile, k), id_u, k + m > 0);
+                    umma_ss<id_u>(tm + L::kU, v + mn_step(i), wk_desc + (m * L::kTile >> 4) + mn_step(i), i + m > 0);
             commit(&s.u_full);
             if constexpr (OUT) {
                 if (!(ok = lane_wait(&s.s_full, par, &s))) break;
                 if (c && !(ok = lane_wait(&s.o_free, prev, &s))) break;
                 after_sync();
+#pragma unroll
                 for (int m = 0; m < 2; ++m)
-                    for (int k = 0; k < ksteps; ++k)
-                        umma_ts(tm + L::kO1, tm + L::kS + m * (DK / 2) + k * 8, k_major(tiles, k), id_q, m + k > 0);
+#pragma unroll
+                    for (int i = 0; i < DK / 16; ++i)
+                        umma_ts<id_q>(tm + L::kO1, tm + L::kS + m * (DK / 2) + i * 8, q + k_step(i), m + i > 0);
                 commit(&s.qs_full);
                 if (!(ok = lane_wait(&s.p_full, par, &s))) break;
                 after_sync();
+#pragma unroll
                 for (int m = 0; m < 2; ++m)
-                    for (int k = 0; k < kChunk / 16; ++k)
-                        umma_ss(tm + L::kO2, mn_major(v, k), k_major(base + L::kP + m * kBlk, k), id_p, m + k > 0);
+#pragma unroll
+                    for (int i = 0; i < kChunk / 16; ++i)
+                        umma_ss<id_p>(tm + L::kO2, v + mn_step(i), p_desc + (m * kBlk >> 4) + k_step(i), m + i > 0);
                 commit(&s.o_full);
             }
             commit(&s.empty[st]);
@@ -541,10 +626,41 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, float* seg_state, doubl
     __syncwarp();
     before_sync();
     __syncthreads();
-    if (warp == 15) {
+    if (warp == 18) {
         after_sync();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm));
     }
+}
+
+// ---- host ----
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiled encode_tiled() {
+    static const EncodeTiled f = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<EncodeTiled>(fn);
+    }();
+    return f;
+}
+
+// The map of a [rows][heads][width] bf16 tensor in boxes of 64 columns and 64
+// rows of one head, zeros beyond the width.  false: not a tensor TMA takes
+// (a broadcast stride); its tiles go by 16-byte copies.
+inline bool tensor_map(CUtensorMap* m, const void* p, int width, int heads, int rows, long long head, long long row) {
+    if ((heads > 1 && head <= 0) || (rows > 1 && row <= 0) || !encode_tiled()) return false;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(std::max(heads > 1 ? head : 8LL, 8LL)) * 2,
+                                   static_cast<cuuint64_t>(std::max(rows > 1 ? row : 8LL, 8LL)) * 2};
+    const cuuint32_t box[3] = {64, 1, kChunk}, one[3] = {1, 1, 1};
+    return encode_tiled()(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, one,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace tc
