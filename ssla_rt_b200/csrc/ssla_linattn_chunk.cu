@@ -547,7 +547,7 @@ int wide_inputs(const LinArgs& a, int dtype) {
 
 Shape shape_of(const LinArgs& a, int dtype) {
     // bf16 with wide heads: the tcgen05 form, whose copies are 16 bytes wide
-    if (dtype == SSLA_DT_BF16 && a.dk > 32 && a.dv > 32 && wide_inputs(a, dtype) == 7 && a.out_row <= INT_MAX)
+    if (dtype == SSLA_DT_BF16 && a.dk > 32 && a.dv > 32 && wide_inputs(a, dtype) == 7)
         return Shape{a.dk <= 64 ? 64 : 128, 128, 1, true, 155};
     return with_shape(dtype, a.dk, a.dv, [](auto t, auto k, auto v) {
         constexpr int K = decltype(k)::value, V = decltype(v)::value;
@@ -640,13 +640,15 @@ int chunk_launch(const LinArgs& a, int dtype, const std::vector<Seq>& seqs, void
                     tc::tensor_map(&maps.q, a.q, a.dk, a.heads / a.q_share, a.n_rows, a.q_head, a.q_row) &&
                     tc::tensor_map(&maps.k, a.k, a.dk, a.heads / a.k_share, a.n_rows, a.k_head, a.k_row) &&
                     tc::tensor_map(&maps.v, a.v, a.dv, a.heads, a.n_rows, a.v_head, a.v_row);
+                const int out = aligned(a.out, 16) && a.out_row % 8 == 0 && a.out_head % 8 == 0 &&
+                                tc::tensor_map(&maps.out, a.out, a.dv, a.heads, a.n_rows, a.out_head, a.out_row, 32);
                 if (divided) {
                     allow_smem<tc::k_chunk_tc<K, false>>(bytes);
-                    tc::k_chunk_tc<K, false><<<grid, tc::kTcThreads, bytes, st>>>(a, tab, maps, tma, states, decays);
+                    tc::k_chunk_tc<K, false><<<grid, tc::kTcThreads, bytes, st>>>(a, tab, maps, tma, out, states, decays);
                     join();
                 }
                 allow_smem<tc::k_chunk_tc<K, true>>(bytes);
-                tc::k_chunk_tc<K, true><<<grid, tc::kTcThreads, bytes, st>>>(a, tab, maps, tma, states, decays);
+                tc::k_chunk_tc<K, true><<<grid, tc::kTcThreads, bytes, st>>>(a, tab, maps, tma, out, states, decays);
                 return launched("k_chunk_tc");
             };
             const int rc = sh.dk == 64 ? go(std::integral_constant<int, 64>()) : go(std::integral_constant<int, 128>());

@@ -14,10 +14,10 @@
 // and, in registers, S <- e^{G_C} S + update, out = scale (e^{G_t} carried + inner).
 //
 // Roles (20 warps, one CTA per SM):
-//     warps 0-3    scores -> P: pieces to shared memory
-//     warps 4-11   the state, half of dk each group: wK pieces to shared memory,
-//                  update -> S, pieces of S to tensor memory
-//     warps 12-15  carried, inner -> out
+//     warps 0-3    scores -> P: pieces to shared memory; half of the wK pieces
+//     warps 4-11   the state, half of dk each group: update -> S, pieces of S to
+//                  tensor memory
+//     warps 12-15  carried, inner -> out, through shared memory; half of the wK pieces
 //     warps 16, 19 tiles into shared memory (three stages): whole chunks by TMA,
 //                  a sequence's last, partial one by 16-byte copies with zeros
 //     warp 17      decay sums
@@ -42,7 +42,10 @@ template <int DK> struct Plan {
     static constexpr int kTile = DK / 64 * kBlk;  // Q or K of one stage
     static constexpr int kVTile = 2 * kBlk;
     static constexpr int kStage = 2 * kTile + kVTile;
-    static constexpr int kWk = kStages * kStage, kP = kWk + 3 * kTile, kEnd = kP + 2 * kBlk;
+    static constexpr int kWk = kStages * kStage, kP = kWk + 3 * kTile, kEnd = kP + 2 * kBlk + (DK < 128 ? 2 * kBlk : 0);
+    // a chunk's outputs: in the place of its Q, which both its products have
+    // read, where that is large enough
+    __host__ __device__ static constexpr int out_at(int st) { return DK < 128 ? kP + 2 * kBlk : st * kStage; }
     static constexpr int bytes = kEnd + 1024;     // + alignment slack
     // tensor memory columns
     static constexpr int kU = 0, kSc = DK, kO1 = DK + 64, kO2 = DK + 128, kS = DK + 192;
@@ -80,6 +83,11 @@ __host__ __device__ constexpr uint32_t mn_step(int ks) { return ks * 16 * kSwRow
 __host__ __device__ constexpr uint32_t umma_idesc(int m, int n, int at, int bt) {
     return 1u << 4 | 1u << 7 | 1u << 10 | static_cast<uint32_t>(at) << 15 | static_cast<uint32_t>(bt) << 16 |
            static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
+}
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 template <uint32_t ID> __device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, bool acc) {
     asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -223,12 +231,44 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const __nv_bfloat16* p, 
 }
 
 struct Maps {
-    CUtensorMap q, k, v;
+    CUtensorMap q, k, v, out;
 };
+
+// A stage's K decayed to its chunk's end, as three bf16 pieces; thread t of 256.
+template <int DK> __device__ __forceinline__ void put_keys(uint8_t* gen, Side& s, int st, int t) {
+    using L = Plan<DK>;
+    const uint8_t* K = gen + st * L::kStage + L::kTile;
+#pragma unroll
+    for (int i = 0; i < kChunk * DK / 8 / 256; ++i) {
+        const int e = t + i * 256, r = e / (DK / 8), ch = e % (DK / 8);
+        const uint32_t at = piece_at(r, ch);
+        const uint4 u = *reinterpret_cast<const uint4*>(K + at);
+        const float w = s.wk[st][r];
+        float2 f[4] = {unpack2(u.x), unpack2(u.y), unpack2(u.z), unpack2(u.w)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j].x *= w, f[j].y *= w;
+#pragma unroll
+        for (int m = 0; m < 3; ++m) {
+            uint4 o;
+            o.x = take(f[0].x, f[0].y); o.y = take(f[1].x, f[1].y);
+            o.z = take(f[2].x, f[2].y); o.w = take(f[3].x, f[3].y);
+            *reinterpret_cast<uint4*>(gen + L::kWk + m * L::kTile + at) = o;
+        }
+    }
+    to_async();
+    warp_arrive(&s.wk_full);
+}
+
+__device__ __forceinline__ void stmatrix4_trans(uint32_t addr, const uint32_t (&r)[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                 :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+// Piece `ch` (16 bytes) of row t of an output warp's [64][32] tile, 64-byte swizzle.
+__device__ __forceinline__ uint32_t out_piece(int t, int ch) { return static_cast<uint32_t>(t * 64 + ((ch ^ (t >> 1 & 3)) << 4)); }
 
 template <int DK, bool OUT>
 __global__ void __launch_bounds__(kTcThreads, 1)
-k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__ Maps maps, int use_tma, float* seg_state,
+k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__ Maps maps, int use_tma, int tma_out, float* seg_state,
            double* seg_decay) {
     using L = Plan<DK>;
     using T = __nv_bfloat16;
@@ -257,7 +297,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
             bar_init(&s.full[i], 3);              // two copying warps, the decay warp
-            bar_init(&s.empty[i], OUT ? 17 : 9);  // the matrix unit, the state warps, the P and output warps
+            bar_init(&s.empty[i], 17);            // the matrix unit, the state, P and output warps
             bar_init(&s.checked[i], 8);
         }
         bar_init(&s.sc_full, 1); bar_init(&s.sc_free, 4); bar_init(&s.p_full, 4);
@@ -282,17 +322,19 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
     const uint32_t tm = s.tmem;
 
     if (warp < 4) {
-        // ---- scores -> P ----
-        if constexpr (OUT) {
-            const int ra = warp * 16 + lane / 4, rb = ra + 8, t2 = lane % 4 * 2;
-            uint8_t* const pa = gen + L::kP + ra * kSwRow + t2 * 2;
-            uint8_t* const pb = pa + 8 * kSwRow;
-            Turn at;
-            for (int c = 0; c < chunks; ++c, at.next()) {
-                const int st = at.st;
-                if (!bar_wait(&s.full[st], at.ph, &s)) break;
+        // ---- scores -> P; wK ----
+        const int ra = warp * 16 + lane / 4, rb = ra + 8, t2 = lane % 4 * 2;
+        uint8_t* const pa = gen + L::kP + ra * kSwRow + t2 * 2;
+        uint8_t* const pb = pa + 8 * kSwRow;
+        Turn at;
+        bool ok = bar_wait(&s.full[0], 0, &s);
+        if (ok) put_keys<DK>(gen, s, 0, tid);
+        for (int c = 0; ok && c < chunks; ++c) {
+            const int st = at.st;
+            const uint32_t par = at.par;
+            if constexpr (OUT) {
                 const float2 ga = s.g[st][ra], gb = s.g[st][rb];
-                if (!bar_wait(&s.sc_full, at.par, &s)) break;
+                if (!(ok = bar_wait(&s.sc_full, par, &s))) break;
                 after_sync();
                 uint32_t r[32];
                 tmem_ld_frag(tm + (static_cast<uint32_t>(warp * 32) << 16) + L::kSc, r);
@@ -317,7 +359,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     }
                 }
                 // the chunk before has been read: by the matrix unit, and where v was not finite by the output warps
-                if (c && !bar_wait(&s.o_free, at.par ^ 1, &s)) break;
+                if (c && !(ok = bar_wait(&s.o_free, par ^ 1, &s))) break;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int ch = (j ^ ra % 8) << 4;             // (rb is the same row of its atom)
@@ -330,12 +372,18 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 }
                 to_async();
                 warp_arrive(&s.p_full);
-                warp_arrive(&s.empty[st]);
+            }
+            warp_arrive(&s.empty[st]);
+            at.next();
+            if (c + 1 < chunks) {
+                if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
+                if (!(ok = bar_wait(&s.u_full, par, &s))) break;  // the matrix unit has read the last wK
+                put_keys<DK>(gen, s, at.st, tid);
             }
         }
     } else if (warp < 12) {
         // ---- the state: value column d, dk columns [k0, k0 + HC) ----
-        const int wg = (warp - 4) / 4, quad = warp % 4, d = quad * 32 + lane, k0 = wg * HC, me = tid - 128;
+        const int wg = (warp - 4) / 4, quad = warp % 4, d = quad * 32 + lane, k0 = wg * HC;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         float S[HC];
         const float* from = nullptr;
@@ -361,37 +409,13 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             before_sync();
             warp_arrive(&s.s_full);
         };
-        auto put_keys = [&](int st) {              // a stage's K decayed to the chunk's end, three pieces
-            const uint8_t* K = gen + st * L::kStage + L::kTile;
-#pragma unroll
-            for (int i = 0; i < kChunk * DK / 8 / 256; ++i) {
-                const int e = me + i * 256, r = e / (DK / 8), ch = e % (DK / 8);
-                const uint32_t at = piece_at(r, ch);
-                const uint4 u = *reinterpret_cast<const uint4*>(K + at);
-                const float w = s.wk[st][r];
-                float2 f[4] = {unpack2(u.x), unpack2(u.y), unpack2(u.z), unpack2(u.w)};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) f[j].x *= w, f[j].y *= w;
-#pragma unroll
-                for (int m = 0; m < 3; ++m) {
-                    uint4 o;
-                    o.x = take(f[0].x, f[0].y); o.y = take(f[1].x, f[1].y);
-                    o.z = take(f[2].x, f[2].y); o.w = take(f[3].x, f[3].y);
-                    *reinterpret_cast<uint4*>(gen + L::kWk + m * L::kTile + at) = o;
-                }
-            }
-            to_async();
-            warp_arrive(&s.wk_full);
-        };
         if (OUT) put_pieces();
-        bool ok = bar_wait(&s.full[0], 0, &s);
-        if (ok) put_keys(0);
         Turn at;
-        for (int c = 0; ok && c < chunks; ++c) {
+        for (int c = 0; c < chunks; ++c, at.next()) {
             const int st = at.st;
-            const uint32_t par = at.par;
-            const float gam = s.gam[st];           // (its stage is full)
-            if (!(ok = bar_wait(&s.u_full, par, &s))) break;
+            if (!bar_wait(&s.full[st], at.ph, &s)) break;
+            const float gam = s.gam[st];
+            if (!bar_wait(&s.u_full, at.par, &s)) break;
             after_sync();
             bool odd = false;
 #pragma unroll
@@ -411,15 +435,10 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 warp_arrive(&s.checked[st]);
             }
             warp_arrive(&s.empty[st]);
-            at.next();
-            if (c + 1 < chunks) {
-                if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
-                put_keys(at.st);
-                if (OUT) {
-                    if (!(ok = bar_wait(&s.qs_full, par, &s))) break;
-                    after_sync();
-                    put_pieces();
-                }
+            if (OUT && c + 1 < chunks) {
+                if (!bar_wait(&s.qs_full, at.par, &s)) break;
+                after_sync();
+                put_pieces();
             }
         }
         float* to = nullptr;
@@ -430,81 +449,115 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             for (int i = 0; i < HC; ++i)
                 if (k0 + i < a.dk) to[static_cast<size_t>(k0 + i) * a.dv + c0 + d] = S[i];
     } else if (warp < 16) {
-        // ---- carried, inner -> out: value column d, 64 tokens ----
-        if constexpr (OUT) {
-            const int d = (warp - 12) * 32 + lane;
-            const uint32_t lanes = static_cast<uint32_t>((warp - 12) * 32) << 16;
-            const int stride = static_cast<int>(a.out_row);
-            Turn at;
-            for (int c = 0; c < chunks; ++c, at.next()) {
-                const int st = at.st, n = min(kChunk, count - c * kChunk);
-                if (!bar_wait(&s.full[st], at.ph, &s)) break;
-                if (!bar_wait(&s.checked[st], at.ph, &s)) break;
+        // ---- carried, inner -> out: 32 value columns a warp, 64 tokens; wK ----
+        const int ow = warp - 12, d = ow * 32 + lane, cols = min(32, width - ow * 32);
+        const uint32_t lanes = static_cast<uint32_t>(ow * 32) << 16;
+        Turn at;
+        bool ok = bar_wait(&s.full[0], 0, &s);
+        if (ok) put_keys<DK>(gen, s, 0, tid - 256);
+        for (int c = 0; ok && c < chunks; ++c) {
+            const int st = at.st, n = min(kChunk, count - c * kChunk);
+            const uint32_t par = at.par, ph = at.ph;
+            at.next();
+            if (c + 1 < chunks) {
+                if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
+                if (!(ok = bar_wait(&s.u_full, par, &s))) break;  // the matrix unit has read the last wK
+                put_keys<DK>(gen, s, at.st, tid - 256);
+            }
+            if constexpr (OUT) {
+                if (!(ok = bar_wait(&s.checked[st], ph, &s))) break;
                 const bool odd = s.odd[st] != 0;
-                if (!bar_wait(&s.o_full, at.par, &s)) break;
+                if (!(ok = bar_wait(&s.o_full, par, &s))) break;
                 after_sync();
-                uint32_t y[kChunk / 2];            // outputs, two tokens a word
+                uint8_t* const tile = gen + L::out_at(st) + ow * (kChunk * 64);
+                const uint32_t tile_at = smem_addr(tile);
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    uint32_t r[16], u[16];
-                    tmem_ld16(tm + lanes + L::kO1 + b * 16, r);
-                    tmem_ld16(tm + lanes + L::kO2 + b * 16, u);
+                for (int half = 0; half < 2; ++half) {            // 16 value columns
+                    uint32_t r[32], u[32];
+                    tmem_ld_frag(tm + lanes + (static_cast<uint32_t>(half * 16) << 16) + L::kO1, r);
+                    tmem_ld_frag(tm + lanes + (static_cast<uint32_t>(half * 16) << 16) + L::kO2, u);
                     ld_wait(r);
                     ld_wait(u);
+                    if (half == 1 && !odd) {
+                        before_sync();
+                        warp_arrive(&s.o_free);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const float4 e = *reinterpret_cast<const float4*>(&s.eg[st][b * 16 + i]);
-                        y[b * 8 + i / 2] = pack2(fmaf(e.x, __uint_as_float(r[i]), __uint_as_float(u[i])),
-                                                 fmaf(e.y, __uint_as_float(r[i + 1]), __uint_as_float(u[i + 1])));
-                        y[b * 8 + i / 2 + 1] = pack2(fmaf(e.z, __uint_as_float(r[i + 2]), __uint_as_float(u[i + 2])),
-                                                     fmaf(e.w, __uint_as_float(r[i + 3]), __uint_as_float(u[i + 3])));
+                    for (int j = 0; j < 8; j += 2) {              // tokens j * 8 .. + 16
+                        uint32_t m[4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float2 e = *reinterpret_cast<const float2*>(&s.eg[st][(j + i) * 8 + lane % 4 * 2]);
+                            const uint32_t *x = r + (j + i) * 4, *z = u + (j + i) * 4;
+                            m[2 * i] = pack2(fmaf(e.x, __uint_as_float(x[0]), __uint_as_float(z[0])),
+                                             fmaf(e.y, __uint_as_float(x[1]), __uint_as_float(z[1])));
+                            m[2 * i + 1] = pack2(fmaf(e.x, __uint_as_float(x[2]), __uint_as_float(z[2])),
+                                                 fmaf(e.y, __uint_as_float(x[3]), __uint_as_float(z[3])));
+                        }
+                        // matrices: (tokens j, columns 0-7), (j, 8-15), (j + 1, 0-7), (j + 1, 8-15)
+                        stmatrix4_trans(tile_at + out_piece((j + lane / 16) * 8 + lane % 8, half * 2 + lane / 8 % 2), m);
                     }
                 }
-                T* const p = static_cast<T*>(a.out) + (row0 + static_cast<long long>(c) * kChunk) * a.out_row + h * a.out_head + c0 + d;
-                if (!odd) {
-                    before_sync();
-                    warp_arrive(&s.o_free);
-#pragma unroll
-                    for (int i = 0; i < kChunk; ++i)
-                        if (i < n && d < width)
-                            p[static_cast<long long>(i) * stride] =
-                                __ushort_as_bfloat16(static_cast<unsigned short>(i % 2 ? y[i / 2] >> 16 : y[i / 2] & 0xFFFFu));
-                } else {
-                    // A value in this chunk was not finite: if it is in this column, the product with
+                __syncwarp();
+                if (odd) {
+                    // A value in this chunk was not finite: if it is in this lane's column, the product with
                     // masked zeros has reached the tokens before it.  Their inner sums again, one by one.
                     const uint8_t* V = gen + st * L::kStage + 2 * L::kTile;
+                    const uint8_t* P = gen + L::kP;
                     auto value = [&](int t) {
                         return __bfloat162float(*reinterpret_cast<const T*>(V + piece_at(t, d / 8) + d % 8 * 2));
                     };
                     int bad = 0;
                     while (bad < n && finite(value(bad))) ++bad;
-                    const uint8_t* P = gen + L::kP;
                     for (int i = 0; i < n; ++i) {
-                        uint32_t o1, o2;
+                        uint32_t o1;
                         __syncwarp();
                         asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o1) : "r"(tm + lanes + L::kO1 + i));
-                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o2) : "r"(tm + lanes + L::kO2 + i));
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(o1), "+r"(o2) :: "memory");
-                        float inner = __uint_as_float(o2);
-                        if (bad < n) {
-                            inner = i < bad ? 0.0f : __int_as_float(0x7FC00000);
-                            if (i < bad)
-                                for (int t = 0; t <= i; ++t) {
-                                    const uint32_t at_p = piece_at(i, t / 8) + t % 8 * 2;
-                                    const float w = __bfloat162float(*reinterpret_cast<const T*>(P + at_p)) +
-                                                    __bfloat162float(*reinterpret_cast<const T*>(P + kBlk + at_p));
-                                    inner = fmaf(w, value(t), inner);
-                                }
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(o1) :: "memory");
+                        if (bad == n) continue;
+                        float inner = __int_as_float(0x7FC00000);
+                        if (i < bad) {
+                            inner = 0.0f;
+                            for (int t = 0; t <= i; ++t) {
+                                const uint32_t at_p = piece_at(i, t / 8) + t % 8 * 2;
+                                inner = fmaf(__bfloat162float(*reinterpret_cast<const T*>(P + at_p)) +
+                                                 __bfloat162float(*reinterpret_cast<const T*>(P + kBlk + at_p)),
+                                             value(t), inner);
+                            }
                         }
-                        if (d < width)
-                            p[static_cast<long long>(i) * stride] = __float2bfloat16_rn(fmaf(s.eg[st][i], __uint_as_float(o1), inner));
+                        *reinterpret_cast<T*>(tile + out_piece(i, lane / 8) + lane % 8 * 2) =
+                            __float2bfloat16_rn(fmaf(s.eg[st][i], __uint_as_float(o1), inner));
                     }
                     before_sync();
                     warp_arrive(&s.o_free);
                 }
-                warp_arrive(&s.empty[st]);
+                const long long row = row0 + static_cast<long long>(c) * kChunk;
+                to_async();                        // before the store reads the tile, and the next copy writes it
+                __syncwarp();
+                if (cols > 0 && tma_out && n == kChunk) {
+                    if (lane == 0) {
+                        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
+                                     :: "l"(&maps.out), "r"(c0 + ow * 32), "r"(h), "r"(static_cast<int>(row)), "r"(tile_at) : "memory");
+                        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+                    }
+                } else if (cols > 0) {
+                    T* const p = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + c0 + ow * 32;
+                    for (int i = lane; i < n * 4; i += 32) {
+                        const int t = i / 4, ch = i % 4;
+                        const uint8_t* from = tile + out_piece(t, ch);
+                        T* to = p + t * a.out_row + ch * 8;
+                        if (tma_out && ch * 8 + 8 <= cols) {
+                            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+                        } else {
+                            for (int j = 0; j < 8; ++j)
+                                if (ch * 8 + j < cols) to[j] = reinterpret_cast<const T*>(from)[j];
+                        }
+                    }
+                }
             }
+            warp_arrive(&s.empty[st]);
         }
+        // (the last stores read shared memory that outlives them: wait_group.read above)
     } else if (warp == 16 || warp == 19) {
         // ---- tiles ----
         const int t = lane + (warp == 19 ? 32 : 0), hq = h / a.q_share, hk = h / a.k_share;
@@ -563,18 +616,21 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             g = ahead;
         }
         if (!OUT && lane == 0 && blockIdx.x == 0) seg_decay[static_cast<size_t>(blockIdx.z) * a.heads + h] = total;
-    } else if (lane == 0) {
-        // ---- matrix instructions ----
+    } else {
+        // ---- matrix instructions: the warp as one, one lane issues ----
         constexpr uint32_t id_sc = umma_idesc(64, 64, 0, 0), id_u = umma_idesc(128, DK, 1, 1), id_q = umma_idesc(128, 64, 0, 0),
                            id_p = umma_idesc(128, 64, 1, 0);
         const uint32_t wk_desc = mn_major(base + L::kWk), p_desc = k_major(base + L::kP);
         auto scores = [&](int st) {
             const uint32_t q = k_major(base + st * L::kStage), k = k_major(base + st * L::kStage + L::kTile);
+            if (elect()) {
 #pragma unroll
-            for (int i = 0; i < DK / 16; ++i) umma_ss<id_sc>(tm + L::kSc, q + k_step(i), k + k_step(i), i > 0);
-            commit(&s.sc_full);
+                for (int i = 0; i < DK / 16; ++i) umma_ss<id_sc>(tm + L::kSc, q + k_step(i), k + k_step(i), i > 0);
+                commit(&s.sc_full);
+            }
+            __syncwarp();
         };
-        bool ok = lane_wait(&s.full[0], 0, &s);
+        bool ok = bar_wait(&s.full[0], 0, &s);
         after_sync();
         if (OUT && ok) scores(0);
         Turn at;
@@ -582,39 +638,49 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             const uint32_t par = at.par, prev = par ^ 1, tiles = base + at.st * L::kStage;
             const uint32_t q = k_major(tiles), v = mn_major(tiles + 2 * L::kTile);
             const int st = at.st;
-            if (!(ok = lane_wait(&s.wk_full, par, &s))) break;
-            if (c && !(ok = lane_wait(&s.u_free, prev, &s))) break;
+            if (!(ok = bar_wait(&s.wk_full, par, &s))) break;
+            if (c && !(ok = bar_wait(&s.u_free, prev, &s))) break;
             after_sync();
+            if (elect()) {
 #pragma unroll
-            for (int i = 0; i < kChunk / 16; ++i)
+                for (int i = 0; i < kChunk / 16; ++i)
 #pragma unroll
-                for (int m = 0; m < 3; ++m)
-                    umma_ss<id_u>(tm + L::kU, v + mn_step(i), wk_desc + (m * L::kTile >> 4) + mn_step(i), i + m > 0);
-            commit(&s.u_full);
-            if constexpr (OUT) {
-                if (!(ok = lane_wait(&s.s_full, par, &s))) break;
-                if (c && !(ok = lane_wait(&s.o_free, prev, &s))) break;
-                after_sync();
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < DK / 16; ++i)
-                        umma_ts<id_q>(tm + L::kO1, tm + L::kS + m * (DK / 2) + i * 8, q + k_step(i), m + i > 0);
-                commit(&s.qs_full);
-                if (!(ok = lane_wait(&s.p_full, par, &s))) break;
-                after_sync();
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < kChunk / 16; ++i)
-                        umma_ss<id_p>(tm + L::kO2, v + mn_step(i), p_desc + (m * kBlk >> 4) + k_step(i), m + i > 0);
-                commit(&s.o_full);
+                    for (int m = 0; m < 3; ++m)
+                        umma_ss<id_u>(tm + L::kU, v + mn_step(i), wk_desc + (m * L::kTile >> 4) + mn_step(i), i + m > 0);
+                commit(&s.u_full);
             }
-            commit(&s.empty[st]);
+            __syncwarp();
+            if constexpr (OUT) {
+                if (!(ok = bar_wait(&s.s_full, par, &s))) break;
+                if (c && !(ok = bar_wait(&s.o_free, prev, &s))) break;
+                after_sync();
+                if (elect()) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int i = 0; i < DK / 16; ++i)
+                            umma_ts<id_q>(tm + L::kO1, tm + L::kS + m * (DK / 2) + i * 8, q + k_step(i), m + i > 0);
+                    commit(&s.qs_full);
+                }
+                __syncwarp();
+                if (!(ok = bar_wait(&s.p_full, par, &s))) break;
+                after_sync();
+                if (elect()) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int i = 0; i < kChunk / 16; ++i)
+                            umma_ss<id_p>(tm + L::kO2, v + mn_step(i), p_desc + (m * kBlk >> 4) + k_step(i), m + i > 0);
+                    commit(&s.o_full);
+                }
+                __syncwarp();
+            }
+            if (elect()) commit(&s.empty[st]);
+            __syncwarp();
             at.next();
             if (OUT && c + 1 < chunks) {
-                if (!(ok = lane_wait(&s.full[at.st], at.ph, &s))) break;
-                if (!(ok = lane_wait(&s.sc_free, par, &s))) break;
+                if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
+                if (!(ok = bar_wait(&s.sc_free, par, &s))) break;
                 after_sync();
                 scores(at.st);
             }
@@ -649,17 +715,18 @@ inline EncodeTiled encode_tiled() {
     return f;
 }
 
-// The map of a [rows][heads][width] bf16 tensor in boxes of 64 columns and 64
-// rows of one head, zeros beyond the width.  false: not a tensor TMA takes
+// The map of a [rows][heads][width] bf16 tensor in boxes of `cols` columns (64:
+// 128-byte swizzle, 32: 64-byte) and 64 rows of one head, zeros beyond the width.  false: not a tensor TMA takes
 // (a broadcast stride); its tiles go by 16-byte copies.
-inline bool tensor_map(CUtensorMap* m, const void* p, int width, int heads, int rows, long long head, long long row) {
+inline bool tensor_map(CUtensorMap* m, const void* p, int width, int heads, int rows, long long head, long long row,
+                       int cols = 64) {
     if ((heads > 1 && head <= 0) || (rows > 1 && row <= 0) || !encode_tiled()) return false;
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(std::max(heads > 1 ? head : 8LL, 8LL)) * 2,
                                    static_cast<cuuint64_t>(std::max(rows > 1 ? row : 8LL, 8LL)) * 2};
-    const cuuint32_t box[3] = {64, 1, kChunk}, one[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(cols), 1, kChunk}, one[3] = {1, 1, 1};
     return encode_tiled()(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, one,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
