@@ -14,10 +14,12 @@
 // and, in registers, S <- e^{G_C} S + update, out = scale (e^{G_t} carried + inner).
 //
 // Roles (20 warps, one CTA per SM):
-//     warps 0-3    scores -> P: pieces to shared memory; half of the wK pieces
+//     warps 0-3    scores -> P: pieces to shared memory
 //     warps 4-11   the state, half of dk each group: update -> S, pieces of S to
 //                  tensor memory
-//     warps 12-15  carried, inner -> out, through shared memory; half of the wK pieces
+//     warps 12-15  carried, inner -> out, through shared memory
+//     (and all of these: wK pieces to shared memory, as soon as the update
+//     before has read the last ones)
 //     warps 16, 19 tiles into shared memory (three stages): whole chunks by TMA,
 //                  a sequence's last, partial one by 16-byte copies with zeros
 //     warp 17      decay sums
@@ -42,10 +44,14 @@ template <int DK> struct Plan {
     static constexpr int kTile = DK / 64 * kBlk;  // Q or K of one stage
     static constexpr int kVTile = 2 * kBlk;
     static constexpr int kStage = 2 * kTile + kVTile;
-    static constexpr int kWk = kStages * kStage, kP = kWk + 3 * kTile, kEnd = kP + 2 * kBlk + (DK < 128 ? 2 * kBlk : 0);
-    // a chunk's outputs: in the place of its Q, which both its products have
-    // read, where that is large enough
-    __host__ __device__ static constexpr int out_at(int st) { return DK < 128 ? kP + 2 * kBlk : st * kStage; }
+    static constexpr int kWk = kStages * kStage, kOwn = kWk + 3 * kTile, kEnd = kOwn + (DK < 128 ? 6 * kBlk : 0);
+    // A chunk's P and outputs take the place of its K and Q, which the products
+    // before have read, where those are large enough; else P has two buffers
+    // in turn and the outputs one.
+    __host__ __device__ static constexpr int p_at(int st, int par) {
+        return DK < 128 ? kOwn + par * 2 * kBlk : st * kStage + kTile;
+    }
+    __host__ __device__ static constexpr int out_at(int st) { return DK < 128 ? kOwn + 4 * kBlk : st * kStage; }
     static constexpr int bytes = kEnd + 1024;     // + alignment slack
     // tensor memory columns
     static constexpr int kU = 0, kSc = DK, kO1 = DK + 64, kO2 = DK + 128, kS = DK + 192;
@@ -174,6 +180,14 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t addr, uint32_t (&r)[32]) {
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
+__device__ __forceinline__ void tmem_ld_frag(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
 // Waits for the loads of r (its operands, so that nothing uses them earlier).
 __device__ __forceinline__ void ld_wait(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -198,6 +212,12 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) 
 // 16-byte piece `ch` of row r in a tile of 64-column blocks.
 __device__ __forceinline__ uint32_t piece_at(int r, int ch) {
     return static_cast<uint32_t>(ch / 8 * kBlk + r * kSwRow + ((ch % 8 ^ r % 8) << 4));
+}
+// The next bf16 piece of a pair, packed; what is left stays in it.
+__device__ __forceinline__ uint32_t take2(float2& x) {
+    const uint32_t p = pack2(x.x, x.y);
+    x = __ffma2_rn(unpack2(p), make_float2(-1.0f, -1.0f), x);
+    return p;
 }
 // A 64-column, 64-row box of a [rows][heads][columns] tensor map.
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint64_t* bar) {
@@ -234,24 +254,24 @@ struct Maps {
     CUtensorMap q, k, v, out;
 };
 
-// A stage's K decayed to its chunk's end, as three bf16 pieces; thread t of 256.
+// A stage's K decayed to its chunk's end, as three bf16 pieces; thread t of the
+// 512 of the P, state and output warps.
 template <int DK> __device__ __forceinline__ void put_keys(uint8_t* gen, Side& s, int st, int t) {
     using L = Plan<DK>;
     const uint8_t* K = gen + st * L::kStage + L::kTile;
-#pragma unroll
-    for (int i = 0; i < kChunk * DK / 8 / 256; ++i) {
-        const int e = t + i * 256, r = e / (DK / 8), ch = e % (DK / 8);
+#pragma unroll 1
+    for (int i = 0; i < kChunk * DK / 8 / 512; ++i) {
+        const int e = t + i * 512, r = e / (DK / 8), ch = e % (DK / 8);
         const uint32_t at = piece_at(r, ch);
         const uint4 u = *reinterpret_cast<const uint4*>(K + at);
-        const float w = s.wk[st][r];
+        const float2 w = make_float2(s.wk[st][r], s.wk[st][r]);
         float2 f[4] = {unpack2(u.x), unpack2(u.y), unpack2(u.z), unpack2(u.w)};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j].x *= w, f[j].y *= w;
+        for (int j = 0; j < 4; ++j) f[j] = __fmul2_rn(f[j], w);
 #pragma unroll
         for (int m = 0; m < 3; ++m) {
             uint4 o;
-            o.x = take(f[0].x, f[0].y); o.y = take(f[1].x, f[1].y);
-            o.z = take(f[2].x, f[2].y); o.w = take(f[3].x, f[3].y);
+            o.x = take2(f[0]); o.y = take2(f[1]); o.z = take2(f[2]); o.w = take2(f[3]);
             *reinterpret_cast<uint4*>(gen + L::kWk + m * L::kTile + at) = o;
         }
     }
@@ -301,7 +321,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             bar_init(&s.checked[i], 8);
         }
         bar_init(&s.sc_full, 1); bar_init(&s.sc_free, 4); bar_init(&s.p_full, 4);
-        bar_init(&s.o_full, 1); bar_init(&s.o_free, 4); bar_init(&s.wk_full, 8);
+        bar_init(&s.o_full, 1); bar_init(&s.o_free, 4); bar_init(&s.wk_full, 16);
         bar_init(&s.u_full, 1); bar_init(&s.u_free, 8); bar_init(&s.s_full, 8); bar_init(&s.qs_full, 1);
         s.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -321,11 +341,13 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
     after_sync();
     const uint32_t tm = s.tmem;
 
+    // Registers go from the small roles to the state's: launched with 96 a
+    // thread (640 x 96 = 61,440), then 80, 120, 120, 96 and 56 a warpgroup
+    // (60,416).
     if (warp < 4) {
         // ---- scores -> P; wK ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const int ra = warp * 16 + lane / 4, rb = ra + 8, t2 = lane % 4 * 2;
-        uint8_t* const pa = gen + L::kP + ra * kSwRow + t2 * 2;
-        uint8_t* const pb = pa + 8 * kSwRow;
         Turn at;
         bool ok = bar_wait(&s.full[0], 0, &s);
         if (ok) put_keys<DK>(gen, s, 0, tid);
@@ -335,40 +357,41 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             if constexpr (OUT) {
                 const float2 ga = s.g[st][ra], gb = s.g[st][rb];
                 if (!(ok = bar_wait(&s.sc_full, par, &s))) break;
+                // (where P takes K's place, its pieces have been made by all warps)
+                if (DK == 128 && !(ok = bar_wait(&s.wk_full, par, &s))) break;
                 after_sync();
-                uint32_t r[32];
-                tmem_ld_frag(tm + (static_cast<uint32_t>(warp * 32) << 16) + L::kSc, r);
-                ld_wait(r);
-                before_sync();
-                warp_arrive(&s.sc_free);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (j * 8 > warp * 16 + 15) {                 // wholly above the diagonal
-                        r[j * 4] = r[j * 4 + 1] = r[j * 4 + 2] = r[j * 4 + 3] = 0;
-                        continue;
+                uint8_t* const pa = gen + L::p_at(st, par) + ra * kSwRow + t2 * 2;
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {            // (unrolled code would not stay in the instruction cache)
+                    uint32_t r[16];
+                    tmem_ld_frag(tm + (static_cast<uint32_t>(warp * 32) << 16) + L::kSc + half * 32, r);
+                    ld_wait(r);
+                    if (half == 1) {
+                        before_sync();
+                        warp_arrive(&s.sc_free);
                     }
-                    const float4 g = *reinterpret_cast<const float4*>(&s.g[st][j * 8 + t2]);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int col = j * 8 + t2 + e;
-                        const float hs = e ? g.z : g.x, ls = e ? g.w : g.y;
-                        const float xa = __uint_as_float(r[j * 4 + e]) * exp2_fast((ga.x - hs) + (ga.y - ls)) * a.scale;
-                        const float xb = __uint_as_float(r[j * 4 + 2 + e]) * exp2_fast((gb.x - hs) + (gb.y - ls)) * a.scale;
-                        r[j * 4 + e] = col <= ra ? __float_as_uint(xa) : 0u;
-                        r[j * 4 + 2 + e] = col <= rb ? __float_as_uint(xb) : 0u;
+                    for (int j = 0; j < 4; ++j) {
+                        const int col = half * 32 + j * 8 + t2;
+                        const float4 g = *reinterpret_cast<const float4*>(&s.g[st][col]);
+                        auto decayed = [&](float2 row, int e) {   // row's two scores from register e on
+                            const float2 hi2 = __fadd2_rn(make_float2(row.x, row.x), make_float2(-g.x, -g.z));
+                            const float2 x = __fadd2_rn(hi2, __fadd2_rn(make_float2(row.y, row.y), make_float2(-g.y, -g.w)));
+                            return __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])),
+                                                         make_float2(exp2_fast(x.x), exp2_fast(x.y))),
+                                              make_float2(a.scale, a.scale));
+                        };
+                        float2 x = decayed(ga, j * 4), y = decayed(gb, j * 4 + 2);
+                        if (col > ra) x.x = 0.0f;
+                        if (col + 1 > ra) x.y = 0.0f;
+                        if (col > rb) y.x = 0.0f;
+                        if (col + 1 > rb) y.y = 0.0f;
+                        uint8_t* const to = pa + (((half * 4 + j) ^ ra % 8) << 4);   // (rb is the same row of its atom)
+                        *reinterpret_cast<uint32_t*>(to) = take2(x);
+                        *reinterpret_cast<uint32_t*>(to + kBlk) = pack2(x.x, x.y);
+                        *reinterpret_cast<uint32_t*>(to + 8 * kSwRow) = take2(y);
+                        *reinterpret_cast<uint32_t*>(to + 8 * kSwRow + kBlk) = pack2(y.x, y.y);
                     }
-                }
-                // the chunk before has been read: by the matrix unit, and where v was not finite by the output warps
-                if (c && !(ok = bar_wait(&s.o_free, par ^ 1, &s))) break;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int ch = (j ^ ra % 8) << 4;             // (rb is the same row of its atom)
-                    float x0 = __uint_as_float(r[j * 4]), x1 = __uint_as_float(r[j * 4 + 1]);
-                    float y0 = __uint_as_float(r[j * 4 + 2]), y1 = __uint_as_float(r[j * 4 + 3]);
-                    *reinterpret_cast<uint32_t*>(pa + ch) = take(x0, x1);
-                    *reinterpret_cast<uint32_t*>(pa + kBlk + ch) = pack2(x0, x1);
-                    *reinterpret_cast<uint32_t*>(pb + ch) = take(y0, y1);
-                    *reinterpret_cast<uint32_t*>(pb + kBlk + ch) = pack2(y0, y1);
                 }
                 to_async();
                 warp_arrive(&s.p_full);
@@ -383,24 +406,35 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         }
     } else if (warp < 12) {
         // ---- the state: value column d, dk columns [k0, k0 + HC) ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
         const int wg = (warp - 4) / 4, quad = warp % 4, d = quad * 32 + lane, k0 = wg * HC;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-        float S[HC];
+        float2 S[HC / 2];
         const float* from = nullptr;
         if (OUT && seg > 0) from = seg_state + (static_cast<size_t>(blockIdx.z - 1) * a.heads + h) * head_state;
         else if (OUT && slot >= 0) from = a.state + (static_cast<size_t>(slot) * a.heads + h) * head_state;
+        {
+            const bool there = from && d < width;
+            const float* p = there ? from + static_cast<size_t>(k0) * a.dv + c0 + d : nullptr;
+            int left = there ? a.dk - k0 : 0;
 #pragma unroll
-        for (int i = 0; i < HC; ++i)
-            S[i] = from && d < width && k0 + i < a.dk ? from[static_cast<size_t>(k0 + i) * a.dv + c0 + d] : 0.0f;
+            for (int i = 0; i < HC / 2; ++i) {
+                S[i].x = left > 0 ? *p : 0.0f;
+                p += a.dv;
+                S[i].y = left > 1 ? *p : 0.0f;
+                p += a.dv;
+                left -= 2;
+            }
+        }
         auto put_pieces = [&]() {                  // S as two bf16 pieces, two columns a word
 #pragma unroll
             for (int b = 0; b < HC / 16; ++b) {
                 uint32_t big[8], small[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    float x = S[b * 16 + 2 * i], y = S[b * 16 + 2 * i + 1];
-                    big[i] = take(x, y);
-                    small[i] = pack2(x, y);
+                    float2 x = S[b * 8 + i];
+                    big[i] = take2(x);
+                    small[i] = pack2(x.x, x.y);
                 }
                 tmem_st8(tm + lanes + L::kS + k0 / 2 + b * 8, big);
                 tmem_st8(tm + lanes + L::kS + DK / 2 + k0 / 2 + b * 8, small);
@@ -411,11 +445,13 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         };
         if (OUT) put_pieces();
         Turn at;
-        for (int c = 0; c < chunks; ++c, at.next()) {
+        bool ok = bar_wait(&s.full[0], 0, &s);
+        if (ok) put_keys<DK>(gen, s, 0, tid);
+        for (int c = 0; ok && c < chunks; ++c) {
             const int st = at.st;
-            if (!bar_wait(&s.full[st], at.ph, &s)) break;
-            const float gam = s.gam[st];
-            if (!bar_wait(&s.u_full, at.par, &s)) break;
+            const uint32_t par = at.par;
+            const float2 gam = make_float2(s.gam[st], s.gam[st]);
+            if (!(ok = bar_wait(&s.u_full, par, &s))) break;
             after_sync();
             bool odd = false;
 #pragma unroll
@@ -426,7 +462,9 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 // every column of this lane has every v of value column d as a factor
                 if (b == 0) odd = (u[0] & 0x7F800000u) == 0x7F800000u;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) S[b * 16 + i] = fmaf(gam, S[b * 16 + i], __uint_as_float(u[i]));
+                for (int i = 0; i < 8; ++i)
+                    S[b * 8 + i] = __ffma2_rn(gam, S[b * 8 + i],
+                                              make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])));
             }
             before_sync();
             warp_arrive(&s.u_free);
@@ -435,26 +473,40 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 warp_arrive(&s.checked[st]);
             }
             warp_arrive(&s.empty[st]);
-            if (OUT && c + 1 < chunks) {
-                if (!bar_wait(&s.qs_full, at.par, &s)) break;
-                after_sync();
-                put_pieces();
+            at.next();
+            if (c + 1 < chunks) {
+                if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
+                put_keys<DK>(gen, s, at.st, tid);
+                if (OUT) {
+                    if (!(ok = bar_wait(&s.qs_full, par, &s))) break;
+                    after_sync();
+                    put_pieces();
+                }
             }
         }
         float* to = nullptr;
         if (!OUT) to = seg_state + (static_cast<size_t>(blockIdx.z) * a.heads + h) * head_state;
         else if (seg == nseg - 1 && slot >= 0) to = a.state + (static_cast<size_t>(slot) * a.heads + h) * head_state;
-        if (to && d < width)
+        if (to && d < width) {
+            float* p = to + static_cast<size_t>(k0) * a.dv + c0 + d;
+            int left = a.dk - k0;
 #pragma unroll
-            for (int i = 0; i < HC; ++i)
-                if (k0 + i < a.dk) to[static_cast<size_t>(k0 + i) * a.dv + c0 + d] = S[i];
+            for (int i = 0; i < HC / 2; ++i) {
+                if (left > 0) *p = S[i].x;
+                p += a.dv;
+                if (left > 1) *p = S[i].y;
+                p += a.dv;
+                left -= 2;
+            }
+        }
     } else if (warp < 16) {
         // ---- carried, inner -> out: 32 value columns a warp, 64 tokens; wK ----
         const int ow = warp - 12, d = ow * 32 + lane, cols = min(32, width - ow * 32);
         const uint32_t lanes = static_cast<uint32_t>(ow * 32) << 16;
+        int before = 0;                            // the stage of the chunk before
         Turn at;
         bool ok = bar_wait(&s.full[0], 0, &s);
-        if (ok) put_keys<DK>(gen, s, 0, tid - 256);
+        if (ok) put_keys<DK>(gen, s, 0, tid);
         for (int c = 0; ok && c < chunks; ++c) {
             const int st = at.st, n = min(kChunk, count - c * kChunk);
             const uint32_t par = at.par, ph = at.ph;
@@ -462,16 +514,21 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             if (c + 1 < chunks) {
                 if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
                 if (!(ok = bar_wait(&s.u_full, par, &s))) break;  // the matrix unit has read the last wK
-                put_keys<DK>(gen, s, at.st, tid - 256);
+                put_keys<DK>(gen, s, at.st, tid);
             }
             if constexpr (OUT) {
                 if (!(ok = bar_wait(&s.checked[st], ph, &s))) break;
                 const bool odd = s.odd[st] != 0;
                 if (!(ok = bar_wait(&s.o_full, par, &s))) break;
                 after_sync();
+                if (c) {                           // the last chunk's store has read its tile
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    warp_arrive(&s.empty[before]);
+                }
+                before = st;
                 uint8_t* const tile = gen + L::out_at(st) + ow * (kChunk * 64);
                 const uint32_t tile_at = smem_addr(tile);
-#pragma unroll
+#pragma unroll 1
                 for (int half = 0; half < 2; ++half) {            // 16 value columns
                     uint32_t r[32], u[32];
                     tmem_ld_frag(tm + lanes + (static_cast<uint32_t>(half * 16) << 16) + L::kO1, r);
@@ -489,10 +546,12 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                         for (int i = 0; i < 2; ++i) {
                             const float2 e = *reinterpret_cast<const float2*>(&s.eg[st][(j + i) * 8 + lane % 4 * 2]);
                             const uint32_t *x = r + (j + i) * 4, *z = u + (j + i) * 4;
-                            m[2 * i] = pack2(fmaf(e.x, __uint_as_float(x[0]), __uint_as_float(z[0])),
-                                             fmaf(e.y, __uint_as_float(x[1]), __uint_as_float(z[1])));
-                            m[2 * i + 1] = pack2(fmaf(e.x, __uint_as_float(x[2]), __uint_as_float(z[2])),
-                                                 fmaf(e.y, __uint_as_float(x[3]), __uint_as_float(z[3])));
+                            const float2 y0 = __ffma2_rn(e, make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])),
+                                                         make_float2(__uint_as_float(z[0]), __uint_as_float(z[1])));
+                            const float2 y1 = __ffma2_rn(e, make_float2(__uint_as_float(x[2]), __uint_as_float(x[3])),
+                                                         make_float2(__uint_as_float(z[2]), __uint_as_float(z[3])));
+                            m[2 * i] = pack2(y0.x, y0.y);
+                            m[2 * i + 1] = pack2(y1.x, y1.y);
                         }
                         // matrices: (tokens j, columns 0-7), (j, 8-15), (j + 1, 0-7), (j + 1, 8-15)
                         stmatrix4_trans(tile_at + out_piece((j + lane / 16) * 8 + lane % 8, half * 2 + lane / 8 % 2), m);
@@ -503,7 +562,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     // A value in this chunk was not finite: if it is in this lane's column, the product with
                     // masked zeros has reached the tokens before it.  Their inner sums again, one by one.
                     const uint8_t* V = gen + st * L::kStage + 2 * L::kTile;
-                    const uint8_t* P = gen + L::kP;
+                    const uint8_t* P = gen + L::p_at(st, par);
                     auto value = [&](int t) {
                         return __bfloat162float(*reinterpret_cast<const T*>(V + piece_at(t, d / 8) + d % 8 * 2));
                     };
@@ -538,7 +597,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     if (lane == 0) {
                         asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
                                      :: "l"(&maps.out), "r"(c0 + ow * 32), "r"(h), "r"(static_cast<int>(row)), "r"(tile_at) : "memory");
-                        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                 } else if (cols > 0) {
                     T* const p = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + c0 + ow * 32;
@@ -555,11 +614,12 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     }
                 }
             }
-            warp_arrive(&s.empty[st]);
+            if (!OUT) warp_arrive(&s.empty[st]);
         }
-        // (the last stores read shared memory that outlives them: wait_group.read above)
+        if (OUT && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     } else if (warp == 16 || warp == 19) {
         // ---- tiles ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         const int t = lane + (warp == 19 ? 32 : 0), hq = h / a.q_share, hk = h / a.k_share;
         const T* Q = static_cast<const T*>(a.q) + hq * a.q_head + row0 * a.q_row;
         const T* K = static_cast<const T*>(a.k) + hk * a.k_head + row0 * a.k_row;
@@ -596,6 +656,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             }
         }
     } else if (warp == 17) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         // ---- decay sums, the next chunk's values in flight ----
         double total = 0.0;
         Turn at;
@@ -618,9 +679,10 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         if (!OUT && lane == 0 && blockIdx.x == 0) seg_decay[static_cast<size_t>(blockIdx.z) * a.heads + h] = total;
     } else {
         // ---- matrix instructions: the warp as one, one lane issues ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         constexpr uint32_t id_sc = umma_idesc(64, 64, 0, 0), id_u = umma_idesc(128, DK, 1, 1), id_q = umma_idesc(128, 64, 0, 0),
                            id_p = umma_idesc(128, 64, 1, 0);
-        const uint32_t wk_desc = mn_major(base + L::kWk), p_desc = k_major(base + L::kP);
+        const uint32_t wk_desc = mn_major(base + L::kWk);
         auto scores = [&](int st) {
             const uint32_t q = k_major(base + st * L::kStage), k = k_major(base + st * L::kStage + L::kTile);
             if (elect()) {
@@ -637,6 +699,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         for (int c = 0; ok && c < chunks; ++c) {
             const uint32_t par = at.par, prev = par ^ 1, tiles = base + at.st * L::kStage;
             const uint32_t q = k_major(tiles), v = mn_major(tiles + 2 * L::kTile);
+            const uint32_t p_desc = k_major(base + L::p_at(at.st, par));
             const int st = at.st;
             if (!(ok = bar_wait(&s.wk_full, par, &s))) break;
             if (c && !(ok = bar_wait(&s.u_free, prev, &s))) break;
