@@ -123,7 +123,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 }
 __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
     return ok != 0;
 }
@@ -132,23 +132,17 @@ __device__ __forceinline__ unsigned long long now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-// Waits for a phase, two seconds at most; false: give up.  (A try suspends
-// the thread for a while by itself.)
+// Waits for a phase; false: give up.  A try suspends the thread for up to a
+// microsecond or so, and there are 2^21 of them, seconds, before the CTA aborts.
 __device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity, Side* s) {
-    if (bar_try(bar, parity)) return true;
-    unsigned long long t0 = 0;
-    for (unsigned i = 1;; ++i) {
-        if (bar_try(bar, parity)) return true;
-        if (i % 16) continue;
-        if (*reinterpret_cast<volatile int*>(&s->abort)) return false;
-        const unsigned long long t = now_ns();
-        if (!t0) t0 = t;
-        if (t - t0 > 2000000000ull) {
-            *reinterpret_cast<volatile int*>(&s->abort) = 1;
+    for (int i = 1 << 21; !bar_try(bar, parity); --i) {
+        if (i == 0) {
+            s->abort = 1;
             atomicOr(&g_status, kTimedOut);
-            return false;
         }
+        if (*reinterpret_cast<volatile int*>(&s->abort)) return false;
     }
+    return true;
 }
 // The same for a whole warp, which goes on or gives up as one.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, Side* s) {
@@ -242,7 +236,7 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const __nv_bfloat16* p, 
     const int have = max(0, min(16, (width - ch * 8) * 2));
     const __nv_bfloat16* src = p + r0 * stride + ch * 8;
     const long long step = kStep * stride;
-#pragma unroll
+#pragma unroll 2
     for (int i = 0; i < kChunk / kStep; ++i) {
         const int r = r0 + i * kStep, bytes = r < n ? have : 0;
         copy16(dst + piece_at(r, ch), bytes ? src : p, bytes);
@@ -349,16 +343,17 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const int ra = warp * 16 + lane / 4, rb = ra + 8, t2 = lane % 4 * 2;
         Turn at;
-        bool ok = bar_wait(&s.full[0], 0, &s);
-        if (ok) put_keys<DK>(gen, s, 0, tid);
-        for (int c = 0; ok && c < chunks; ++c) {
+        for (int c = 0; c < chunks; ++c, at.next()) {
             const int st = at.st;
             const uint32_t par = at.par;
+            if (!bar_wait(&s.full[st], at.ph, &s)) break;
+            if (c && !bar_wait(&s.u_full, par ^ 1, &s)) break;    // the matrix unit has read the last wK
+            put_keys<DK>(gen, s, st, tid);
             if constexpr (OUT) {
                 const float2 ga = s.g[st][ra], gb = s.g[st][rb];
-                if (!(ok = bar_wait(&s.sc_full, par, &s))) break;
+                if (!bar_wait(&s.sc_full, par, &s)) break;
                 // (where P takes K's place, its pieces have been made by all warps)
-                if (DK == 128 && !(ok = bar_wait(&s.wk_full, par, &s))) break;
+                if (DK == 128 && !bar_wait(&s.wk_full, par, &s)) break;
                 after_sync();
                 uint8_t* const pa = gen + L::p_at(st, par) + ra * kSwRow + t2 * 2;
 #pragma unroll 1
@@ -397,12 +392,6 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 warp_arrive(&s.p_full);
             }
             warp_arrive(&s.empty[st]);
-            at.next();
-            if (c + 1 < chunks) {
-                if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
-                if (!(ok = bar_wait(&s.u_full, par, &s))) break;  // the matrix unit has read the last wK
-                put_keys<DK>(gen, s, at.st, tid);
-            }
         }
     } else if (warp < 12) {
         // ---- the state: value column d, dk columns [k0, k0 + HC) ----
@@ -443,15 +432,19 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             before_sync();
             warp_arrive(&s.s_full);
         };
-        if (OUT) put_pieces();
         Turn at;
-        bool ok = bar_wait(&s.full[0], 0, &s);
-        if (ok) put_keys<DK>(gen, s, 0, tid);
-        for (int c = 0; ok && c < chunks; ++c) {
+        for (int c = 0; c < chunks; ++c, at.next()) {
             const int st = at.st;
             const uint32_t par = at.par;
+            if (!bar_wait(&s.full[st], at.ph, &s)) break;
+            put_keys<DK>(gen, s, st, tid);         // (the update before has been waited for)
+            if (OUT) {
+                if (c && !bar_wait(&s.qs_full, par ^ 1, &s)) break;
+                after_sync();
+                put_pieces();
+            }
             const float2 gam = make_float2(s.gam[st], s.gam[st]);
-            if (!(ok = bar_wait(&s.u_full, par, &s))) break;
+            if (!bar_wait(&s.u_full, par, &s)) break;
             after_sync();
             bool odd = false;
 #pragma unroll
@@ -473,16 +466,6 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 warp_arrive(&s.checked[st]);
             }
             warp_arrive(&s.empty[st]);
-            at.next();
-            if (c + 1 < chunks) {
-                if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
-                put_keys<DK>(gen, s, at.st, tid);
-                if (OUT) {
-                    if (!(ok = bar_wait(&s.qs_full, par, &s))) break;
-                    after_sync();
-                    put_pieces();
-                }
-            }
         }
         float* to = nullptr;
         if (!OUT) to = seg_state + (static_cast<size_t>(blockIdx.z) * a.heads + h) * head_state;
@@ -503,29 +486,27 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         // ---- carried, inner -> out: 32 value columns a warp, 64 tokens; wK ----
         const int ow = warp - 12, d = ow * 32 + lane, cols = min(32, width - ow * 32);
         const uint32_t lanes = static_cast<uint32_t>(ow * 32) << 16;
-        int before = 0;                            // the stage of the chunk before
-        Turn at;
-        bool ok = bar_wait(&s.full[0], 0, &s);
-        if (ok) put_keys<DK>(gen, s, 0, tid);
-        for (int c = 0; ok && c < chunks; ++c) {
-            const int st = at.st, n = min(kChunk, count - c * kChunk);
-            const uint32_t par = at.par, ph = at.ph;
-            at.next();
-            if (c + 1 < chunks) {
-                if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
-                if (!(ok = bar_wait(&s.u_full, par, &s))) break;  // the matrix unit has read the last wK
-                put_keys<DK>(gen, s, at.st, tid);
+        Turn keys, at;                             // of chunk c, of chunk c - 1
+        for (int c = 0; c <= chunks; ++c) {
+            if (c < chunks) {
+                if (!bar_wait(&s.full[keys.st], keys.ph, &s)) break;
+                if (c && !bar_wait(&s.u_full, keys.par ^ 1, &s)) break;  // the matrix unit has read the last wK
+                put_keys<DK>(gen, s, keys.st, tid);
+                if (!OUT) warp_arrive(&s.empty[keys.st]);
+                keys.next();
             }
-            if constexpr (OUT) {
-                if (!(ok = bar_wait(&s.checked[st], ph, &s))) break;
+            if (OUT && c) {
+                const int st = at.st, done = c - 1, n = min(kChunk, count - done * kChunk);
+                const uint32_t par = at.par;
+                if (!bar_wait(&s.checked[st], at.ph, &s)) break;
                 const bool odd = s.odd[st] != 0;
-                if (!(ok = bar_wait(&s.o_full, par, &s))) break;
+                if (!bar_wait(&s.o_full, par, &s)) break;
                 after_sync();
-                if (c) {                           // the last chunk's store has read its tile
+                if (done) {                        // the last chunk's store has read its tile
                     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    warp_arrive(&s.empty[before]);
+                    warp_arrive(&s.empty[st ? st - 1 : kStages - 1]);
                 }
-                before = st;
+                at.next();
                 uint8_t* const tile = gen + L::out_at(st) + ow * (kChunk * 64);
                 const uint32_t tile_at = smem_addr(tile);
 #pragma unroll 1
@@ -590,7 +571,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     before_sync();
                     warp_arrive(&s.o_free);
                 }
-                const long long row = row0 + static_cast<long long>(c) * kChunk;
+                const long long row = row0 + static_cast<long long>(done) * kChunk;
                 to_async();                        // before the store reads the tile, and the next copy writes it
                 __syncwarp();
                 if (cols > 0 && tma_out && n == kChunk) {
@@ -614,7 +595,6 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     }
                 }
             }
-            if (!OUT) warp_arrive(&s.empty[st]);
         }
         if (OUT && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     } else if (warp == 16 || warp == 19) {
