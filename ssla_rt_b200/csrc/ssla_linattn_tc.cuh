@@ -18,8 +18,9 @@
 //     warps 4-11   the state, half of dk each group: update -> S, pieces of S to
 //                  tensor memory
 //     warps 12-15  carried, inner -> out, through shared memory
-//     (and all of these: wK pieces to shared memory, as soon as the update
-//     before has read the last ones)
+//     (wK pieces to shared memory, as soon as the update before has read the
+//     last ones: the state and output warps, and the P warps where they have
+//     no P to make)
 //     warps 16, 19 tiles into shared memory (three stages): whole chunks by TMA,
 //                  a sequence's last, partial one by 16-byte copies with zeros
 //     warp 17      decay sums
@@ -44,14 +45,12 @@ template <int DK> struct Plan {
     static constexpr int kTile = DK / 64 * kBlk;  // Q or K of one stage
     static constexpr int kVTile = 2 * kBlk;
     static constexpr int kStage = 2 * kTile + kVTile;
-    static constexpr int kWk = kStages * kStage, kOwn = kWk + 3 * kTile, kEnd = kOwn + (DK < 128 ? 6 * kBlk : 0);
-    // A chunk's P and outputs take the place of its K and Q, which the products
-    // before have read, where those are large enough; else P has two buffers
-    // in turn and the outputs one.
+    static constexpr int kWk = kStages * kStage, kOwn = kWk + 3 * kTile, kOut = kOwn + (DK < 128 ? 4 * kBlk : 0), kEnd = kOut + 2 * kBlk;
+    // A chunk's P takes the place of its K, which the products before have
+    // read, where that is large enough; else it has two buffers in turn.
     __host__ __device__ static constexpr int p_at(int st, int par) {
         return DK < 128 ? kOwn + par * 2 * kBlk : st * kStage + kTile;
     }
-    __host__ __device__ static constexpr int out_at(int st) { return DK < 128 ? kOwn + 4 * kBlk : st * kStage; }
     static constexpr int bytes = kEnd + 1024;     // + alignment slack
     // tensor memory columns
     static constexpr int kU = 0, kSc = DK, kO1 = DK + 64, kO2 = DK + 128, kS = DK + 192;
@@ -134,7 +133,8 @@ __device__ __forceinline__ unsigned long long now_ns() {
 }
 // Waits for a phase; false: give up.  A try suspends the thread for up to a
 // microsecond or so, and there are 2^21 of them, seconds, before the CTA aborts.
-__device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity, Side* s) {
+// The lanes of a warp wait as one: what they test is one word.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, Side* s) {
     for (int i = 1 << 21; !bar_try(bar, parity); --i) {
         if (i == 0) {
             s->abort = 1;
@@ -143,10 +143,6 @@ __device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity, Side* 
         if (*reinterpret_cast<volatile int*>(&s->abort)) return false;
     }
     return true;
-}
-// The same for a whole warp, which goes on or gives up as one.
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, Side* s) {
-    return __all_sync(0xFFFFFFFFu, lane_wait(bar, parity, s));
 }
 // A last wait for the matrix unit, whether or not the CTA gave up: 100 ms at most.
 __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
@@ -174,13 +170,10 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t addr, uint32_t (&r)[32]) {
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_ld_frag(uint32_t addr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(addr));
+__device__ __forceinline__ void tmem_ld_frag(uint32_t addr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
 }
 // Waits for the loads of r (its operands, so that nothing uses them earlier).
 __device__ __forceinline__ void ld_wait(uint32_t (&r)[32]) {
@@ -195,6 +188,11 @@ __device__ __forceinline__ void ld_wait(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :: "memory");
+}
+__device__ __forceinline__ void ld_wait(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
                  :: "memory");
 }
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
@@ -248,14 +246,14 @@ struct Maps {
     CUtensorMap q, k, v, out;
 };
 
-// A stage's K decayed to its chunk's end, as three bf16 pieces; thread t of the
-// 512 of the P, state and output warps.
-template <int DK> __device__ __forceinline__ void put_keys(uint8_t* gen, Side& s, int st, int t) {
+// A stage's K decayed to its chunk's end, as three bf16 pieces: 16-byte pieces
+// e, e + step, ... below `end`.
+template <int DK> __device__ __forceinline__ void put_keys(uint8_t* gen, Side& s, int st, int e, int end, int step) {
     using L = Plan<DK>;
     const uint8_t* K = gen + st * L::kStage + L::kTile;
 #pragma unroll 1
-    for (int i = 0; i < kChunk * DK / 8 / 512; ++i) {
-        const int e = t + i * 512, r = e / (DK / 8), ch = e % (DK / 8);
+    for (; e < end; e += step) {
+        const int r = e / (DK / 8), ch = e % (DK / 8);
         const uint32_t at = piece_at(r, ch);
         const uint4 u = *reinterpret_cast<const uint4*>(K + at);
         const float2 w = make_float2(s.wk[st][r], s.wk[st][r]);
@@ -307,6 +305,8 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
     const long long row0 = static_cast<long long>(tab.start[seq]) + first;
     const int slot = tab.slot[seq];
     const size_t head_state = static_cast<size_t>(a.dk) * a.dv;
+    // pieces of wK: the state warps' first kOwnKeys, then the others'
+    constexpr int kKeys = kChunk * DK / 8, kOwnKeys = OUT ? (DK == 128 ? 768 : 256) : kKeys / 2;
 
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
@@ -315,7 +315,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             bar_init(&s.checked[i], 8);
         }
         bar_init(&s.sc_full, 1); bar_init(&s.sc_free, 4); bar_init(&s.p_full, 4);
-        bar_init(&s.o_full, 1); bar_init(&s.o_free, 4); bar_init(&s.wk_full, 16);
+        bar_init(&s.o_full, 1); bar_init(&s.o_free, 4); bar_init(&s.wk_full, OUT ? 12 : 16);
         bar_init(&s.u_full, 1); bar_init(&s.u_free, 8); bar_init(&s.s_full, 8); bar_init(&s.qs_full, 1);
         s.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -347,27 +347,48 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             const int st = at.st;
             const uint32_t par = at.par;
             if (!bar_wait(&s.full[st], at.ph, &s)) break;
-            if (c && !bar_wait(&s.u_full, par ^ 1, &s)) break;    // the matrix unit has read the last wK
-            put_keys<DK>(gen, s, st, tid);
-            if constexpr (OUT) {
+            if constexpr (!OUT) {
+                if (c && !bar_wait(&s.u_full, par ^ 1, &s)) break;    // the matrix unit has read the last wK
+                put_keys<DK>(gen, s, st, kOwnKeys + tid, kKeys, 256);
+            } else {
                 const float2 ga = s.g[st][ra], gb = s.g[st][rb];
                 if (!bar_wait(&s.sc_full, par, &s)) break;
                 // (where P takes K's place, its pieces have been made by all warps)
                 if (DK == 128 && !bar_wait(&s.wk_full, par, &s)) break;
                 after_sync();
                 uint8_t* const pa = gen + L::p_at(st, par) + ra * kSwRow + t2 * 2;
+                // 16 x 16 tiles: below the diagonal, on it, above it (loops not
+                // unrolled: the roles' code has to stay in the instruction cache)
+                const uint32_t sc = tm + (static_cast<uint32_t>(warp * 32) << 16) + L::kSc;
+                uint32_t ahead[8];
+                tmem_ld_frag(sc, ahead);
+                ld_wait(ahead);
 #pragma unroll 1
-                for (int half = 0; half < 2; ++half) {            // (unrolled code would not stay in the instruction cache)
-                    uint32_t r[16];
-                    tmem_ld_frag(tm + (static_cast<uint32_t>(warp * 32) << 16) + L::kSc + half * 32, r);
-                    ld_wait(r);
-                    if (half == 1) {
+                for (int tile = 0; tile < 4; ++tile) {
+                    uint8_t* const to0 = pa + ((tile * 2 ^ ra % 8) << 4);        // (rb is the same row of its atom)
+                    uint8_t* const to1 = pa + ((tile * 2 + 1 ^ ra % 8) << 4);
+                    if (tile > warp) {
+#pragma unroll
+                        for (int m = 0; m < 2; ++m)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                *reinterpret_cast<uint32_t*>(to0 + m * kBlk + e * 8 * kSwRow) = 0;
+                                *reinterpret_cast<uint32_t*>(to1 + m * kBlk + e * 8 * kSwRow) = 0;
+                            }
+                        continue;
+                    }
+                    uint32_t r[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) r[i] = ahead[i];
+                    if (tile < warp) {
+                        tmem_ld_frag(sc + (tile + 1) * 16, ahead);
+                    } else {
                         before_sync();
                         warp_arrive(&s.sc_free);
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int col = half * 32 + j * 8 + t2;
+                    for (int j = 0; j < 2; ++j) {
+                        const int col = tile * 16 + j * 8 + t2;
                         const float4 g = *reinterpret_cast<const float4*>(&s.g[st][col]);
                         auto decayed = [&](float2 row, int e) {   // row's two scores from register e on
                             const float2 hi2 = __fadd2_rn(make_float2(row.x, row.x), make_float2(-g.x, -g.z));
@@ -377,16 +398,19 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                                               make_float2(a.scale, a.scale));
                         };
                         float2 x = decayed(ga, j * 4), y = decayed(gb, j * 4 + 2);
-                        if (col > ra) x.x = 0.0f;
-                        if (col + 1 > ra) x.y = 0.0f;
-                        if (col > rb) y.x = 0.0f;
-                        if (col + 1 > rb) y.y = 0.0f;
-                        uint8_t* const to = pa + (((half * 4 + j) ^ ra % 8) << 4);   // (rb is the same row of its atom)
+                        if (tile == warp) {
+                            if (col > ra) x.x = 0.0f;
+                            if (col + 1 > ra) x.y = 0.0f;
+                            if (col > rb) y.x = 0.0f;
+                            if (col + 1 > rb) y.y = 0.0f;
+                        }
+                        uint8_t* const to = j ? to1 : to0;
                         *reinterpret_cast<uint32_t*>(to) = take2(x);
                         *reinterpret_cast<uint32_t*>(to + kBlk) = pack2(x.x, x.y);
                         *reinterpret_cast<uint32_t*>(to + 8 * kSwRow) = take2(y);
                         *reinterpret_cast<uint32_t*>(to + 8 * kSwRow + kBlk) = pack2(y.x, y.y);
                     }
+                    ld_wait(ahead);
                 }
                 to_async();
                 warp_arrive(&s.p_full);
@@ -437,7 +461,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             const int st = at.st;
             const uint32_t par = at.par;
             if (!bar_wait(&s.full[st], at.ph, &s)) break;
-            put_keys<DK>(gen, s, st, tid);         // (the update before has been waited for)
+            put_keys<DK>(gen, s, st, tid - 128, kOwnKeys, 256);   // (the update before has been waited for)
             if (OUT) {
                 if (c && !bar_wait(&s.qs_full, par ^ 1, &s)) break;
                 after_sync();
@@ -491,7 +515,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             if (c < chunks) {
                 if (!bar_wait(&s.full[keys.st], keys.ph, &s)) break;
                 if (c && !bar_wait(&s.u_full, keys.par ^ 1, &s)) break;  // the matrix unit has read the last wK
-                put_keys<DK>(gen, s, keys.st, tid);
+                put_keys<DK>(gen, s, keys.st, OUT ? kOwnKeys + tid - 384 : kOwnKeys + tid - 256, kKeys, OUT ? 128 : 256);
                 if (!OUT) warp_arrive(&s.empty[keys.st]);
                 keys.next();
             }
@@ -502,12 +526,11 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 const bool odd = s.odd[st] != 0;
                 if (!bar_wait(&s.o_full, par, &s)) break;
                 after_sync();
-                if (done) {                        // the last chunk's store has read its tile
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    warp_arrive(&s.empty[st ? st - 1 : kStages - 1]);
-                }
                 at.next();
-                uint8_t* const tile = gen + L::out_at(st) + ow * (kChunk * 64);
+                // the last chunk's store has read the tile
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
+                uint8_t* const tile = gen + L::kOut + ow * (kChunk * 64);
                 const uint32_t tile_at = smem_addr(tile);
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {            // 16 value columns
@@ -572,8 +595,8 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     warp_arrive(&s.o_free);
                 }
                 const long long row = row0 + static_cast<long long>(done) * kChunk;
-                to_async();                        // before the store reads the tile, and the next copy writes it
-                __syncwarp();
+                to_async();                        // before the store reads the tile
+                warp_arrive(&s.empty[st]);
                 if (cols > 0 && tma_out && n == kChunk) {
                     if (lane == 0) {
                         asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
