@@ -32,8 +32,8 @@ enum { SSLA_LINATTN_MAX_DK = 128, SSLA_LINATTN_MAX_DV = 256 };
  * Rows are tokens.  q, k: [n_rows][q_heads or k_heads][dk]; v, out:
  * [n_rows][heads][dv]; the last index is contiguous, row and head strides are
  * in elements.  Head h reads query head h / (heads / q_heads), keys alike.
- * decay: logarithms, strides decay_row and decay_head (decay_row 0: one decay
- * per head); -infinity clears the state before the token.
+ * decay: logarithms, at most 0, strides decay_row and decay_head (decay_row 0:
+ * one decay per head); -infinity clears the state before the token.
  * state: [n_slots][heads][dk][dv], contiguous, updated in place.  `out` does
  * not overlap any input. */
 typedef struct SslaLinAttn {

@@ -21,10 +21,11 @@
 //     (wK pieces to shared memory, as soon as the update before has read the
 //     last ones: the state and output warps, and the P warps where they have
 //     no P to make)
-//     warps 16, 19 tiles into shared memory (three stages): whole chunks by TMA,
-//                  a sequence's last, partial one by 16-byte copies with zeros
-//     warp 17      decay sums
-//     warp 18      issues the matrix instructions
+//     warps 16, 17 tiles into shared memory (three stages): whole chunks by TMA,
+//                  a sequence's last, partial one by 16-byte copies with zeros;
+//                  decay sums
+//     warps 18, 19 issue the matrix instructions: update and carried; scores and
+//                  inner
 // They meet at mbarriers only.  Every wait is bounded: one that runs out sets
 // the abort flag and a bit of the device's status word, all roles leave, and
 // the tensor memory is freed.
@@ -69,6 +70,7 @@ struct Turn {
 struct Side {                                     // what the roles share besides the tiles
     alignas(16) float2 g[kStages][kChunk];        // decay sums as (hi, lo)
     alignas(16) float eg[kStages][kChunk], wk[kStages][kChunk], gam[kStages];   // eg: times scale
+    alignas(16) float end16[kStages][kChunk];     // decay from a token to the end of its 16
     int odd[kStages];                             // an update was not finite
     uint64_t full[kStages], empty[kStages], checked[kStages];
     uint64_t sc_full, sc_free, p_full, o_full, o_free, wk_full, u_full, u_free, s_full, qs_full;
@@ -310,8 +312,8 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
 
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
-            bar_init(&s.full[i], 3);              // two copying warps, the decay warp
-            bar_init(&s.empty[i], 17);            // the matrix unit, the state, P and output warps
+            bar_init(&s.full[i], 3);              // two copying warps, the decay sums
+            bar_init(&s.empty[i], OUT ? 18 : 17); // the matrix unit, the state, P and output warps
             bar_init(&s.checked[i], 8);
         }
         bar_init(&s.sc_full, 1); bar_init(&s.sc_free, 4); bar_init(&s.p_full, 4);
@@ -380,35 +382,43 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     uint32_t r[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) r[i] = ahead[i];
+                    float2 x[2], y[2];                            // rows ra, rb of the tile's two column groups
                     if (tile < warp) {
                         tmem_ld_frag(sc + (tile + 1) * 16, ahead);
+                        // below the diagonal: the decay to the end of the columns' 16 tokens, times that from there
+                        const float2 ge = s.g[st][tile * 16 + 15];
+                        const float ea = exp2_fast((ga.x - ge.x) + (ga.y - ge.y)) * a.scale;
+                        const float eb = exp2_fast((gb.x - ge.x) + (gb.y - ge.y)) * a.scale;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float2 e = *reinterpret_cast<const float2*>(&s.end16[st][tile * 16 + j * 8 + t2]);
+                            x[j] = __fmul2_rn(make_float2(__uint_as_float(r[j * 4]), __uint_as_float(r[j * 4 + 1])),
+                                              __fmul2_rn(e, make_float2(ea, ea)));
+                            y[j] = __fmul2_rn(make_float2(__uint_as_float(r[j * 4 + 2]), __uint_as_float(r[j * 4 + 3])),
+                                              __fmul2_rn(e, make_float2(eb, eb)));
+                        }
                     } else {
                         before_sync();
                         warp_arrive(&s.sc_free);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int col = tile * 16 + j * 8 + t2;
+                            const float4 g = *reinterpret_cast<const float4*>(&s.g[st][col]);
+                            const float e0 = exp2_fast((ga.x - g.x) + (ga.y - g.y)), e1 = exp2_fast((ga.x - g.z) + (ga.y - g.w));
+                            const float f0 = exp2_fast((gb.x - g.x) + (gb.y - g.y)), f1 = exp2_fast((gb.x - g.z) + (gb.y - g.w));
+                            x[j].x = col <= ra ? __uint_as_float(r[j * 4]) * (e0 * a.scale) : 0.0f;
+                            x[j].y = col + 1 <= ra ? __uint_as_float(r[j * 4 + 1]) * (e1 * a.scale) : 0.0f;
+                            y[j].x = col <= rb ? __uint_as_float(r[j * 4 + 2]) * (f0 * a.scale) : 0.0f;
+                            y[j].y = col + 1 <= rb ? __uint_as_float(r[j * 4 + 3]) * (f1 * a.scale) : 0.0f;
+                        }
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const int col = tile * 16 + j * 8 + t2;
-                        const float4 g = *reinterpret_cast<const float4*>(&s.g[st][col]);
-                        auto decayed = [&](float2 row, int e) {   // row's two scores from register e on
-                            const float2 hi2 = __fadd2_rn(make_float2(row.x, row.x), make_float2(-g.x, -g.z));
-                            const float2 x = __fadd2_rn(hi2, __fadd2_rn(make_float2(row.y, row.y), make_float2(-g.y, -g.w)));
-                            return __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])),
-                                                         make_float2(exp2_fast(x.x), exp2_fast(x.y))),
-                                              make_float2(a.scale, a.scale));
-                        };
-                        float2 x = decayed(ga, j * 4), y = decayed(gb, j * 4 + 2);
-                        if (tile == warp) {
-                            if (col > ra) x.x = 0.0f;
-                            if (col + 1 > ra) x.y = 0.0f;
-                            if (col > rb) y.x = 0.0f;
-                            if (col + 1 > rb) y.y = 0.0f;
-                        }
                         uint8_t* const to = j ? to1 : to0;
-                        *reinterpret_cast<uint32_t*>(to) = take2(x);
-                        *reinterpret_cast<uint32_t*>(to + kBlk) = pack2(x.x, x.y);
-                        *reinterpret_cast<uint32_t*>(to + 8 * kSwRow) = take2(y);
-                        *reinterpret_cast<uint32_t*>(to + 8 * kSwRow + kBlk) = pack2(y.x, y.y);
+                        *reinterpret_cast<uint32_t*>(to) = take2(x[j]);
+                        *reinterpret_cast<uint32_t*>(to + kBlk) = pack2(x[j].x, x[j].y);
+                        *reinterpret_cast<uint32_t*>(to + 8 * kSwRow) = take2(y[j]);
+                        *reinterpret_cast<uint32_t*>(to + 8 * kSwRow + kBlk) = pack2(y[j].x, y[j].y);
                     }
                     ld_wait(ahead);
                 }
@@ -524,6 +534,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 const uint32_t par = at.par;
                 if (!bar_wait(&s.checked[st], at.ph, &s)) break;
                 const bool odd = s.odd[st] != 0;
+                if (!bar_wait(&s.qs_full, par, &s)) break;
                 if (!bar_wait(&s.o_full, par, &s)) break;
                 after_sync();
                 at.next();
@@ -620,92 +631,77 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             }
         }
         if (OUT && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    } else if (warp == 16 || warp == 19) {
-        // ---- tiles ----
+    } else if (warp < 18) {
+        // ---- tiles; decay sums (warp 16), the next chunk's values in flight ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        const int t = lane + (warp == 19 ? 32 : 0), hq = h / a.q_share, hk = h / a.k_share;
+        const int t = lane + (warp - 16) * 32, hq = h / a.q_share, hk = h / a.k_share;
         const T* Q = static_cast<const T*>(a.q) + hq * a.q_head + row0 * a.q_row;
         const T* K = static_cast<const T*>(a.k) + hk * a.k_head + row0 * a.k_row;
         const T* V = static_cast<const T*>(a.v) + h * a.v_head + c0 + row0 * a.v_row;
+        double total = 0.0;
+        float2 g = make_float2(0.0f, 0.0f);
+        if (warp == 16) g = chunk_decay_values(a, row0, min(kChunk, count), h, lane);
         Turn at;
         for (int c = 0; c < chunks; ++c, at.next()) {
-            const int n = min(kChunk, count - c * kChunk);
-            if (c >= kStages && !bar_wait(&s.empty[at.st], at.ph ^ 1, &s)) break;
-            uint64_t* const bar = &s.full[at.st];
-            const uint32_t to = base + at.st * L::kStage;
-            if (warp == 16 && lane == 0) s.odd[at.st] = 0;
-            if (use_tma && n == kChunk) {
-                if (warp == 16 && lane == 0) {
-                    const int row = static_cast<int>(row0) + c * kChunk;
-                    const uint32_t bytes = ((OUT ? 2 : 1) * (DK / 64) + (width > 64 ? 2 : 1)) * kBlk;
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
-#pragma unroll
-                    for (int b = 0; b < DK / 64; ++b) tma_box(to + L::kTile + b * kBlk, &maps.k, b * 64, hk, row, bar);
-                    tma_box(to + 2 * L::kTile, &maps.v, c0, h, row, bar);
-                    if (width > 64) tma_box(to + 2 * L::kTile + kBlk, &maps.v, c0 + 64, h, row, bar);
-                    if (OUT)
-#pragma unroll
-                        for (int b = 0; b < DK / 64; ++b) tma_box(to + b * kBlk, &maps.q, b * 64, hq, row, bar);
-                }
-                if (warp == 19) warp_arrive(bar);
-            } else {
+            const int n = min(kChunk, count - c * kChunk), st = at.st;
+            if (c >= kStages && !bar_wait(&s.empty[st], at.ph ^ 1, &s)) break;
+            uint64_t* const bar = &s.full[st];
+            const uint32_t to = base + st * L::kStage;
+            const bool tma = use_tma && n == kChunk;
+            if (!tma) {
                 const long long row = static_cast<long long>(c) * kChunk;
                 copy_tile<DK>(to + L::kTile, K + row * a.k_row, a.k_row, n, a.dk, t);
                 copy_tile<128>(to + 2 * L::kTile, V + row * a.v_row, a.v_row, n, width, t);
                 if (OUT) copy_tile<DK>(to, Q + row * a.q_row, a.q_row, n, a.dk, t);
-                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-                to_async();
-                warp_arrive(bar);
-            }
-        }
-    } else if (warp == 17) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        // ---- decay sums, the next chunk's values in flight ----
-        double total = 0.0;
-        Turn at;
-        float2 g = chunk_decay_values(a, row0, min(kChunk, count), h, lane);
-        for (int c = 0; c < chunks; ++c, at.next()) {
-            float2 ahead = make_float2(0.0f, 0.0f);
-            if (c + 1 < chunks)
-                ahead = chunk_decay_values(a, row0 + (c + 1LL) * kChunk, min(kChunk, count - (c + 1) * kChunk), h, lane);
-            if (c >= kStages && !bar_wait(&s.empty[at.st], at.ph ^ 1, &s)) break;
-            const int st = at.st;
-            const DecaySums d = chunk_decays(g, lane);
-            total += d.total;
-            *reinterpret_cast<float4*>(&s.g[st][2 * lane]) = make_float4(d.hi[0], d.lo[0], d.hi[1], d.lo[1]);
-            *reinterpret_cast<float2*>(&s.eg[st][2 * lane]) = make_float2(d.grown[0] * a.scale, d.grown[1] * a.scale);
-            *reinterpret_cast<float2*>(&s.wk[st][2 * lane]) = make_float2(d.left[0], d.left[1]);
-            if (lane == 0) s.gam[st] = d.whole;
-            warp_arrive(&s.full[st]);
-            g = ahead;
-        }
-        if (!OUT && lane == 0 && blockIdx.x == 0) seg_decay[static_cast<size_t>(blockIdx.z) * a.heads + h] = total;
-    } else {
-        // ---- matrix instructions: the warp as one, one lane issues ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        constexpr uint32_t id_sc = umma_idesc(64, 64, 0, 0), id_u = umma_idesc(128, DK, 1, 1), id_q = umma_idesc(128, 64, 0, 0),
-                           id_p = umma_idesc(128, 64, 1, 0);
-        const uint32_t wk_desc = mn_major(base + L::kWk);
-        auto scores = [&](int st) {
-            const uint32_t q = k_major(base + st * L::kStage), k = k_major(base + st * L::kStage + L::kTile);
-            if (elect()) {
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            } else if (warp == 16 && elect()) {
+                const int row = static_cast<int>(row0) + c * kChunk;
+                const uint32_t bytes = ((OUT ? 2 : 1) * (DK / 64) + (width > 64 ? 2 : 1)) * kBlk;
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
 #pragma unroll
-                for (int i = 0; i < DK / 16; ++i) umma_ss<id_sc>(tm + L::kSc, q + k_step(i), k + k_step(i), i > 0);
-                commit(&s.sc_full);
+                for (int b = 0; b < DK / 64; ++b) tma_box(to + L::kTile + b * kBlk, &maps.k, b * 64, hk, row, bar);
+                tma_box(to + 2 * L::kTile, &maps.v, c0, h, row, bar);
+                if (width > 64) tma_box(to + 2 * L::kTile + kBlk, &maps.v, c0 + 64, h, row, bar);
+                if (OUT)
+#pragma unroll
+                    for (int b = 0; b < DK / 64; ++b) tma_box(to + b * kBlk, &maps.q, b * 64, hq, row, bar);
             }
             __syncwarp();
-        };
-        bool ok = bar_wait(&s.full[0], 0, &s);
-        after_sync();
-        if (OUT && ok) scores(0);
+            if (warp == 16) {
+                float2 ahead = make_float2(0.0f, 0.0f);
+                if (c + 1 < chunks)
+                    ahead = chunk_decay_values(a, row0 + (c + 1LL) * kChunk, min(kChunk, count - (c + 1) * kChunk), h, lane);
+                const DecaySums d = chunk_decays(g, lane);
+                total += d.total;
+                *reinterpret_cast<float4*>(&s.g[st][2 * lane]) = make_float4(d.hi[0], d.lo[0], d.hi[1], d.lo[1]);
+                *reinterpret_cast<float2*>(&s.eg[st][2 * lane]) = make_float2(d.grown[0] * a.scale, d.grown[1] * a.scale);
+                *reinterpret_cast<float2*>(&s.wk[st][2 * lane]) = make_float2(d.left[0], d.left[1]);
+                const float hi16 = __shfl_sync(0xFFFFFFFFu, d.hi[1], lane | 7), lo16 = __shfl_sync(0xFFFFFFFFu, d.lo[1], lane | 7);
+                *reinterpret_cast<float2*>(&s.end16[st][2 * lane]) =
+                    make_float2(exp2_fast((hi16 - d.hi[0]) + (lo16 - d.lo[0])), exp2_fast((hi16 - d.hi[1]) + (lo16 - d.lo[1])));
+                if (lane == 0) s.gam[st] = d.whole, s.odd[st] = 0;
+                warp_arrive(bar);
+                g = ahead;
+            }
+            if (!tma) {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                to_async();
+            }
+            if (!tma || warp == 17) warp_arrive(bar);
+        }
+        if (!OUT && warp == 16 && lane == 0 && blockIdx.x == 0) seg_decay[static_cast<size_t>(blockIdx.z) * a.heads + h] = total;
+    } else if (warp == 18) {
+        // ---- matrix instructions of the state: update, carried (the warp as one, one lane issues) ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        constexpr uint32_t id_u = umma_idesc(128, DK, 1, 1), id_q = umma_idesc(128, 64, 0, 0);
+        const uint32_t wk_desc = mn_major(base + L::kWk);
         Turn at;
-        for (int c = 0; ok && c < chunks; ++c) {
-            const uint32_t par = at.par, prev = par ^ 1, tiles = base + at.st * L::kStage;
+        for (int c = 0; c < chunks; ++c, at.next()) {
+            const uint32_t par = at.par, tiles = base + at.st * L::kStage;
             const uint32_t q = k_major(tiles), v = mn_major(tiles + 2 * L::kTile);
-            const uint32_t p_desc = k_major(base + L::p_at(at.st, par));
-            const int st = at.st;
-            if (!(ok = bar_wait(&s.wk_full, par, &s))) break;
-            if (c && !(ok = bar_wait(&s.u_free, prev, &s))) break;
+            if (!bar_wait(&s.full[at.st], at.ph, &s)) break;
+            if (c && !bar_wait(&s.u_free, par ^ 1, &s)) break;
+            if (!bar_wait(&s.wk_full, par, &s)) break;
             after_sync();
             if (elect()) {
 #pragma unroll
@@ -714,11 +710,12 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     for (int m = 0; m < 3; ++m)
                         umma_ss<id_u>(tm + L::kU, v + mn_step(i), wk_desc + (m * L::kTile >> 4) + mn_step(i), i + m > 0);
                 commit(&s.u_full);
+                if (!OUT) commit(&s.empty[at.st]);
             }
             __syncwarp();
             if constexpr (OUT) {
-                if (!(ok = bar_wait(&s.s_full, par, &s))) break;
-                if (c && !(ok = bar_wait(&s.o_free, prev, &s))) break;
+                if (c && !bar_wait(&s.o_free, par ^ 1, &s)) break;
+                if (!bar_wait(&s.s_full, par, &s)) break;
                 after_sync();
                 if (elect()) {
 #pragma unroll
@@ -727,8 +724,44 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                         for (int i = 0; i < DK / 16; ++i)
                             umma_ts<id_q>(tm + L::kO1, tm + L::kS + m * (DK / 2) + i * 8, q + k_step(i), m + i > 0);
                     commit(&s.qs_full);
+                    commit(&s.empty[at.st]);
                 }
                 __syncwarp();
+            }
+        }
+        // nothing of this warp's may be in flight when the CTA frees its tensor memory
+        drain(&s.u_full, (chunks - 1) & 1);
+        if (OUT) drain(&s.qs_full, (chunks - 1) & 1);
+    } else {
+        // ---- matrix instructions of the chunk itself: scores, inner ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if constexpr (OUT) {
+            constexpr uint32_t id_sc = umma_idesc(64, 64, 0, 0), id_p = umma_idesc(128, 64, 1, 0);
+            auto scores = [&](int st) {
+                const uint32_t q = k_major(base + st * L::kStage), k = k_major(base + st * L::kStage + L::kTile);
+                if (elect()) {
+#pragma unroll
+                    for (int i = 0; i < DK / 16; ++i) umma_ss<id_sc>(tm + L::kSc, q + k_step(i), k + k_step(i), i > 0);
+                    commit(&s.sc_full);
+                }
+                __syncwarp();
+            };
+            bool ok = bar_wait(&s.full[0], 0, &s);
+            after_sync();
+            if (ok) scores(0);
+            Turn at;
+            for (int c = 0; ok && c < chunks; ++c) {
+                const int st = at.st;
+                const uint32_t par = at.par, v = mn_major(base + st * L::kStage + 2 * L::kTile);
+                const uint32_t p_desc = k_major(base + L::p_at(st, par));
+                at.next();
+                if (c + 1 < chunks) {              // the next scores first, so that P follows P
+                    if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
+                    if (!(ok = bar_wait(&s.sc_free, par, &s))) break;
+                    after_sync();
+                    scores(at.st);
+                }
+                if (c && !(ok = bar_wait(&s.o_free, par ^ 1, &s))) break;
                 if (!(ok = bar_wait(&s.p_full, par, &s))) break;
                 after_sync();
                 if (elect()) {
@@ -738,22 +771,12 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                         for (int i = 0; i < kChunk / 16; ++i)
                             umma_ss<id_p>(tm + L::kO2, v + mn_step(i), p_desc + (m * kBlk >> 4) + k_step(i), m + i > 0);
                     commit(&s.o_full);
+                    commit(&s.empty[st]);
                 }
                 __syncwarp();
             }
-            if (elect()) commit(&s.empty[st]);
-            __syncwarp();
-            at.next();
-            if (OUT && c + 1 < chunks) {
-                if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
-                if (!(ok = bar_wait(&s.sc_free, par, &s))) break;
-                after_sync();
-                scores(at.st);
-            }
+            drain(&s.o_full, (chunks - 1) & 1);
         }
-        // nothing of this CTA's may be in flight when it frees its tensor memory
-        drain(&s.u_full, (chunks - 1) & 1);
-        if (OUT) drain(&s.o_full, (chunks - 1) & 1);
     }
     __syncwarp();
     before_sync();
