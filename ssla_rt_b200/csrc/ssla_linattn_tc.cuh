@@ -19,12 +19,11 @@
 //                  tensor memory
 //     warps 12-15  carried, inner -> out, through shared memory
 //     (wK pieces to shared memory, as soon as the update before has read the
-//     last ones: the state and output warps, and the P warps where they have
-//     no P to make)
-//     warps 16, 17 tiles into shared memory (three stages): whole chunks by TMA,
+//     last ones: the state warps, and all three kinds where there are no outputs)
+//     warps 18, 19 tiles into shared memory (three stages): whole chunks by TMA,
 //                  a sequence's last, partial one by 16-byte copies with zeros;
 //                  decay sums
-//     warps 18, 19 issue the matrix instructions: update and carried; scores and
+//     warps 16, 17 issue the matrix instructions: update and carried; scores and
 //                  inner
 // They meet at mbarriers only.  Every wait is bounded: one that runs out sets
 // the abort flag and a bit of the device's status word, all roles leave, and
@@ -46,12 +45,10 @@ template <int DK> struct Plan {
     static constexpr int kTile = DK / 64 * kBlk;  // Q or K of one stage
     static constexpr int kVTile = 2 * kBlk;
     static constexpr int kStage = 2 * kTile + kVTile;
-    static constexpr int kWk = kStages * kStage, kOwn = kWk + 3 * kTile, kOut = kOwn + (DK < 128 ? 4 * kBlk : 0), kEnd = kOut + 2 * kBlk;
+    static constexpr int kWk = kStages * kStage, kOwn = kWk + 3 * kTile, kOut = kOwn + (DK < 128 ? kStages * 2 * kBlk : 0), kEnd = kOut + 2 * kBlk;
     // A chunk's P takes the place of its K, which the products before have
-    // read, where that is large enough; else it has two buffers in turn.
-    __host__ __device__ static constexpr int p_at(int st, int par) {
-        return DK < 128 ? kOwn + par * 2 * kBlk : st * kStage + kTile;
-    }
+    // read, where that is large enough.
+    __host__ __device__ static constexpr int p_at(int st) { return DK < 128 ? kOwn + st * 2 * kBlk : st * kStage + kTile; }
     static constexpr int bytes = kEnd + 1024;     // + alignment slack
     // tensor memory columns
     static constexpr int kU = 0, kSc = DK, kO1 = DK + 64, kO2 = DK + 128, kS = DK + 192;
@@ -72,8 +69,11 @@ struct Side {                                     // what the roles share beside
     alignas(16) float eg[kStages][kChunk], wk[kStages][kChunk], gam[kStages];   // eg: times scale
     alignas(16) float end16[kStages][kChunk];     // decay from a token to the end of its 16
     int odd[kStages];                             // an update was not finite
-    uint64_t full[kStages], empty[kStages], checked[kStages];
-    uint64_t sc_full, sc_free, p_full, o_full, o_free, wk_full, u_full, u_free, s_full, qs_full;
+    // A barrier of its own for each stage where a waiter does not hold back the
+    // next phase by itself (a stage comes again only after everyone has left
+    // it); the others' next phase needs every waiter's own arrival first.
+    uint64_t full[kStages], empty[kStages], checked[kStages], p_full[kStages], wk_full[kStages];
+    uint64_t sc_full, sc_free, o_full, o_free, wk_free[2], u_full, u_free, s_full, qs_full;
     uint32_t tmem;
     int abort;
 };
@@ -248,29 +248,39 @@ struct Maps {
     CUtensorMap q, k, v, out;
 };
 
-// A stage's K decayed to its chunk's end, as three bf16 pieces: 16-byte pieces
-// e, e + step, ... below `end`.
-template <int DK> __device__ __forceinline__ void put_keys(uint8_t* gen, Side& s, int st, int e, int end, int step) {
+// A stage's K decayed to its chunk's end, as three bf16 pieces: the 16 bytes
+// e, e + STEP, ... (N of them) of each.  Piece m of the chunk before (parity
+// `prev`, where there is one) is overwritten once the matrix unit has read it.
+template <int DK, int N, int STEP>
+__device__ __forceinline__ bool put_keys(uint8_t* gen, Side& s, int st, int e, bool again, uint32_t prev) {
     using L = Plan<DK>;
     const uint8_t* K = gen + st * L::kStage + L::kTile;
-#pragma unroll 1
-    for (; e < end; e += step) {
-        const int r = e / (DK / 8), ch = e % (DK / 8);
-        const uint32_t at = piece_at(r, ch);
-        const uint4 u = *reinterpret_cast<const uint4*>(K + at);
+    float2 f[N][4];
+    uint32_t at[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r = (e + i * STEP) / (DK / 8);
+        at[i] = piece_at(r, (e + i * STEP) % (DK / 8));
+        const uint4 u = *reinterpret_cast<const uint4*>(K + at[i]);
         const float2 w = make_float2(s.wk[st][r], s.wk[st][r]);
-        float2 f[4] = {unpack2(u.x), unpack2(u.y), unpack2(u.z), unpack2(u.w)};
+        f[i][0] = __fmul2_rn(unpack2(u.x), w);
+        f[i][1] = __fmul2_rn(unpack2(u.y), w);
+        f[i][2] = __fmul2_rn(unpack2(u.z), w);
+        f[i][3] = __fmul2_rn(unpack2(u.w), w);
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = __fmul2_rn(f[j], w);
+    for (int m = 0; m < 3; ++m) {
+        if (again && !bar_wait(m < 2 ? &s.wk_free[m] : &s.u_full, prev, &s)) return false;
 #pragma unroll
-        for (int m = 0; m < 3; ++m) {
+        for (int i = 0; i < N; ++i) {
             uint4 o;
-            o.x = take2(f[0]); o.y = take2(f[1]); o.z = take2(f[2]); o.w = take2(f[3]);
-            *reinterpret_cast<uint4*>(gen + L::kWk + m * L::kTile + at) = o;
+            o.x = take2(f[i][0]); o.y = take2(f[i][1]); o.z = take2(f[i][2]); o.w = take2(f[i][3]);
+            *reinterpret_cast<uint4*>(gen + L::kWk + m * L::kTile + at[i]) = o;
         }
     }
     to_async();
-    warp_arrive(&s.wk_full);
+    warp_arrive(&s.wk_full[st]);
+    return true;
 }
 
 __device__ __forceinline__ void stmatrix4_trans(uint32_t addr, const uint32_t (&r)[4]) {
@@ -308,17 +318,19 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
     const int slot = tab.slot[seq];
     const size_t head_state = static_cast<size_t>(a.dk) * a.dv;
     // pieces of wK: the state warps' first kOwnKeys, then the others'
-    constexpr int kKeys = kChunk * DK / 8, kOwnKeys = OUT ? (DK == 128 ? 768 : 256) : kKeys / 2;
+    constexpr int kKeys = kChunk * DK / 8, kOwnKeys = OUT ? kKeys : kKeys / 2, kOwn = kOwnKeys / 256, kRest = kKeys / 2 / 256;
 
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) {
             bar_init(&s.full[i], 3);              // two copying warps, the decay sums
             bar_init(&s.empty[i], OUT ? 18 : 17); // the matrix unit, the state, P and output warps
             bar_init(&s.checked[i], 8);
+            bar_init(&s.p_full[i], 4);
+            bar_init(&s.wk_full[i], OUT ? 8 : 16);
         }
-        bar_init(&s.sc_full, 1); bar_init(&s.sc_free, 4); bar_init(&s.p_full, 4);
-        bar_init(&s.o_full, 1); bar_init(&s.o_free, 4); bar_init(&s.wk_full, OUT ? 12 : 16);
-        bar_init(&s.u_full, 1); bar_init(&s.u_free, 8); bar_init(&s.s_full, 8); bar_init(&s.qs_full, 1);
+        bar_init(&s.sc_full, 1); bar_init(&s.sc_free, 4);
+        bar_init(&s.o_full, 1); bar_init(&s.o_free, 4);
+        bar_init(&s.wk_free[0], 1); bar_init(&s.wk_free[1], 1); bar_init(&s.u_full, 1); bar_init(&s.u_free, 8); bar_init(&s.s_full, 8); bar_init(&s.qs_full, 1);
         s.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -350,15 +362,14 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             const uint32_t par = at.par;
             if (!bar_wait(&s.full[st], at.ph, &s)) break;
             if constexpr (!OUT) {
-                if (c && !bar_wait(&s.u_full, par ^ 1, &s)) break;    // the matrix unit has read the last wK
-                put_keys<DK>(gen, s, st, kOwnKeys + tid, kKeys, 256);
+                if (!put_keys<DK, kRest, 256>(gen, s, st, kOwnKeys + tid, c > 0, par ^ 1)) break;
             } else {
                 const float2 ga = s.g[st][ra], gb = s.g[st][rb];
                 if (!bar_wait(&s.sc_full, par, &s)) break;
                 // (where P takes K's place, its pieces have been made by all warps)
-                if (DK == 128 && !bar_wait(&s.wk_full, par, &s)) break;
+                if (DK == 128 && !bar_wait(&s.wk_full[st], at.ph, &s)) break;
                 after_sync();
-                uint8_t* const pa = gen + L::p_at(st, par) + ra * kSwRow + t2 * 2;
+                uint8_t* const pa = gen + L::p_at(st) + ra * kSwRow + t2 * 2;
                 // 16 x 16 tiles: below the diagonal, on it, above it (loops not
                 // unrolled: the roles' code has to stay in the instruction cache)
                 const uint32_t sc = tm + (static_cast<uint32_t>(warp * 32) << 16) + L::kSc;
@@ -423,7 +434,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     ld_wait(ahead);
                 }
                 to_async();
-                warp_arrive(&s.p_full);
+                warp_arrive(&s.p_full[st]);
             }
             warp_arrive(&s.empty[st]);
         }
@@ -466,40 +477,46 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             before_sync();
             warp_arrive(&s.s_full);
         };
-        Turn at;
-        for (int c = 0; c < chunks; ++c, at.next()) {
-            const int st = at.st;
-            const uint32_t par = at.par;
-            if (!bar_wait(&s.full[st], at.ph, &s)) break;
-            put_keys<DK>(gen, s, st, tid - 128, kOwnKeys, 256);   // (the update before has been waited for)
-            if (OUT) {
-                if (c && !bar_wait(&s.qs_full, par ^ 1, &s)) break;
+        Turn keys, at;                             // of chunk c, of chunk c - 1
+        for (int c = 0; c <= chunks; ++c) {
+            const bool more = c < chunks;
+            if (more) {
+                if (!bar_wait(&s.full[keys.st], keys.ph, &s)) break;
+                if (!put_keys<DK, kOwn, 256>(gen, s, keys.st, tid - 128, c > 0, keys.par ^ 1)) break;
+                keys.next();
+            }
+            if (c) {
+                const int st = at.st;
+                const float2 gam = make_float2(s.gam[st], s.gam[st]);
+                if (!bar_wait(&s.u_full, at.par, &s)) break;
+                after_sync();
+                bool odd = false;
+#pragma unroll
+                for (int b = 0; b < HC / 16; ++b) {
+                    uint32_t u[16];
+                    tmem_ld16(tm + lanes + L::kU + k0 + b * 16, u);
+                    ld_wait(u);
+                    // every column of this lane has every v of value column d as a factor
+                    if (b == 0) odd = (u[0] & 0x7F800000u) == 0x7F800000u;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        S[b * 8 + i] = __ffma2_rn(gam, S[b * 8 + i],
+                                                  make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])));
+                }
+                before_sync();
+                warp_arrive(&s.u_free);
+                if (OUT) {
+                    if (odd) s.odd[st] = 1;
+                    warp_arrive(&s.checked[st]);
+                }
+                warp_arrive(&s.empty[st]);
+                if (OUT && more && !bar_wait(&s.qs_full, at.par, &s)) break;
+                at.next();
+            }
+            if (OUT && more) {
                 after_sync();
                 put_pieces();
             }
-            const float2 gam = make_float2(s.gam[st], s.gam[st]);
-            if (!bar_wait(&s.u_full, par, &s)) break;
-            after_sync();
-            bool odd = false;
-#pragma unroll
-            for (int b = 0; b < HC / 16; ++b) {
-                uint32_t u[16];
-                tmem_ld16(tm + lanes + L::kU + k0 + b * 16, u);
-                ld_wait(u);
-                // every column of this lane has every v of value column d as a factor
-                if (b == 0) odd = (u[0] & 0x7F800000u) == 0x7F800000u;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    S[b * 8 + i] = __ffma2_rn(gam, S[b * 8 + i],
-                                              make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])));
-            }
-            before_sync();
-            warp_arrive(&s.u_free);
-            if (OUT) {
-                if (odd) s.odd[st] = 1;
-                warp_arrive(&s.checked[st]);
-            }
-            warp_arrive(&s.empty[st]);
         }
         float* to = nullptr;
         if (!OUT) to = seg_state + (static_cast<size_t>(blockIdx.z) * a.heads + h) * head_state;
@@ -522,17 +539,16 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         const uint32_t lanes = static_cast<uint32_t>(ow * 32) << 16;
         Turn keys, at;                             // of chunk c, of chunk c - 1
         for (int c = 0; c <= chunks; ++c) {
-            if (c < chunks) {
+            if (!OUT && c < chunks) {
                 if (!bar_wait(&s.full[keys.st], keys.ph, &s)) break;
-                if (c && !bar_wait(&s.u_full, keys.par ^ 1, &s)) break;  // the matrix unit has read the last wK
-                put_keys<DK>(gen, s, keys.st, OUT ? kOwnKeys + tid - 384 : kOwnKeys + tid - 256, kKeys, OUT ? 128 : 256);
-                if (!OUT) warp_arrive(&s.empty[keys.st]);
+                if (!put_keys<DK, kRest, 256>(gen, s, keys.st, kOwnKeys + tid - 256, c > 0, keys.par ^ 1)) break;
+                warp_arrive(&s.empty[keys.st]);
                 keys.next();
             }
             if (OUT && c) {
                 const int st = at.st, done = c - 1, n = min(kChunk, count - done * kChunk);
                 const uint32_t par = at.par;
-                if (!bar_wait(&s.checked[st], at.ph, &s)) break;
+                if (!bar_wait(&s.full[st], at.ph, &s) || !bar_wait(&s.checked[st], at.ph, &s)) break;
                 const bool odd = s.odd[st] != 0;
                 if (!bar_wait(&s.qs_full, par, &s)) break;
                 if (!bar_wait(&s.o_full, par, &s)) break;
@@ -577,7 +593,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     // A value in this chunk was not finite: if it is in this lane's column, the product with
                     // masked zeros has reached the tokens before it.  Their inner sums again, one by one.
                     const uint8_t* V = gen + st * L::kStage + 2 * L::kTile;
-                    const uint8_t* P = gen + L::p_at(st, par);
+                    const uint8_t* P = gen + L::p_at(st);
                     auto value = [&](int t) {
                         return __bfloat162float(*reinterpret_cast<const T*>(V + piece_at(t, d / 8) + d % 8 * 2));
                     };
@@ -631,16 +647,16 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             }
         }
         if (OUT && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    } else if (warp < 18) {
-        // ---- tiles; decay sums (warp 16), the next chunk's values in flight ----
+    } else if (warp >= 18) {
+        // ---- tiles; decay sums (warp 18), the next chunk's values in flight ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        const int t = lane + (warp - 16) * 32, hq = h / a.q_share, hk = h / a.k_share;
+        const int t = lane + (warp - 18) * 32, hq = h / a.q_share, hk = h / a.k_share;
         const T* Q = static_cast<const T*>(a.q) + hq * a.q_head + row0 * a.q_row;
         const T* K = static_cast<const T*>(a.k) + hk * a.k_head + row0 * a.k_row;
         const T* V = static_cast<const T*>(a.v) + h * a.v_head + c0 + row0 * a.v_row;
         double total = 0.0;
         float2 g = make_float2(0.0f, 0.0f);
-        if (warp == 16) g = chunk_decay_values(a, row0, min(kChunk, count), h, lane);
+        if (warp == 18) g = chunk_decay_values(a, row0, min(kChunk, count), h, lane);
         Turn at;
         for (int c = 0; c < chunks; ++c, at.next()) {
             const int n = min(kChunk, count - c * kChunk), st = at.st;
@@ -654,7 +670,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 copy_tile<128>(to + 2 * L::kTile, V + row * a.v_row, a.v_row, n, width, t);
                 if (OUT) copy_tile<DK>(to, Q + row * a.q_row, a.q_row, n, a.dk, t);
                 asm volatile("cp.async.commit_group;" ::: "memory");
-            } else if (warp == 16 && elect()) {
+            } else if (warp == 18 && elect()) {
                 const int row = static_cast<int>(row0) + c * kChunk;
                 const uint32_t bytes = ((OUT ? 2 : 1) * (DK / 64) + (width > 64 ? 2 : 1)) * kBlk;
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
@@ -667,7 +683,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     for (int b = 0; b < DK / 64; ++b) tma_box(to + b * kBlk, &maps.q, b * 64, hq, row, bar);
             }
             __syncwarp();
-            if (warp == 16) {
+            if (warp == 18) {
                 float2 ahead = make_float2(0.0f, 0.0f);
                 if (c + 1 < chunks)
                     ahead = chunk_decay_values(a, row0 + (c + 1LL) * kChunk, min(kChunk, count - (c + 1) * kChunk), h, lane);
@@ -687,10 +703,10 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
                 to_async();
             }
-            if (!tma || warp == 17) warp_arrive(bar);
+            if (!tma || warp == 19) warp_arrive(bar);
         }
-        if (!OUT && warp == 16 && lane == 0 && blockIdx.x == 0) seg_decay[static_cast<size_t>(blockIdx.z) * a.heads + h] = total;
-    } else if (warp == 18) {
+        if (!OUT && warp == 18 && lane == 0 && blockIdx.x == 0) seg_decay[static_cast<size_t>(blockIdx.z) * a.heads + h] = total;
+    } else if (warp == 16) {
         // ---- matrix instructions of the state: update, carried (the warp as one, one lane issues) ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         constexpr uint32_t id_u = umma_idesc(128, DK, 1, 1), id_q = umma_idesc(128, 64, 0, 0);
@@ -701,15 +717,16 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             const uint32_t q = k_major(tiles), v = mn_major(tiles + 2 * L::kTile);
             if (!bar_wait(&s.full[at.st], at.ph, &s)) break;
             if (c && !bar_wait(&s.u_free, par ^ 1, &s)) break;
-            if (!bar_wait(&s.wk_full, par, &s)) break;
+            if (!bar_wait(&s.wk_full[at.st], at.ph, &s)) break;
             after_sync();
             if (elect()) {
 #pragma unroll
-                for (int i = 0; i < kChunk / 16; ++i)
+                for (int m = 0; m < 3; ++m) {
 #pragma unroll
-                    for (int m = 0; m < 3; ++m)
+                    for (int i = 0; i < kChunk / 16; ++i)
                         umma_ss<id_u>(tm + L::kU, v + mn_step(i), wk_desc + (m * L::kTile >> 4) + mn_step(i), i + m > 0);
-                commit(&s.u_full);
+                    commit(m < 2 ? &s.wk_free[m] : &s.u_full);
+                }
                 if (!OUT) commit(&s.empty[at.st]);
             }
             __syncwarp();
@@ -753,7 +770,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             for (int c = 0; ok && c < chunks; ++c) {
                 const int st = at.st;
                 const uint32_t par = at.par, v = mn_major(base + st * L::kStage + 2 * L::kTile);
-                const uint32_t p_desc = k_major(base + L::p_at(st, par));
+                const uint32_t p_desc = k_major(base + L::p_at(st)), ph = at.ph;
                 at.next();
                 if (c + 1 < chunks) {              // the next scores first, so that P follows P
                     if (!(ok = bar_wait(&s.full[at.st], at.ph, &s))) break;
@@ -762,7 +779,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                     scores(at.st);
                 }
                 if (c && !(ok = bar_wait(&s.o_free, par ^ 1, &s))) break;
-                if (!(ok = bar_wait(&s.p_full, par, &s))) break;
+                if (!(ok = bar_wait(&s.p_full[st], ph, &s))) break;
                 after_sync();
                 if (elect()) {
 #pragma unroll
