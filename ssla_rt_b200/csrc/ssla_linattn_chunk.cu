@@ -118,35 +118,55 @@ __device__ __forceinline__ void load8(const T* p, int c, int width, bool wide, f
     }
 }
 
-// Stages rows [0, rows) x [0, width) of a token tile as IN pieces.  With
-// `bad`, non-finite values become zero and their first row is noted by column.
-template <typename T, int D, int IN>
-__device__ __forceinline__ bool stage(__nv_bfloat16* s, const T* p, long long stride, int rows, int width, bool wide,
-                                      int* bad) {
-    constexpr int LD = D + 8, G = D / 8;
-    bool any = false;
+// Rows [0, rows) x [0, width) of a token tile, on the way from global memory:
+// thread t's eight values of row (t + i * kThreads) / (D / 8).
+template <int D> struct Moving {
+    static constexpr int N = kChunk * (D / 8) / kThreads;
+    float x[N][8];
+
+    template <typename T> __device__ void load(const T* p, long long stride, int rows, int width, bool wide) {
 #pragma unroll
-    for (int i = threadIdx.x; i < kChunk * G; i += kThreads) {
-        const int r = i / G, c = i % G * 8;
-        float x[8] = {};
-        if (r < rows && c < width) load8<T>(p + r * stride, c, width, wide, x);
-        if (bad) {
+        for (int i = 0; i < N; ++i) {
+            const int e = threadIdx.x + i * kThreads, r = e / (D / 8), c = e % (D / 8) * 8;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (!finite(x[j])) {
-                    atomicMin(bad + c + j, r);
-                    x[j] = 0.0f;
-                    any = true;
-                }
-        }
-#pragma unroll
-        for (int n = 0; n < IN; ++n) {
-            uint4 u;
-            u.x = take(x[0], x[1]); u.y = take(x[2], x[3]); u.z = take(x[4], x[5]); u.w = take(x[6], x[7]);
-            *reinterpret_cast<uint4*>(s + n * kChunk * LD + r * LD + c) = u;
+            for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
+            if (r < rows && c < width) load8<T>(p + r * stride, c, width, wide, x[i]);
         }
     }
-    return any;
+    // To shared memory as IN pieces.  With `bad`, non-finite values become
+    // zero and their first row is noted by column.
+    template <int IN> __device__ bool store(__nv_bfloat16* s, int* bad) {
+        constexpr int LD = D + 8;
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = threadIdx.x + i * kThreads, r = e / (D / 8), c = e % (D / 8) * 8;
+            if (bad) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!finite(x[i][j])) {
+                        atomicMin(bad + c + j, r);
+                        x[i][j] = 0.0f;
+                        any = true;
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < IN; ++n) {
+                uint4 u;
+                u.x = take(x[i][0], x[i][1]); u.y = take(x[i][2], x[i][3]);
+                u.z = take(x[i][4], x[i][5]); u.w = take(x[i][6], x[i][7]);
+                *reinterpret_cast<uint4*>(s + n * kChunk * LD + r * LD + c) = u;
+            }
+        }
+        return any;
+    }
+};
+
+// Asks for the lines of rows [0, rows) x `bytes` in L2.
+template <typename T> __device__ __forceinline__ void fetch_ahead(const T* p, long long stride, int rows, int width) {
+    for (int r = threadIdx.x; r < rows; r += kThreads)
+        for (int c = 0; c < width; c += 128 / static_cast<int>(sizeof(T)))
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(p + r * stride + c));
 }
 
 // One float2 of a state row, bounds-checked.
@@ -270,9 +290,31 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
         const int n = min(kChunk, last - c);
         const long long row = static_cast<long long>(row0) + c;
         // ---- the chunk's tiles, decays and the state's pieces into shared memory ----
-        if (OUT) stage<T, DK, IN>(sQ, Q + row * a.q_row, a.q_row, n, a.dk, wide & 1, nullptr);
-        stage<T, DK, IN>(sK, K + row * a.k_row, a.k_row, n, a.dk, wide & 2, nullptr);
-        bool any = stage<T, DV, IN>(sV, V + row * a.v_row, a.v_row, n, a.dv - c0, wide & 4, bad);
+        bool any;
+        {
+            const T *q = Q + row * a.q_row, *k = K + row * a.k_row, *v = V + row * a.v_row;
+            Moving<DV> mv;
+            Moving<DK> mk;
+            // all loads before the first store, where the registers are there
+            mv.load(v, a.v_row, n, a.dv - c0, wide & 4);
+            mk.load(k, a.k_row, n, a.dk, wide & 2);
+            if constexpr (OUT && DK <= 32) {
+                Moving<DK> mq;
+                mq.load(q, a.q_row, n, a.dk, wide & 1);
+                mq.template store<IN>(sQ, nullptr);
+            }
+            mk.template store<IN>(sK, nullptr);
+            any = mv.template store<IN>(sV, bad);
+            if constexpr (OUT && DK > 32) {
+                Moving<DK> mq;
+                mq.load(q, a.q_row, n, a.dk, wide & 1);
+                mq.template store<IN>(sQ, nullptr);
+            }
+            const int ahead = min(kChunk, last - c - n);
+            if (OUT) fetch_ahead(q + n * a.q_row, a.q_row, ahead, a.dk);
+            fetch_ahead(k + n * a.k_row, a.k_row, ahead, a.dk);
+            fetch_ahead(v + n * a.v_row, a.v_row, ahead, min(a.dv - c0, DV));
+        }
         if (OUT && !zero) {
 #pragma unroll
             for (int i = 0; i < MT; ++i)
