@@ -82,6 +82,26 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// c0, c1 += the product of a (NA pieces) and b (NB pieces, columns of two
+// tiles), pieces of combined order up to ORD, the smallest first.  The matrix
+// unit's adder truncates; FRESH (32-bit results) lets it add only one step's
+// products and rounds the step into c.
+template <int ORD, bool FRESH, int NA, int NB>
+__device__ __forceinline__ void mma_pieces(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
+    float t0[4] = {}, t1[4] = {};
+#pragma unroll
+    for (int o = ORD; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (o - i >= 0 && o - i < NB) {
+                mma(FRESH ? t0 : c0, a[i], b[o - i][0], b[o - i][1]);
+                mma(FRESH ? t1 : c1, a[i], b[o - i][2], b[o - i][3]);
+            }
+    if (FRESH)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c0[e] += t0[e], c1[e] += t1[e];
+}
+
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&p);
@@ -96,6 +116,11 @@ __device__ __forceinline__ uint32_t take(float& x, float& y) {
     x -= f.x;
     y -= f.y;
     return p;
+}
+__device__ __forceinline__ float exp2_fast(float x) {     // 2^-22; results below 2^-126 become zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
@@ -232,9 +257,10 @@ __device__ __forceinline__ DecaySums chunk_decays(float2 g, int lane) {
 
 // Segment states: [segment][head][dk][dv]; segment decays: [segment][head].
 template <typename T, int DK, int DV, bool OUT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, DK <= 32 && DV <= 32 ? 4 : 1)
 k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* seg_decay, int wide) {
     using L = Tile<T, DK, DV>;
+    constexpr bool FRESH = sizeof(T) == 4;
     constexpr int IN = L::IN, MID = L::MID, ORD = Pieces<T>::order, LK = L::LK, LV = L::LV, NT = DV / 8;
     constexpr int MT = DK >= 64 ? DK / 64 : 1;            // 16-row state tiles of a warp
     constexpr int SN = DK >= 64 ? NT : NT / 2;            // and its 8-column tiles
@@ -361,32 +387,22 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
                     ldsm4(qa[i], sQ + i * kChunk * LK + (r0 + lane % 16) * LK + ks + lane / 16 * 8);
 #pragma unroll
                 for (int p = 0; p < 4; ++p)
-                    if (p <= warp)
+                    if (p <= warp) {
+                        uint32_t b[IN][4];
 #pragma unroll
-                        for (int i = 0; i < IN; ++i) {
-                            uint32_t b[4];
-                            ldsm4(b, sK + i * kChunk * LK + (p * 16 + lane % 8 + lane / 16 * 8) * LK + ks + lane / 8 % 2 * 8);
-#pragma unroll
-                            for (int q = 0; q < IN; ++q)
-                                if (q + i <= (IN == 1 ? 0 : ORD)) {
-                                    mma(A[2 * p], qa[q], b[0], b[1]);
-                                    mma(A[2 * p + 1], qa[q], b[2], b[3]);
-                                }
-                        }
+                        for (int i = 0; i < IN; ++i)
+                            ldsm4(b[i], sK + i * kChunk * LK + (p * 16 + lane % 8 + lane / 16 * 8) * LK + ks + lane / 8 % 2 * 8);
+                        mma_pieces<IN == 1 ? 0 : ORD, FRESH>(A[2 * p], A[2 * p + 1], qa, b);
+                    }
                 if (!zero)
 #pragma unroll
-                    for (int p = 0; p < NT / 2; ++p)
+                    for (int p = 0; p < NT / 2; ++p) {
+                        uint32_t b[MID][4];
 #pragma unroll
-                        for (int i = 0; i < MID; ++i) {
-                            uint32_t b[4];
-                            ldsm4t(b, sS + i * DK * LV + (ks + lane % 16) * LV + p * 16 + lane / 16 * 8);
-#pragma unroll
-                            for (int q = 0; q < IN; ++q)
-                                if (q + i <= ORD) {
-                                    mma(O[2 * p], qa[q], b[0], b[1]);
-                                    mma(O[2 * p + 1], qa[q], b[2], b[3]);
-                                }
-                        }
+                        for (int i = 0; i < MID; ++i)
+                            ldsm4t(b[i], sS + i * DK * LV + (ks + lane % 16) * LV + p * 16 + lane / 16 * 8);
+                        mma_pieces<ORD, FRESH>(O[2 * p], O[2 * p + 1], qa, b);
+                    }
             }
             const int ra = r0 + g8, rb = ra + 8;
             const float ea = eg[ra], eb = eg[rb], ha = ghi[ra], la = glo[ra], hb = ghi[rb], lb = glo[rb];
@@ -403,8 +419,8 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
                         for (int e = 0; e < 2; ++e) {
                             const int s = p * 16 + j * 8 + t2 + e;
                             const float hs = ghi[s], ls = glo[s];
-                            P[j][e] = s <= ra ? A[2 * p + j][e] * exp2f((ha - hs) + (la - ls)) : 0.0f;
-                            P[j][2 + e] = s <= rb ? A[2 * p + j][2 + e] * exp2f((hb - hs) + (lb - ls)) : 0.0f;
+                            P[j][e] = s <= ra ? A[2 * p + j][e] * exp2_fast((ha - hs) + (la - ls)) : 0.0f;
+                            P[j][2 + e] = s <= rb ? A[2 * p + j][2 + e] * exp2_fast((hb - hs) + (lb - ls)) : 0.0f;
                         }
                     uint32_t pa[MID][4];
 #pragma unroll
@@ -415,18 +431,13 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
                         pa[i][3] = take(P[1][2], P[1][3]);
                     }
 #pragma unroll
-                    for (int m = 0; m < NT / 2; ++m)
+                    for (int m = 0; m < NT / 2; ++m) {
+                        uint32_t b[IN][4];
 #pragma unroll
-                        for (int i = 0; i < IN; ++i) {
-                            uint32_t b[4];
-                            ldsm4t(b, sV + i * kChunk * LV + (p * 16 + lane % 16) * LV + m * 16 + lane / 16 * 8);
-#pragma unroll
-                            for (int q = 0; q < MID; ++q)
-                                if (q + i <= ORD) {
-                                    mma(O[2 * m], pa[q], b[0], b[1]);
-                                    mma(O[2 * m + 1], pa[q], b[2], b[3]);
-                                }
-                        }
+                        for (int i = 0; i < IN; ++i)
+                            ldsm4t(b[i], sV + i * kChunk * LV + (p * 16 + lane % 16) * LV + m * 16 + lane / 16 * 8);
+                        mma_pieces<ORD, FRESH>(O[2 * m], O[2 * m + 1], pa, b);
+                    }
                 }
             if (any)
 #pragma unroll
@@ -482,18 +493,13 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
 #pragma unroll
                     for (int e = 0; e < 4; ++e) ka[m][e] = take(f[e].x, f[e].y);
 #pragma unroll
-                for (int p = 0; p < SN / 2; ++p)
+                for (int p = 0; p < SN / 2; ++p) {
+                    uint32_t b[IN][4];
 #pragma unroll
-                    for (int m = 0; m < IN; ++m) {
-                        uint32_t b[4];
-                        ldsm4t(b, sV + m * kChunk * LV + (ks + lane % 16) * LV + n0 + p * 16 + lane / 16 * 8);
-#pragma unroll
-                        for (int q = 0; q < 3; ++q)
-                            if (q + m <= 2) {
-                                mma(U[2 * p], ka[q], b[0], b[1]);
-                                mma(U[2 * p + 1], ka[q], b[2], b[3]);
-                            }
-                    }
+                    for (int m = 0; m < IN; ++m)
+                        ldsm4t(b[m], sV + m * kChunk * LV + (ks + lane % 16) * LV + n0 + p * 16 + lane / 16 * 8);
+                    mma_pieces<2, FRESH>(U[2 * p], U[2 * p + 1], ka, b);
+                }
             }
 #pragma unroll
             for (int j = 0; j < SN; ++j)

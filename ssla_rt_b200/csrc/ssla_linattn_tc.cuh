@@ -218,11 +218,6 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  :: "r"(dst), "l"(map), "r"(x), "r"(head), "r"(row), "r"(smem_addr(bar)) : "memory");
 }
-__device__ __forceinline__ float exp2_fast(float x) {     // 2^-22; results below 2^-126 become zero
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
