@@ -389,6 +389,20 @@ int  ssla_engine_write_state(SslaEngine* eng, int kind, int partition, int index
 void* ssla_engine_state_ptr(SslaEngine* eng, int kind, int partition, int index);
 int  ssla_engine_info(SslaEngine* eng, SslaEngineInfo* info);
 
+/* Parks a partition's whole state in a device buffer of
+ * ssla_engine_park_bytes (16-byte aligned), a third or less of its size, and
+ * resumes it, into the same partition or another one (of an engine of the
+ * same model and layout).  Hidden states are held in 8 bits, `format` an
+ * SSLA_FMT_* of ssla_ops.h, with one scale per cell (ssla_state_store); gate
+ * counters, timestamps, predictions and versions unchanged, so that the gates
+ * go on exactly.  Asynchronous on `stream`, ordered with drains on the same
+ * stream; not while a live loop runs on the partition.  No reference
+ * counterpart (its runtime state lives and dies with the process). */
+int  ssla_engine_park_bytes(SslaEngine* eng, size_t* bytes);
+int  ssla_engine_park(SslaEngine* eng, int partition, int format, void* buf_dev, size_t bytes, void* stream);
+int  ssla_engine_resume(SslaEngine* eng, int partition, int format, const void* buf_dev, size_t bytes,
+                        void* stream);
+
 /* drain_n contract of the reference's P1 kernels: each block processes its
  * records in order and writes one HybridS2S3OutputSlot per record; weights,
  * hidden state and tdrop counters are read from / written to the device

@@ -127,6 +127,7 @@ EXPORTED = (
     "ssla_engine_strip_drain", "ssla_strip_drain_lockstep", "ssla_engine_strip_status",
     "ssla_engine_rings_attach", "ssla_engine_drain_rings", "ssla_engine_serve_rings",
     "ssla_replay_start", "ssla_replay_stop", "ssla_replay_join",
+    "ssla_engine_park_bytes", "ssla_engine_park", "ssla_engine_resume",
 )
 
 class SslaLinAttn(C.Structure):

@@ -21,6 +21,7 @@
 #include <vector>
 
 #include "ssla_b200.h"
+#include "ssla_ops.h"
 #include "ssla_kernels.cuh"
 #include "ssla_weights.h"
 
@@ -1917,6 +1918,93 @@ int ssla_engine_write_state(SslaEngine* eng, int kind, int partition, int index,
 void* ssla_engine_state_ptr(SslaEngine* eng, int kind, int partition, int index) {
     if (!state_args_ok(eng, kind, partition, index)) return nullptr;
     return eng->e.state_ptr(kind, partition, index);
+}
+
+// A parked partition: the hidden layers as 8-bit codes with one scale per
+// cell, then everything else of the partition unchanged.  Parts start at
+// multiples of 256 bytes, in this order.
+namespace {
+struct ParkPart {
+    int kind, index;
+    size_t at, bytes;               // place and size in the buffer (hidden: of the codes)
+    size_t scales_at;               // hidden only
+};
+size_t park_layout(const ssla::Engine& e, std::vector<ParkPart>& parts) {
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at = (at + n + 255) / 256 * 256;
+        return here;
+    };
+    for (int l = 0; l < 8; ++l) {
+        ParkPart p{SSLA_STATE_HIDDEN, l, 0, e.state_elems(SSLA_STATE_HIDDEN, l), 0};
+        p.at = take(p.bytes);
+        p.scales_at = take(p.bytes / ssla::chans(l / 2) * 4);
+        parts.push_back(p);
+    }
+    for (int kind : {SSLA_STATE_COUNTER, SSLA_STATE_LAST_T, SSLA_STATE_PREDS_DEC, SSLA_STATE_PREDS_RAW, SSLA_STATE_VERSION})
+        for (int i = 0; i < (kind == SSLA_STATE_COUNTER ? 4 : 1); ++i) {
+            ParkPart p{kind, i, 0, e.state_elems(kind, i) * ssla::Engine::elem_size(kind), 0};
+            p.at = take(p.bytes);
+            parts.push_back(p);
+        }
+    return at;
+}
+int park_move(SslaEngine* eng, int partition, int format, char* buf, size_t bytes, cudaStream_t st, bool store) {
+    ssla::Engine& e = eng->e;
+    std::vector<ParkPart> parts;
+    const size_t need = park_layout(e, parts);
+    if (partition < 0 || partition >= e.g.P) throw std::invalid_argument("no such partition");
+    if (format != SSLA_FMT_INT8 && format != SSLA_FMT_E4M3) throw std::invalid_argument("format is not an SSLA_FMT_* value");
+    if (!buf || bytes < need) throw std::invalid_argument("parking buffer smaller than ssla_engine_park_bytes");
+    if (reinterpret_cast<uintptr_t>(buf) % 16) throw std::invalid_argument("parking buffer is not 16-byte aligned");
+    ssla::DeviceGuard dg(e.device);
+    for (const ParkPart& p : parts) {
+        char* state = e.state_ptr(p.kind, partition, p.index);
+        if (p.kind != SSLA_STATE_HIDDEN) {
+            SSLA_CK(cudaMemcpyAsync(store ? buf + p.at : state, store ? state : buf + p.at, p.bytes, cudaMemcpyDeviceToDevice, st));
+            continue;
+        }
+        const int ch = ssla::chans(p.index / 2);
+        SslaStateCache c = {};
+        c.codes = buf + p.at;
+        c.scales = reinterpret_cast<float*>(buf + p.scales_at);
+        c.n = c.n_slots = 1;
+        c.rows = static_cast<int>(p.bytes / ch);
+        c.cols = c.block = ch;
+        c.x_row = ch;
+        c.format = format;
+        c.dtype = SSLA_DT_F32;
+        c.device = e.device;
+        const int rc = store ? ssla_state_store(&c, state, st) : ssla_state_load(&c, state, st);
+        if (rc != SSLA_OK) return rc;
+    }
+    return SSLA_OK;
+}
+}  // namespace
+
+int ssla_engine_park_bytes(SslaEngine* eng, size_t* bytes) {
+    if (!eng || !bytes) { ssla::g_last_error = "null argument"; return SSLA_ERR_ARG; }
+    return ssla::guarded([&] {
+        std::vector<ParkPart> parts;
+        *bytes = park_layout(eng->e, parts);
+        return SSLA_OK;
+    });
+}
+
+int ssla_engine_park(SslaEngine* eng, int partition, int format, void* buf_dev, size_t bytes, void* stream) {
+    if (!eng) { ssla::g_last_error = "null engine"; return SSLA_ERR_ARG; }
+    return ssla::guarded([&] {
+        return park_move(eng, partition, format, static_cast<char*>(buf_dev), bytes, static_cast<cudaStream_t>(stream), true);
+    });
+}
+
+int ssla_engine_resume(SslaEngine* eng, int partition, int format, const void* buf_dev, size_t bytes, void* stream) {
+    if (!eng) { ssla::g_last_error = "null engine"; return SSLA_ERR_ARG; }
+    return ssla::guarded([&] {
+        return park_move(eng, partition, format, static_cast<char*>(const_cast<void*>(buf_dev)), bytes,
+                         static_cast<cudaStream_t>(stream), false);
+    });
 }
 
 int ssla_engine_info(SslaEngine* eng, SslaEngineInfo* info) {

@@ -79,6 +79,9 @@ def load_library() -> C.CDLL:
         "ssla_s2s3_drain_n_multi": (i, [C.POINTER(abi.HybridS2S3Config), vp, vp, vp, vp, vp]),
         "ssla_s2s3_drain_n": (i, [C.POINTER(abi.HybridS2S3Config), vp, vp, i, i, vp, vp, vp, vp, vp]),
         "ssla_s2s3_gate_codes_noalloc": (i, [C.POINTER(abi.HybridS2S3Config), vp, vp, vp, vp]),
+        "ssla_engine_park_bytes": (i, [vp, C.POINTER(C.c_size_t)]),
+        "ssla_engine_park": (i, [vp, i, i, vp, C.c_size_t, vp]),
+        "ssla_engine_resume": (i, [vp, i, i, vp, C.c_size_t, vp]),
         "ssla_linattn_chunk": (i, [C.POINTER(abi.SslaLinAttn), vp, vp, vp, i, vp, C.c_size_t, vp]),
         "ssla_linattn_chunk_workspace": (i, [C.POINTER(abi.SslaLinAttn), vp, vp, i, C.POINTER(C.c_size_t)]),
         "ssla_linattn_status": (i, [i, C.POINTER(C.c_uint)]),
@@ -404,6 +407,31 @@ class SslaEngine:
 
     def flags(self, n: int) -> np.ndarray:
         return self._read(abi.STATE_FLAGS, 0, 0, np.uint8)[:n]
+
+    # ---- parked partitions ----
+    def park_bytes(self) -> int:
+        """Size of a parking buffer: a partition's state with its hidden layers in 8 bits."""
+        nb = C.c_size_t()
+        _check(self.lib.ssla_engine_park_bytes(self.h, C.byref(nb)))
+        return nb.value
+
+    @staticmethod
+    def _buffer_bytes(buf) -> int:
+        if not hasattr(buf, "data_ptr") or not buf.is_cuda or not buf.is_contiguous():
+            raise ValueError("a parking buffer is a contiguous CUDA tensor")
+        return buf.numel() * buf.element_size()
+
+    def park(self, buf, partition: int = 0, fmt: int = abi.FMT_INT8, stream=None) -> None:
+        """Writes a partition's state into ``buf`` (a CUDA tensor of
+        park_bytes): hidden layers as abi.FMT_INT8 or abi.FMT_E4M3 with one
+        scale per cell, everything else unchanged.  Asynchronous on
+        ``stream``, like a drain."""
+        _check(self.lib.ssla_engine_park(self.h, partition, fmt, _ptr(buf), self._buffer_bytes(buf), _stream(stream)))
+
+    def resume(self, buf, partition: int = 0, fmt: int = abi.FMT_INT8, stream=None) -> None:
+        """Puts a parked state back, into the same partition or another one.
+        Asynchronous on ``stream``."""
+        _check(self.lib.ssla_engine_resume(self.h, partition, fmt, _ptr(buf), self._buffer_bytes(buf), _stream(stream)))
 
     def set_profiling(self, on: bool) -> None:
         _check(self.lib.ssla_engine_set_profiling(self.h, 1 if on else 0))

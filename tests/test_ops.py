@@ -236,3 +236,14 @@ def test_errors_name_the_code():
     with pytest.raises(SslaError):
         from ssla_rt_b200.engine import _check
         _check(load_library().ssla_linattn_step(None, None, None))
+
+
+def test_park_refuses_null_arguments():
+    lib = load_library()
+    assert lib.ssla_engine_park_bytes(None, None) == abi.SSLA_ERR_ARG
+    assert lib.ssla_engine_park(None, 0, 0, None, 0, None) == abi.SSLA_ERR_ARG
+    assert lib.ssla_engine_resume(None, 0, 0, None, 0, None) == abi.SSLA_ERR_ARG
+    from ssla_rt_b200.engine import SslaEngine
+    for buf in (None, torch.zeros(8), [0]):
+        with pytest.raises(ValueError, match="CUDA tensor"):
+            SslaEngine._buffer_bytes(buf)
