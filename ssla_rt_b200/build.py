@@ -63,8 +63,35 @@ def build_consumer(force: bool = False, verbose: bool = False) -> str:
     return CONSUMER_CUBIN
 
 
+# The repeated calls of ops.py in one step: a Python extension module over
+# torch's tensors (the library itself stays free of torch).
+OPS_TORCH_SRC = os.path.join(CSRC, "ssla_ops_torch.cpp")
+OPS_TORCH = os.path.join(HERE, "_ops_torch.so")
+
+
+def build_ops_torch(force: bool = False, verbose: bool = False) -> str:
+    deps = [OPS_TORCH_SRC] + [os.path.join(REPO, "include", f) for f in ("ssla_b200.h", "ssla_ops.h")]
+    if not force and os.path.exists(OPS_TORCH) and os.path.getmtime(OPS_TORCH) >= max(map(os.path.getmtime, deps)):
+        return OPS_TORCH
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    dirs = [os.path.join(REPO, "include"), sysconfig.get_paths()["include"], "/usr/local/cuda/include",
+            *cpp_extension.include_paths()]
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{d}" for d in dirs], OPS_TORCH_SRC, "-o", OPS_TORCH, f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    return OPS_TORCH
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     build_consumer(force=force, verbose=verbose)
+    build_ops_torch(force=force, verbose=verbose)
     if not force and not _stale():
         return LIB
     cmd = [_nvcc(), *NVCC_FLAGS, f"-I{os.path.join(REPO, 'include')}", f"-I{CSRC}",

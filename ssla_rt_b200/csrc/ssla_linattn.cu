@@ -16,24 +16,25 @@ namespace ops {
 namespace {
 
 // ---------------------------------------------------------------------------
-// One token per row: a CTA holds a head's state columns [c0, c0 + 32) in
-// registers and applies the rows that name its slot.
+// One token per row: a CTA holds a head's state columns [c0, c0 + COLS) in
+// registers and applies the rows that name its slot.  Memory bound: the state
+// is read and written once, 8 dk dv bytes; everything a token needs is asked
+// for together with the state, before the slots are compared, and the state
+// leaves before the output is summed up.
 //
 // Thread (tx, rg): columns c0 + tx * VEC .. + VEC, state rows rg + i * RG.
 // ---------------------------------------------------------------------------
-constexpr int kStepThreads = 128;
-constexpr int kStepCols = 32;
-template <typename T, int VEC, int RPT>
+template <typename T, int VEC, int RPT, int COLS>
 struct StepTile {
-    static constexpr int TX = kStepCols / VEC, RG = kStepThreads / TX;
-    float s[RPT][VEC];
+    static constexpr int kThreads = 4 * COLS, TX = COLS / VEC, RG = kThreads / TX;
+    float s[RPT][VEC], kk[RPT], qq[RPT], vv[VEC], g;
     int tx, rg, c0;
     bool live;                                     // this thread's columns exist
 
     __device__ void place(const LinArgs& a) {
         tx = threadIdx.x % TX;
         rg = threadIdx.x / TX;
-        c0 = blockIdx.x * kStepCols + tx * VEC;
+        c0 = blockIdx.x * COLS + tx * VEC;
         live = c0 < a.dv;
     }
     __device__ float* at(const LinArgs& a, int slot, int h) const {
@@ -51,30 +52,37 @@ struct StepTile {
         for (int i = 0; i < RPT; ++i)
             if (live && rg + i * RG < a.dk) store_vec<float, VEC>(p + static_cast<size_t>(rg + i * RG) * a.dv, s[i]);
     }
-    // One token: updates the state and writes the output columns.
-    __device__ void token(const LinArgs& a, int row, int h, float* red) {
+    __device__ void fetch(const LinArgs& a, int row, int h) {
         const T* q = static_cast<const T*>(a.q) + row * a.q_row + (h / a.q_share) * a.q_head;
         const T* k = static_cast<const T*>(a.k) + row * a.k_row + (h / a.k_share) * a.k_head;
         const T* v = static_cast<const T*>(a.v) + row * a.v_row + h * a.v_head;
-        const float g = expf(a.decay[row * a.decay_row + h * a.decay_head]);
-        float vv[VEC], o[VEC];
+        g = a.decay[row * a.decay_row + h * a.decay_head];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            vv[j] = live ? to_f<T>(v[c0 + j]) : 0.0f;
-            o[j] = 0.0f;
-        }
+        for (int j = 0; j < VEC; ++j) vv[j] = live ? to_f<T>(v[c0 + j]) : 0.0f;
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
             const int r = rg + i * RG;
-            const bool in = r < a.dk;
-            const float kk = in ? to_f<T>(k[r]) : 0.0f, qq = in ? to_f<T>(q[r]) : 0.0f;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                if (in) s[i][j] = fmaf(kk, vv[j], g * s[i][j]);
-                if (in) o[j] = fmaf(qq, s[i][j], o[j]);
-            }
+            kk[i] = r < a.dk ? to_f<T>(k[r]) : 0.0f;
+            qq[i] = r < a.dk ? to_f<T>(q[r]) : 0.0f;
         }
-        // over the row groups: lanes of a warp with the same tx, then the four warps
+    }
+    // The fetched token: updates the state, and leaves its output's parts in o.
+    __device__ void apply(const LinArgs& a, float (&o)[VEC]) {
+        const float e = expf(g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < RPT; ++i)
+            if (rg + i * RG < a.dk)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    s[i][j] = fmaf(kk[i], vv[j], e * s[i][j]);
+                    o[j] = fmaf(qq[i], s[i][j], o[j]);
+                }
+    }
+    // Sums the parts over the row groups (lanes of a warp with the same tx,
+    // then the warps) and writes the output columns.
+    __device__ void output(const LinArgs& a, int row, int h, float (&o)[VEC], float* red) {
 #pragma unroll
         for (int m = TX; m < 32; m <<= 1)
 #pragma unroll
@@ -82,41 +90,43 @@ struct StepTile {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         if (lane < TX)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) red[warp * kStepCols + tx * VEC + j] = o[j];
+            for (int j = 0; j < VEC; ++j) red[warp * COLS + tx * VEC + j] = o[j];
         __syncthreads();
-        const int c = blockIdx.x * kStepCols + threadIdx.x;
-        if (threadIdx.x < kStepCols && c < a.dv) {
+        const int c = blockIdx.x * COLS + threadIdx.x;
+        if (threadIdx.x < COLS && c < a.dv) {
             float t = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kStepThreads / 32; ++w) t += red[w * kStepCols + threadIdx.x];
+            for (int w = 0; w < kThreads / 32; ++w) t += red[w * COLS + threadIdx.x];
             static_cast<T*>(a.out)[row * a.out_row + h * a.out_head + c] = from_f<T>(t * a.scale);
         }
         __syncthreads();
     }
 };
 
-template <typename T, int VEC, int RPT>
-__global__ void __launch_bounds__(kStepThreads) k_linattn_step(LinArgs a, const int* __restrict__ slots) {
-    __shared__ float red[kStepThreads / 32 * kStepCols];
+template <typename T, int VEC, int RPT, int COLS>
+__global__ void __launch_bounds__(4 * COLS) k_linattn_step(LinArgs a, const int* __restrict__ slots) {
+    using Tile = StepTile<T, VEC, RPT, COLS>;
+    __shared__ float red[Tile::kThreads / 32 * COLS];
     __shared__ int next_s;
-    StepTile<T, VEC, RPT> t;
+    Tile t;
     t.place(a);
     const int h = blockIdx.y;
     int row = blockIdx.z;
     const int slot = slots ? slots[row] : row;
     if (slot < 0 || slot >= a.n_slots) {           // padding row
-        const int c = blockIdx.x * kStepCols + threadIdx.x;
-        if (threadIdx.x < kStepCols && c < a.dv)
+        const int c = blockIdx.x * COLS + threadIdx.x;
+        if (threadIdx.x < COLS && c < a.dv)
             static_cast<T*>(a.out)[row * a.out_row + h * a.out_head + c] = from_f<T>(0.0f);
         return;
     }
     t.load(a, slot, h);
+    t.fetch(a, row, h);
     for (;;) {
         int next = INT_MAX, before = 0;
         if (slots) {
             // rows that name this slot: the first of them applies all, in row order
             if (threadIdx.x == 0) next_s = INT_MAX;
-            for (int r = threadIdx.x; r < a.n_rows; r += kStepThreads)
+            for (int r = threadIdx.x; r < a.n_rows; r += Tile::kThreads)
                 if (r != row && slots[r] == slot) {
                     if (r < row) before = 1;
                     else next = min(next, r);
@@ -127,30 +137,38 @@ __global__ void __launch_bounds__(kStepThreads) k_linattn_step(LinArgs a, const 
             __syncthreads();
             next = next_s;
         }
-        t.token(a, row, h, red);
+        float o[VEC];
+        t.apply(a, o);
+        if (next == INT_MAX) t.store(a, slot, h);
+        t.output(a, row, h, o, red);
         if (next == INT_MAX) break;
         row = next;
+        t.fetch(a, row, h);
     }
-    t.store(a, slot, h);
 }
 
 // ---- host ----------------------------------------------------------------
 
-template <typename F> int with_tile(int dtype, bool vec4, int dk, F&& f) {
-    auto by_rows = [&](auto t, auto v) {
-        using T = decltype(t);
-        constexpr int V = decltype(v)::value, RG = StepTile<T, V, 1>::RG;
-        if (dk <= 2 * RG) return f(t, v, std::integral_constant<int, 2>());
-        if (dk <= 4 * RG) return f(t, v, std::integral_constant<int, 4>());
-        if (dk <= 8 * RG) return f(t, v, std::integral_constant<int, 8>());
+// The state rows of a thread, and 64 columns a CTA where there are as many
+// and vectors of four, else 32: wider runs of a state row at a time (256
+// rows, 16 heads of 128 x 128: 105 us with 32 columns).
+template <typename F> int with_tile(int dtype, bool vec4, int dk, int dv, F&& f) {
+    using std::integral_constant;
+    auto by_rows = [&](auto t, auto v, auto c) {
+        constexpr int V = decltype(v)::value, RG = 4 * V;
+        if (dk <= 2 * RG) return f(t, v, integral_constant<int, 2>(), c);
+        if (dk <= 4 * RG) return f(t, v, integral_constant<int, 4>(), c);
+        if (dk <= 8 * RG) return f(t, v, integral_constant<int, 8>(), c);
         if constexpr (V == 1) {
-            if (dk <= 16 * RG) return f(t, v, std::integral_constant<int, 16>());
-            return f(t, v, std::integral_constant<int, 32>());
+            if (dk <= 16 * RG) return f(t, v, integral_constant<int, 16>(), c);
+            return f(t, v, integral_constant<int, 32>(), c);
         }
         return fail(SSLA_ERR_ARG, "dk %d", dk);
     };
     auto by_vec = [&](auto t) {
-        return vec4 ? by_rows(t, std::integral_constant<int, 4>()) : by_rows(t, std::integral_constant<int, 1>());
+        if (!vec4) return by_rows(t, integral_constant<int, 1>(), integral_constant<int, 32>());
+        if (dv < 64) return by_rows(t, integral_constant<int, 4>(), integral_constant<int, 32>());
+        return by_rows(t, integral_constant<int, 4>(), integral_constant<int, 64>());
     };
     return dtype == SSLA_DT_F32 ? by_vec(float()) : dtype == SSLA_DT_BF16 ? by_vec(__nv_bfloat16()) : by_vec(__half());
 }
@@ -280,10 +298,11 @@ int ssla_linattn_step(const SslaLinAttn* a, const int* slots, void* stream) {
     OnDevice dev(a->device);
     if (dev.err != SSLA_OK) return dev.err;
     const LinArgs d = device_args(a);
-    return with_tile(a->dtype, state_vec4(a), a->dk, [&](auto t, auto v, auto r) {
-        const dim3 grid((a->dv + kStepCols - 1) / kStepCols, a->heads, a->n_rows);
-        k_linattn_step<decltype(t), decltype(v)::value, decltype(r)::value>
-            <<<grid, kStepThreads, 0, static_cast<cudaStream_t>(stream)>>>(d, slots);
+    return with_tile(a->dtype, state_vec4(a), a->dk, a->dv, [&](auto t, auto v, auto r, auto c) {
+        constexpr int COLS = decltype(c)::value;
+        const dim3 grid((a->dv + COLS - 1) / COLS, a->heads, a->n_rows);
+        k_linattn_step<decltype(t), decltype(v)::value, decltype(r)::value, COLS>
+            <<<grid, 4 * COLS, 0, static_cast<cudaStream_t>(stream)>>>(d, slots);
         return launched("k_linattn_step");
     });
 }

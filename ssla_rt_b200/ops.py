@@ -35,6 +35,36 @@ _PLANS: dict = {}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def _fast_module():
+    """The extension module that answers repeated calls (build.py), set up; None where it is not built."""
+    try:
+        from . import _ops_torch as m
+    except ImportError:
+        return None
+    lib = load_library()
+    m.init(_PLANS, *[C.cast(getattr(lib, n), C.c_void_p).value for n in (
+        "ssla_linattn_step", "ssla_state_store", "ssla_state_load", "ssla_group_norm", "ssla_group_norm_workspace")])
+    return m
+
+
+_fast = _fast_module()
+
+
+def _keep_plan(key: Optional[bytes], block) -> None:
+    """Leaves a checked argument block for the extension module."""
+    if key is not None:
+        if len(_PLANS) >= 4096:
+            _PLANS.clear()
+        _PLANS[key] = bytes(block)
+
+
+def _fast_result(r):
+    """What the extension module returned: a negative code is an error of the C entry."""
+    if type(r) is int:
+        _check(-r)
+    return r
+
+
 def _sig(t: Optional[torch.Tensor]):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
@@ -274,11 +304,18 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dec
     Rows that name the same slot are applied in row order; a slot outside the
     state marks a padding row: zero output, no state touched.
     """
+    if _fast is not None and stream is None:
+        r = _fast.step(q, k, v, decay, state, slots, scale, out, False)
+        if r is not None:
+            return _fast_result(r)
+    given = out
     if state is None:
         raise ValueError("state is needed")
     if slots is not None and not isinstance(slots, torch.Tensor):
         raise ValueError("slots is a one-dimensional int32 tensor")
     a = _linattn(q, k, v, decay, state, scale, out, slots)
+    if _fast is not None:
+        _keep_plan(_fast.step(q, k, v, decay, state, slots, scale, given, True), a)
     handle, ts = _stream_of(stream, a.device)
     if out is None:
         out = _like(v, ts)
@@ -356,7 +393,13 @@ def state_store(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, b
     is named twice the last state is kept; other slots stay as they were.  A
     block with a non-finite value reads back as NaN.
     """
+    if _fast is not None and stream is None:
+        r = _fast.store(x, codes, scales, block, slots, False)
+        if r is not None:
+            return _check(-r)
     c = _cache(codes, scales, block, slots, x.shape[0], "x", x, x.dtype)
+    if _fast is not None:
+        _keep_plan(_fast.store(x, codes, scales, block, slots, True), c)
     handle, ts = _stream_of(stream, c.device)
     _check(load_library().ssla_state_store(C.byref(c), x.data_ptr(), handle))
     if ts is not None:
@@ -368,11 +411,18 @@ def state_load(codes: torch.Tensor, scales: torch.Tensor, *, block: int = 64, sl
     """Reads states back from the 8-bit cache: (states, rows, cols), state i
     from slot slots[i] (every slot in order without); a slot outside the cache
     gives zeros."""
+    code = _DTYPES.get(out.dtype if out is not None else dtype, -1)
+    if _fast is not None and stream is None:
+        r = _fast.load(codes, scales, block, slots, code, out, False)
+        if r is not None:
+            return _fast_result(r)
     if out is not None:
         n, dtype = out.shape[0], out.dtype
     else:
         n = slots.shape[0] if slots is not None else codes.shape[0]
     c = _cache(codes, scales, block, slots, n, "out", out, dtype)
+    if _fast is not None:
+        _keep_plan(_fast.load(codes, scales, block, slots, code, out, True), c)
     handle, ts = _stream_of(stream, c.device)
     if out is None:
         out = _new(codes, (n, c.rows, c.cols), dtype, ts)
@@ -422,14 +472,22 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     sample's positions and the channels of a group; weight, bias: (channels,)
     float32.  activation: "silu" or "none".  ``out`` may be x.
     """
+    act = _ACTIVATIONS.get(activation, -1)
+    if _fast is not None and stream is None:
+        r = _fast.norm(x, groups, weight, bias, eps, act, out, False)
+        if r is not None:
+            return _fast_result(r)
     if x.dim() == 2:
         y = group_norm(x[:, None], groups, weight, bias, eps=eps, activation=activation,
                        out=None if out is None else out[:, None], stream=stream)
         return y[:, 0] if out is None else out
     _no_grad(x, weight, bias)
+    given = out
     key = ("norm", _sig(x), groups, _sig(weight), _sig(bias), eps, activation, _sig(out))
     a = abi.SslaGroupNorm.from_buffer_copy(
         _plan(key, lambda: _norm_block(x, groups, weight, bias, eps, activation, out)))
+    if _fast is not None:
+        _keep_plan(_fast.norm(x, groups, weight, bias, eps, act, given, True), a)
     handle, ts = _stream_of(stream, a.device)
     if out is None:
         out = _like(x, ts)

@@ -677,3 +677,49 @@ def test_a_stream_given_as_zero_is_the_legacy_default():
 
 def test_no_wait_ran_out():
     assert ops.linear_attention_status() == 0
+
+
+# ---- the repeated call --------------------------------------------------------------------
+
+
+def test_repeated_calls_answer_like_the_first():
+    """The same shapes again (the extension module's path): new values, new
+    places, given outputs; and the same refusals as the first call."""
+    assert ops._fast is not None, "build with `python ssla_rt_b200/build.py`"
+    for rep in range(3):
+        q, k, v, d, state = inputs(101 + 7 * rep, 5, 2, 2, 2, 24, 40, torch.bfloat16, True, slots=6)
+        slots = torch.tensor([[0, 1, 2, 3, 4], [5, 4, 3, 3, -1], [2, 2, 2, 9, 0]][rep], dtype=torch.int32, device="cuda")
+        before = state.clone()
+        out = ops.linear_attention_step(q, k, v, d, state, slots=slots, scale=0.5)
+        named = [s for s in dict.fromkeys(slots.tolist()) if 0 <= s < 6]
+        seqs = [([r for r, x in enumerate(slots.tolist()) if x == s], s) for s in named]
+        check_attention(q, k, v, d, seqs, before, 0.5, out, state)
+        given = torch.empty_like(v)
+        assert ops.linear_attention_step(q, k, v, d, before, slots=slots, scale=0.5, out=given) is given
+        assert torch.equal(given, out) and torch.equal(before, state)
+
+        x = rand(rep, 3, 7, 40)
+        codes, scales = ops.state_cache(4, 7, 40, block=16)
+        s3 = torch.tensor([3, 0, 2], dtype=torch.int32, device="cuda")
+        ops.state_store(x, codes, scales, block=16, slots=s3)
+        want_c, want_s = quantised(x, 16, torch.int8)
+        assert np.array_equal(codes[s3.long()].float().cpu().numpy(), want_c)
+        for back in DT.values():
+            y = ops.state_load(codes, scales, block=16, slots=s3, dtype=back)
+            assert torch.equal(y.cpu(), torch.from_numpy(want_c.astype(np.float32) * np.repeat(want_s, 16, 2)[:, :, :40]).to(back))
+
+        for n, p, c, g in ((3, 1, 96, 4), (2, 300, 96, 8), (1, 20000, 12, 1)):
+            x = rand(rep + 9, n, p, c)
+            w = 1 + 0.1 * rand(rep, c)
+            check_norm(x, g, w, None, "silu", ops.group_norm(x, g, w))
+            y = torch.empty_like(x)
+            assert ops.group_norm(x, g, w, out=y) is y and torch.equal(y, ops.group_norm(x, g, w))
+    from ssla_rt_b200.engine import SslaError
+    with pytest.raises(SslaError):
+        ops.linear_attention_step(q, k, v, d, state, slots=slots, scale=0.5, out=v)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.linear_attention_step(q.clone().requires_grad_(), k, v, d, state, slots=slots, scale=0.5)
+    with pytest.raises(ValueError, match="slots"):
+        ops.linear_attention_step(q, k, v, d, state, slots=slots.long(), scale=0.5)
+    with pytest.raises(SslaError):
+        ops.group_norm(x, g, x.reshape(-1)[:c], out=x)
