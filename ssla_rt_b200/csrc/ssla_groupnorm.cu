@@ -31,6 +31,7 @@ struct GnArgs {
     int n, positions, channels, groups, width;     // width: channels of a group
     int act;
     int wide;                                      // weight and bias are 16-byte aligned
+    int stream;                                    // x and y are too large for L2
     float* shift;                                  // large slabs: what their sums are shifted by
     float eps;
 };
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kGnThreads, LPS <= 32 && EPT == 1 ? kGnSlabCta
                 for (int j = 0; j < VEC; ++j) v[u][e][j] = 0.0f;
                 if (n[u] >= 0 && k < vecs) {
                     const int p = a.positions == 1 ? 0 : k / wv;
-                    load_vec<T, VEC>(xp + p * a.x_pos + (k - p * wv) * VEC, v[u][e]);
+                    load_vec_hint<T, VEC>(xp + p * a.x_pos + (k - p * wv) * VEC, v[u][e], a.stream);
                 }
             }
         }
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kGnThreads, LPS <= 32 && EPT == 1 ? kGnSlabCta
                 if (k < vecs) {
                     const int p = a.positions == 1 ? 0 : k / wv, c = (k - p * wv) * VEC;
                     gn_finish<VEC>(v[u][e], mean[u], rstd[u], w[e], b[e], a.act);
-                    store_vec<T, VEC>(yp + p * a.y_pos + c, v[u][e]);
+                    store_vec_hint<T, VEC>(yp + p * a.y_pos + c, v[u][e], a.stream);
                 }
             }
         }
@@ -594,6 +595,7 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
     d.act = a->activation; d.eps = a->eps;
     d.wide = aligned(a->weight, 16) && aligned(a->bias, 16);
     d.shift = nullptr;
+    d.stream = 2LL * a->n * a->positions * a->channels * dtype_size(a->dtype) > kStreamBytes;
     const int vec = gn_vec(a);
     auto run = [&](auto t, auto v) {
         using T = decltype(t);

@@ -16,17 +16,21 @@ namespace ops {
 namespace {
 
 // ---------------------------------------------------------------------------
-// One token per row: a CTA holds a head's state columns [c0, c0 + COLS) in
+// One token per row: a CTA holds a head's state columns [c0, c0 + 32) in
 // registers and applies the rows that name its slot.  Memory bound: the state
 // is read and written once, 8 dk dv bytes; everything a token needs is asked
 // for together with the state, before the slots are compared, and the state
-// leaves before the output is summed up.
+// leaves before the output is summed up.  256 rows of 16 heads of 128 x 128:
+// 94 us, 89% of the measured copy rate (105 us without the streaming hints).
 //
 // Thread (tx, rg): columns c0 + tx * VEC .. + VEC, state rows rg + i * RG.
 // ---------------------------------------------------------------------------
-template <typename T, int VEC, int RPT, int COLS>
+constexpr int kStepThreads = 128;
+constexpr int kStepCols = 32;
+
+template <typename T, int VEC, int RPT>
 struct StepTile {
-    static constexpr int kThreads = 4 * COLS, TX = COLS / VEC, RG = kThreads / TX;
+    static constexpr int TX = kStepCols / VEC, RG = kStepThreads / TX;
     float s[RPT][VEC], kk[RPT], qq[RPT], vv[VEC], g;
     int tx, rg, c0;
     bool live;                                     // this thread's columns exist
@@ -34,7 +38,7 @@ struct StepTile {
     __device__ void place(const LinArgs& a) {
         tx = threadIdx.x % TX;
         rg = threadIdx.x / TX;
-        c0 = blockIdx.x * COLS + tx * VEC;
+        c0 = blockIdx.x * kStepCols + tx * VEC;
         live = c0 < a.dv;
     }
     __device__ float* at(const LinArgs& a, int slot, int h) const {
@@ -44,13 +48,15 @@ struct StepTile {
         const float* p = at(a, slot, h);
 #pragma unroll
         for (int i = 0; i < RPT; ++i)
-            if (live && rg + i * RG < a.dk) load_vec<float, VEC>(p + static_cast<size_t>(rg + i * RG) * a.dv, s[i]);
+            if (live && rg + i * RG < a.dk)
+                load_vec_hint<float, VEC>(p + static_cast<size_t>(rg + i * RG) * a.dv, s[i], a.stream);
     }
     __device__ void store(const LinArgs& a, int slot, int h) const {
         float* p = at(a, slot, h);
 #pragma unroll
         for (int i = 0; i < RPT; ++i)
-            if (live && rg + i * RG < a.dk) store_vec<float, VEC>(p + static_cast<size_t>(rg + i * RG) * a.dv, s[i]);
+            if (live && rg + i * RG < a.dk)
+                store_vec_hint<float, VEC>(p + static_cast<size_t>(rg + i * RG) * a.dv, s[i], a.stream);
     }
     __device__ void fetch(const LinArgs& a, int row, int h) {
         const T* q = static_cast<const T*>(a.q) + row * a.q_row + (h / a.q_share) * a.q_head;
@@ -90,23 +96,23 @@ struct StepTile {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         if (lane < TX)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) red[warp * COLS + tx * VEC + j] = o[j];
+            for (int j = 0; j < VEC; ++j) red[warp * kStepCols + tx * VEC + j] = o[j];
         __syncthreads();
-        const int c = blockIdx.x * COLS + threadIdx.x;
-        if (threadIdx.x < COLS && c < a.dv) {
+        const int c = blockIdx.x * kStepCols + threadIdx.x;
+        if (threadIdx.x < kStepCols && c < a.dv) {
             float t = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kThreads / 32; ++w) t += red[w * COLS + threadIdx.x];
+            for (int w = 0; w < kStepThreads / 32; ++w) t += red[w * kStepCols + threadIdx.x];
             static_cast<T*>(a.out)[row * a.out_row + h * a.out_head + c] = from_f<T>(t * a.scale);
         }
         __syncthreads();
     }
 };
 
-template <typename T, int VEC, int RPT, int COLS>
-__global__ void __launch_bounds__(4 * COLS) k_linattn_step(LinArgs a, const int* __restrict__ slots) {
-    using Tile = StepTile<T, VEC, RPT, COLS>;
-    __shared__ float red[Tile::kThreads / 32 * COLS];
+template <typename T, int VEC, int RPT>
+__global__ void __launch_bounds__(kStepThreads) k_linattn_step(LinArgs a, const int* __restrict__ slots) {
+    using Tile = StepTile<T, VEC, RPT>;
+    __shared__ float red[kStepThreads / 32 * kStepCols];
     __shared__ int next_s;
     Tile t;
     t.place(a);
@@ -114,8 +120,8 @@ __global__ void __launch_bounds__(4 * COLS) k_linattn_step(LinArgs a, const int*
     int row = blockIdx.z;
     const int slot = slots ? slots[row] : row;
     if (slot < 0 || slot >= a.n_slots) {           // padding row
-        const int c = blockIdx.x * COLS + threadIdx.x;
-        if (threadIdx.x < COLS && c < a.dv)
+        const int c = blockIdx.x * kStepCols + threadIdx.x;
+        if (threadIdx.x < kStepCols && c < a.dv)
             static_cast<T*>(a.out)[row * a.out_row + h * a.out_head + c] = from_f<T>(0.0f);
         return;
     }
@@ -126,7 +132,7 @@ __global__ void __launch_bounds__(4 * COLS) k_linattn_step(LinArgs a, const int*
         if (slots) {
             // rows that name this slot: the first of them applies all, in row order
             if (threadIdx.x == 0) next_s = INT_MAX;
-            for (int r = threadIdx.x; r < a.n_rows; r += Tile::kThreads)
+            for (int r = threadIdx.x; r < a.n_rows; r += kStepThreads)
                 if (r != row && slots[r] == slot) {
                     if (r < row) before = 1;
                     else next = min(next, r);
@@ -149,26 +155,24 @@ __global__ void __launch_bounds__(4 * COLS) k_linattn_step(LinArgs a, const int*
 
 // ---- host ----------------------------------------------------------------
 
-// The state rows of a thread, and 64 columns a CTA where there are as many
-// and vectors of four, else 32: wider runs of a state row at a time (256
-// rows, 16 heads of 128 x 128: 105 us with 32 columns).
-template <typename F> int with_tile(int dtype, bool vec4, int dk, int dv, F&& f) {
+// The state rows of a thread, by dk and the vector width.  (CTAs of 64 columns
+// and 256 threads were slower: 114 us against 105 for 256 rows of 16 heads of
+// 128 x 128.)
+template <typename F> int with_tile(int dtype, bool vec4, int dk, F&& f) {
     using std::integral_constant;
-    auto by_rows = [&](auto t, auto v, auto c) {
+    auto by_rows = [&](auto t, auto v) {
         constexpr int V = decltype(v)::value, RG = 4 * V;
-        if (dk <= 2 * RG) return f(t, v, integral_constant<int, 2>(), c);
-        if (dk <= 4 * RG) return f(t, v, integral_constant<int, 4>(), c);
-        if (dk <= 8 * RG) return f(t, v, integral_constant<int, 8>(), c);
+        if (dk <= 2 * RG) return f(t, v, integral_constant<int, 2>());
+        if (dk <= 4 * RG) return f(t, v, integral_constant<int, 4>());
+        if (dk <= 8 * RG) return f(t, v, integral_constant<int, 8>());
         if constexpr (V == 1) {
-            if (dk <= 16 * RG) return f(t, v, integral_constant<int, 16>(), c);
-            return f(t, v, integral_constant<int, 32>(), c);
+            if (dk <= 16 * RG) return f(t, v, integral_constant<int, 16>());
+            return f(t, v, integral_constant<int, 32>());
         }
         return fail(SSLA_ERR_ARG, "dk %d", dk);
     };
     auto by_vec = [&](auto t) {
-        if (!vec4) return by_rows(t, integral_constant<int, 1>(), integral_constant<int, 32>());
-        if (dv < 64) return by_rows(t, integral_constant<int, 4>(), integral_constant<int, 32>());
-        return by_rows(t, integral_constant<int, 4>(), integral_constant<int, 64>());
+        return vec4 ? by_rows(t, integral_constant<int, 4>()) : by_rows(t, integral_constant<int, 1>());
     };
     return dtype == SSLA_DT_F32 ? by_vec(float()) : dtype == SSLA_DT_BF16 ? by_vec(__nv_bfloat16()) : by_vec(__half());
 }
@@ -235,6 +239,7 @@ LinArgs device_args(const SslaLinAttn* a) {
     d.decay_row = a->decay_row; d.decay_head = a->decay_head;
     d.n_rows = a->n_rows; d.heads = a->heads; d.q_share = a->heads / a->q_heads; d.k_share = a->heads / a->k_heads;
     d.dk = a->dk; d.dv = a->dv; d.n_slots = a->n_slots; d.scale = a->scale;
+    d.stream = 8LL * a->n_rows * a->heads * a->dk * a->dv > kStreamBytes;   // the step's state traffic
     return d;
 }
 
@@ -298,11 +303,10 @@ int ssla_linattn_step(const SslaLinAttn* a, const int* slots, void* stream) {
     OnDevice dev(a->device);
     if (dev.err != SSLA_OK) return dev.err;
     const LinArgs d = device_args(a);
-    return with_tile(a->dtype, state_vec4(a), a->dk, a->dv, [&](auto t, auto v, auto r, auto c) {
-        constexpr int COLS = decltype(c)::value;
-        const dim3 grid((a->dv + COLS - 1) / COLS, a->heads, a->n_rows);
-        k_linattn_step<decltype(t), decltype(v)::value, decltype(r)::value, COLS>
-            <<<grid, 4 * COLS, 0, static_cast<cudaStream_t>(stream)>>>(d, slots);
+    return with_tile(a->dtype, state_vec4(a), a->dk, [&](auto t, auto v, auto r) {
+        const dim3 grid((a->dv + kStepCols - 1) / kStepCols, a->heads, a->n_rows);
+        k_linattn_step<decltype(t), decltype(v)::value, decltype(r)::value>
+            <<<grid, kStepThreads, 0, static_cast<cudaStream_t>(stream)>>>(d, slots);
         return launched("k_linattn_step");
     });
 }

@@ -16,6 +16,7 @@ struct LinArgs {
     long long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head, decay_row, decay_head;
     int n_rows, heads, q_share, k_share, dk, dv, n_slots;
     float scale;
+    int stream;                     // step: the states are too many for L2
 };
 
 struct Seq {

@@ -158,5 +158,58 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[V]) {
     *reinterpret_cast<Pack<T, V>*>(p) = k;
 }
 
+// What a call reads and writes once and is larger than this goes past L2
+// (evict first): it would only push out what others keep there.
+constexpr long long kStreamBytes = 64LL << 20;
+
+// load_vec / store_vec of 4 to 16 bytes with the streaming hint where asked.
+template <typename T, int V>
+__device__ __forceinline__ void load_vec_hint(const T* p, float (&x)[V], bool stream) {
+    constexpr int B = sizeof(T) * V;
+    if constexpr (B == 16 || B == 8 || B == 4) {
+        if (stream) {
+            Pack<T, V> k;
+            if constexpr (B == 16) {
+                const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+                memcpy(&k, &u, B);
+            } else if constexpr (B == 8) {
+                const uint2 u = __ldcs(reinterpret_cast<const uint2*>(p));
+                memcpy(&k, &u, B);
+            } else {
+                const uint32_t u = __ldcs(reinterpret_cast<const uint32_t*>(p));
+                memcpy(&k, &u, B);
+            }
+            unpack_vec<T, V>(k, x);
+            return;
+        }
+    }
+    load_vec<T, V>(p, x);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec_hint(T* p, const float (&x)[V], bool stream) {
+    constexpr int B = sizeof(T) * V;
+    if constexpr (B == 16 || B == 8 || B == 4) {
+        if (stream) {
+            Pack<T, V> k;
+            store_vec<T, V>(k.v, x);
+            if constexpr (B == 16) {
+                uint4 u;
+                memcpy(&u, &k, B);
+                __stcs(reinterpret_cast<uint4*>(p), u);
+            } else if constexpr (B == 8) {
+                uint2 u;
+                memcpy(&u, &k, B);
+                __stcs(reinterpret_cast<uint2*>(p), u);
+            } else {
+                uint32_t u;
+                memcpy(&u, &k, B);
+                __stcs(reinterpret_cast<uint32_t*>(p), u);
+            }
+            return;
+        }
+    }
+    store_vec<T, V>(p, x);
+}
+
 }  // namespace ops
 }  // namespace ssla

@@ -25,6 +25,7 @@ struct CacheArgs {
     const int* slots;
     long long x_state, x_row;
     int n, n_slots, rows, cols, block, blocks;     // blocks per row
+    int stream;                                    // the states are too many for L2
 };
 
 // RN(x / s) for |x| <= about 448 s, given y = RN(1 / s) and s, y well inside
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(kCacheThreads) k_state_store(CacheArgs a, cons
 #pragma unroll
                 for (int e = 0; e < EPT; ++e) {
                     const int k = (e * LG + lane) * VEC;
-                    if (k < width[u]) load_vec<T, VEC>(xp + k, v[u][e]);
+                    if (k < width[u]) load_vec_hint<T, VEC>(xp + k, v[u][e], a.stream);
                 }
             }
         }
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(kCacheThreads) k_state_load(CacheArgs a, T* __
                 }
             }
         }
-        store_vec<T, VEC>(xi + row * a.x_row + c, v);
+        store_vec_hint<T, VEC>(xi + row * a.x_row + c, v, a.stream);
     }
 }
 
@@ -252,6 +253,7 @@ CacheArgs cache_args(const SslaStateCache* c) {
     a.x_state = c->x_state; a.x_row = c->x_row;
     a.n = c->n; a.n_slots = c->n_slots; a.rows = c->rows; a.cols = c->cols; a.block = c->block;
     a.blocks = (c->cols + c->block - 1) / c->block;
+    a.stream = static_cast<long long>(c->n) * c->rows * c->cols * (dtype_size(c->dtype) + 1) > kStreamBytes;
     return a;
 }
 
