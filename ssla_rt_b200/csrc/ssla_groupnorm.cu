@@ -138,13 +138,18 @@ template <int LPS> __device__ __forceinline__ float slab_sum(float v, float* red
     return v;
 }
 
-constexpr int kGnSlabCtas = 4;     // resident CTAs per SM that the one-vector forms are built for
+// Resident CTAs per SM that the forms of one or two vectors are built for.
+// What bounds them is how many warps hide the loads and the exponentials:
+// 16,384 rows of 16 groups of 128 (bf16, SiLU) take 39 us (3.5 TB/s) with four
+// CTAs of two vectors a thread, 40 with one vector, 46 with three CTAs of twice
+// the slabs, 59 where six CTAs make the registers spill.
+constexpr int kGnSlabCtas = 4;
 
 // A thread takes UNR slabs at a time, gridDim.x * (slabs of a CTA) apart:
 // the launch makes that a multiple of the groups where it can, so that a
 // thread's channels, and the weights it keeps, stay the same.
 template <typename T, int VEC, int LPS, int EPT, int UNR>
-__global__ void __launch_bounds__(kGnThreads, LPS <= 32 && EPT == 1 ? kGnSlabCtas : 1) k_gn_slab(GnArgs a, const T* x, T* y) {
+__global__ void __launch_bounds__(kGnThreads, LPS <= 32 && EPT <= 2 ? kGnSlabCtas : 1) k_gn_slab(GnArgs a, const T* x, T* y) {
     __shared__ float red[kGnThreads / 32];
     constexpr int kPer = kGnThreads / LPS;
     const int lane = threadIdx.x % LPS;
@@ -501,8 +506,8 @@ bool gn_small(const SslaGroupNorm* a, int vec, int* lps, int* ept) {
     const long long vecs = static_cast<long long>(a->positions) * (a->channels / a->groups / vec);
     const int most = vec >= 8 ? 4 : 8;             // registers: 32 values a thread
     if (vecs <= 8) *lps = 8, *ept = 1;
-    else if (vecs <= 16) *lps = 16, *ept = 1;
-    else if (vecs <= 32) *lps = 32, *ept = 1;
+    else if (vecs <= 16) *lps = 8, *ept = 2;
+    else if (vecs <= 32) *lps = 16, *ept = 2;
     else if (vecs <= 64) *lps = 32, *ept = 2;
     else if (vecs <= 128) *lps = 32, *ept = 4;
     else if (vecs <= kGnThreads * most) *lps = kGnThreads, *ept = most;
@@ -620,10 +625,10 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
             constexpr integral_constant<int, 2> two;
             constexpr integral_constant<int, 4> four;
             constexpr integral_constant<int, 32> warp;
-            if (lps == 8) return go(integral_constant<int, 8>(), one, two);
-            if (lps == 16) return go(integral_constant<int, 16>(), one, two);
-            if (lps == 32 && ept == 1) return go(warp, one, two);
-            if (lps == 32 && ept == 2) return go(warp, two, two);
+            if (lps == 8 && ept == 1) return go(integral_constant<int, 8>(), one, two);
+            if (lps == 8) return go(integral_constant<int, 8>(), two, one);
+            if (lps == 16) return go(integral_constant<int, 16>(), two, one);
+            if (lps == 32 && ept == 2) return go(warp, two, one);
             if (lps == 32) return go(warp, four, one);
             return go(integral_constant<int, kGnThreads>(), integral_constant<int, (V >= 8 ? 4 : 8)>(), one);
         }
