@@ -34,8 +34,9 @@ enum { SSLA_LINATTN_MAX_DK = 128, SSLA_LINATTN_MAX_DV = 256 };
  * in elements.  Head h reads query head h / (heads / q_heads), keys alike.
  * decay: logarithms, at most 0, strides decay_row and decay_head (decay_row 0:
  * one decay per head); -infinity clears the state before the token.
- * state: [n_slots][heads][dk][dv], contiguous, updated in place.  `out` does
- * not overlap any input. */
+ * state: [n_slots][heads][dk][dv], contiguous, updated in place.  `out` and
+ * `state` overlap neither each other nor an input (the address ranges are
+ * compared). */
 typedef struct SslaLinAttn {
     const void *q, *k, *v;
     void* out;
@@ -70,7 +71,7 @@ int ssla_linattn_chunk_workspace(const SslaLinAttn* a, const int* offsets, const
 enum { SSLA_LINATTN_TIMED_OUT = 1 };
 int ssla_linattn_status(int device, unsigned* status);
 
-/* Recurrent form: one token per row.  Row r updates state slot slots[r]
+/* Recurrent form: one token per row, at most 65535 rows.  Row r updates state slot slots[r]
  * (device array; NULL: slot r, n_rows <= n_slots).  Rows that name the same
  * slot are applied in row order.  A slot outside [0, n_slots) marks a padding
  * row: its output is zero and no state is touched. */
@@ -88,7 +89,7 @@ int ssla_linattn_step(const SslaLinAttn* a, const int* slots, void* stream);
  * contiguous.
  * store writes state i to slot slots[i] (device array; NULL: slot i); where a
  * slot is named twice the last state naming it is kept; slots outside
- * [0, n_slots) are skipped.  load reads slot slots[i] into x[i]; a slot
+ * [0, n_slots) are skipped; at most 65535 states a call.  load reads slot slots[i] into x[i]; a slot
  * outside [0, n_slots) gives zeros. */
 typedef struct SslaStateCache {
     void* codes;

@@ -564,7 +564,15 @@ size_t gn_bytes(const SslaGroupNorm* a) {
     const int vec = gn_vec(a);
     int lps, ept;
     GnCluster c;
-    if (gn_small(a, vec, &lps, &ept) || gn_cluster(a, vec, &c)) return 0;
+    if (gn_small(a, vec, &lps, &ept)) return 0;
+    if (a->n > 65535) {                            // (done in parts: the first, and a smaller last one)
+        SslaGroupNorm part = *a;
+        part.n = 65535;
+        const size_t whole = gn_bytes(&part);
+        part.n = (a->n - 1) % 65535 + 1;
+        return std::max(whole, gn_bytes(&part));
+    }
+    if (gn_cluster(a, vec, &c)) return 0;
     return static_cast<size_t>(a->n) * a->groups * (gn_split(a, vec).splits * sizeof(float2) + sizeof(float));
 }
 
@@ -589,6 +597,19 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
     const size_t need = gn_bytes(a);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return fail(SSLA_ERR_ARG, "group norm: workspace of %zu bytes, %zu needed, 16-byte aligned", workspace_bytes, need);
+    int lps, ept;
+    if (a->n > 65535 && !gn_small(a, gn_vec(a), &lps, &ept)) {
+        // more samples than a grid's depth: in parts, one after the other on the stream
+        const int sz = dtype_size(a->dtype);
+        for (int n0 = 0; n0 < a->n; n0 += 65535) {
+            SslaGroupNorm part = *a;
+            part.n = std::min(a->n - n0, 65535);
+            part.x = static_cast<const char*>(a->x) + n0 * a->x_sample * sz;
+            part.y = static_cast<char*>(a->y) + n0 * a->y_sample * sz;
+            if (const int rc = ssla_group_norm(&part, workspace, workspace_bytes, stream); rc != SSLA_OK) return rc;
+        }
+        return SSLA_OK;
+    }
     OnDevice dev(a->device);
     if (dev.err != SSLA_OK) return dev.err;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -607,7 +628,6 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
         constexpr int V = decltype(v)::value;
         const T* x = static_cast<const T*>(a->x);
         T* y = static_cast<T*>(a->y);
-        int lps, ept;
         const long long slabs = static_cast<long long>(a->n) * a->groups;
         if (gn_small(a, vec, &lps, &ept)) {
             auto go = [&](auto l, auto e, auto un) {
@@ -651,8 +671,7 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
             return launched("k_gn_cluster");
         }
         const GnSplit s = gn_split(a, vec);
-        if (s.chunks > 65535 || a->n > 65535)
-            return fail(SSLA_ERR_ARG, "group norm: more than 65535 samples or group chunks of large slabs");
+        if (s.chunks > 65535) return fail(SSLA_ERR_ARG, "group norm: more than 65535 group chunks of large slabs");
         float2* part = static_cast<float2*>(workspace);
         d.shift = reinterpret_cast<float*>(part + static_cast<size_t>(slabs) * s.splits);
         const dim3 grid(s.splits, s.chunks, a->n);

@@ -256,6 +256,13 @@ __device__ __forceinline__ DecaySums chunk_decays(float2 g, int lane) {
 }
 
 // Segment states: [segment][head][dk][dv]; segment decays: [segment][head].
+// Where a divided sequence's segment finds its first state: the place of the
+// segment before it, the first one that of the last (which leaves none), since
+// the slot itself may already hold the last segment's result.
+__device__ __forceinline__ int first_state_of(const Table& tab, int seq, int seg) {
+    return seg ? tab.seg0[seq] + seg - 1 : tab.seg0[seq + 1] - 1;
+}
+
 template <typename T, int DK, int DV, bool OUT>
 __global__ void __launch_bounds__(kThreads, DK <= 32 && DV <= 32 ? 4 : 1)
 k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* seg_decay, int wide) {
@@ -289,7 +296,7 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
 
     float S[MT][SN][4];
     const float* from = nullptr;
-    if (OUT && seg > 0) from = seg_state + (static_cast<size_t>(blockIdx.z - 1) * a.heads + h) * head_state;
+    if (OUT && nseg > 1) from = seg_state + (static_cast<size_t>(first_state_of(tab, seq, seg)) * a.heads + h) * head_state;
     else if (OUT && slot >= 0) from = a.state + (static_cast<size_t>(slot) * a.heads + h) * head_state;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -536,7 +543,8 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
 #include "ssla_linattn_tc.cuh"
 
 // Chains a sequence's segments: segment i's place in the workspace becomes
-// the state after it.  One thread per state element.
+// the state after it, the last one's the state before all.  One thread per
+// state element.
 __global__ void __launch_bounds__(256)
 k_chunk_join(LinArgs a, const __grid_constant__ Table tab, float* seg_state, const double* seg_decay) {
     const int seq = blockIdx.z, h = blockIdx.y;
@@ -546,6 +554,7 @@ k_chunk_join(LinArgs a, const __grid_constant__ Table tab, float* seg_state, con
     const size_t head_state = static_cast<size_t>(a.dk) * a.dv;
     const int slot = tab.slot[seq];
     float run = slot >= 0 ? a.state[(static_cast<size_t>(slot) * a.heads + h) * head_state + e] : 0.0f;
+    seg_state[(static_cast<size_t>(s1) * a.heads + h) * head_state + e] = run;
     for (int s = s0; s < s1; s += 8) {
         float x[8], g[8];                                   // loads of eight segments in flight
 #pragma unroll

@@ -440,7 +440,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         float2 S[HC / 2];
         const float* from = nullptr;
-        if (OUT && seg > 0) from = seg_state + (static_cast<size_t>(blockIdx.z - 1) * a.heads + h) * head_state;
+        if (OUT && nseg > 1) from = seg_state + (static_cast<size_t>(first_state_of(tab, seq, seg)) * a.heads + h) * head_state;
         else if (OUT && slot >= 0) from = a.state + (static_cast<size_t>(slot) * a.heads + h) * head_state;
         {
             const bool there = from && d < width;

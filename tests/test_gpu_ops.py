@@ -519,6 +519,15 @@ def test_group_norm(dtype, n, p, c, g, act):
     check_norm(x, g, None, None, act, ops.group_norm(x, g, activation=act))
 
 
+@pytest.mark.parametrize("p,c,g", [(1, 3, 1), (1, 8196, 1), (4100, 2, 1)])
+def test_group_norm_more_samples_than_a_grid_is_deep(p, c, g):
+    n = 65535 + 70
+    x = rand(p, n, p, c)
+    y = ops.group_norm(x, g, activation="none")
+    for part in (slice(0, 40), slice(65500, None)):
+        check_norm(x[part], g, None, None, "none", y[part])
+
+
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("n,p,c,g", [(3, 1, 96, 4), (2, 300, 96, 8), (2, 5120, 24, 3)])
 def test_group_norm_large_mean(dtype, n, p, c, g):
