@@ -242,6 +242,84 @@ def test_non_finite_reaches_no_earlier_token(dtype, which, value):
     assert torch.isfinite(state[0, 0]).all() and torch.isfinite(state[1]).all()
 
 
+@pytest.mark.parametrize("dims", [(64, 64), (128, 128), (64, 96), (96, 200)], ids=str)
+@pytest.mark.parametrize("bad", [0, 5, 63, 64, 100, 199])
+@pytest.mark.parametrize("which", ["q", "k", "v"])
+@pytest.mark.parametrize("value", [math.nan, -math.inf])
+def test_non_finite_with_wide_heads(dims, bad, which, value):
+    """The same on the tensor memory path: in whole chunks and in the last, partial one."""
+    n, h, (dk, dv) = 201, 2, dims
+    q, k, v, d, state = inputs(141, n, h, h, h, dk, dv, torch.bfloat16, True, slots=1)
+    t = {"q": q, "k": k, "v": v}
+    before = state.clone()
+    out_clean = ops.linear_attention(q, k, v, d, state=state.clone(), scale=0.5)
+    col = 7 if which != "v" else dv - 3
+    t[which][bad, 1, col] = value
+    out = ops.linear_attention(q, k, v, d, state=state, scale=0.5)
+    seqs = [(range(n), 0)]
+    clean = [torch.nan_to_num(x, nan=0, posinf=0, neginf=0) for x in (q, k, v)]
+    check_attention(*[x[:, :1] for x in clean], d[:, :1], seqs, before[:, :1], 0.5, out[:, :1], None)
+    if bad:
+        check_attention(*[x[:, 1:] for x in clean], d[:, 1:], [(range(bad), 0)], before[:, 1:], 0.5, out[:, 1:], None, list(range(bad)))
+    finite = torch.isfinite(out[:, 1].float())
+    rest = [c for c in range(dv) if c != col]
+    if which == "q":
+        assert not finite[bad].any() and finite[bad + 1:].all() and torch.isfinite(state).all()
+        check_attention(*[x[:, 1:] for x in clean], d[:, 1:], seqs, before[:, 1:], 0.5, out[:, 1:], None,
+                        [r for r in range(n) if r != bad])
+    elif which == "v":
+        assert not finite[bad:, col].any() and finite[:, rest].all()
+        assert not torch.isfinite(state[0, 1, :, col]).any() and torch.isfinite(state[0, 1][:, rest]).all()
+        assert torch.equal(out[:, 1][:, rest], out_clean[:, 1][:, rest])
+    else:
+        assert not finite[bad:].any() and not torch.isfinite(state[0, 1]).all()
+    assert torch.isfinite(state[0, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dims", [(64, 64), (128, 128)], ids=str)
+def test_linear_attention_broadcast_inputs_and_unaligned_outputs(dtype, dims):
+    """Queries shared by all heads, keys by all rows, values by both (strides of 0); outputs off 16-byte places."""
+    h, n, (dk, dv) = 3, 200, dims
+    q = rand(1, n, 1, dk, dtype=DT[dtype], std=dk ** -0.25).expand(n, h, dk)
+    k = rand(2, 1, h, dk, dtype=DT[dtype], std=dk ** -0.25).expand(n, h, dk)
+    v = rand(3, 1, 1, dv, dtype=DT[dtype]).expand(n, h, dv)
+    d = -rand(4, n, h).abs() * 0.3
+    whole = torch.full((n, h, dv + 3), 7.0, dtype=DT[dtype], device="cuda")
+    out = whole[:, :, 1:1 + dv]
+    ops.linear_attention(q, k, v, d, offsets=[0, 130, n], out=out)
+    check_attention(q, k, v, d, [(range(130), -1), (range(130, n), -1)], None, 1.0, out, None)
+    assert (whole[:, :, 0] == 7).all() and (whole[:, :, 1 + dv:] == 7).all()
+
+
+def test_wide_heads_on_two_streams_and_threads():
+    """Two calls at once, each from a thread and on a stream of its own, against the same calls alone."""
+    import threading
+    sets = [inputs(151 + i, 3000, 8, 8, 8, 128, 128, torch.bfloat16, True, slots=1) for i in range(2)]
+    alone = []
+    for q, k, v, d, state in sets:
+        st = state.clone()
+        alone.append((ops.linear_attention(q, k, v, d, state=st), st))
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        q, k, v, d, state = sets[i]
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                st = state.clone()
+                got[i] = (ops.linear_attention(q, k, v, d, state=st), st)
+        s.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    for (o, s), (wo, ws) in zip(got, alone):
+        assert torch.equal(o, wo) and torch.equal(s, ws)
+
+
 def test_linear_attention_empty():
     q, k, v, d, state = inputs(1, 0, 2, 2, 2, 8, 8, torch.bfloat16, True, slots=2)
     before = state.clone()
