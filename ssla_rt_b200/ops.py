@@ -43,7 +43,8 @@ def _fast_module():
         return None
     lib = load_library()
     m.init(_PLANS, *[C.cast(getattr(lib, n), C.c_void_p).value for n in (
-        "ssla_linattn_step", "ssla_state_store", "ssla_state_load", "ssla_group_norm", "ssla_group_norm_workspace")])
+        "ssla_linattn_step", "ssla_state_store", "ssla_state_load", "ssla_group_norm", "ssla_group_norm_workspace",
+        "ssla_linattn_chunk", "ssla_linattn_chunk_workspace")])
     return m
 
 
@@ -245,6 +246,11 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     Returns out, (rows, heads, dv); rows outside every sequence are zero in a
     new tensor and left as they were in a given one.
     """
+    if _fast is not None and stream is None:
+        r = _fast.chunk(q, k, v, decay, state, scale, out, offsets, lengths, slots, False)
+        if r is not None:
+            return _fast_result(r)
+    given = out
     if offsets is None:
         if lengths is not None:
             raise ValueError("lengths without offsets")
@@ -268,6 +274,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
         if slots.size != n_seq:
             raise ValueError(f"{slots.size} slots for {n_seq} sequences")
     a = _linattn(q, k, v, decay, state, scale, out)
+    if _fast is not None:
+        _keep_plan(_fast.chunk(q, k, v, decay, state, scale, given, None, None, None, True), a)
     handle, ts = _stream_of(stream, a.device)
     if out is None:
         out = _like(v, ts, zero=gaps)

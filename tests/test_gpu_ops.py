@@ -810,3 +810,42 @@ def test_repeated_calls_answer_like_the_first():
         ops.linear_attention_step(q, k, v, d, state, slots=slots.long(), scale=0.5)
     with pytest.raises(SslaError):
         ops.group_norm(x, g, x.reshape(-1)[:c], out=x)
+
+
+def test_repeated_sequence_calls_answer_like_the_first():
+    """linear_attention again on the same shapes: other sequences, host arrays of every kind, gaps, given outputs, refusals."""
+    from ssla_rt_b200.engine import SslaError
+    n = 90
+    for rep, kw in enumerate([dict(offsets=[0, 30, 90]), dict(offsets=np.array([0, 30, 90], np.int32)),
+                              dict(offsets=np.array([0, 30, 80], np.int32)), dict(offsets=torch.tensor([0, 1, 90])),
+                              dict(offsets=np.array([5, 50], np.int32), lengths=np.array([20, 40], np.int32)),
+                              dict(offsets=np.array([5, 50], np.int64), lengths=[20, 0]),
+                              dict(offsets=np.array([0, 30, 90], np.int32), slots=np.array([2, -1], np.int32)),
+                              dict(), dict(offsets=np.array([10], np.int32)),
+                              dict(offsets=np.array([0, 30, 90, 7], np.int32)[:3])]):
+        q, k, v, d, state = inputs(201 + rep, n, 2, 2, 2, 24, 40, torch.bfloat16, True, slots=3)
+        before = state.clone()
+        off = [int(x) for x in kw.get("offsets", [0, n])]
+        lens = [int(x) for x in kw["lengths"]] if "lengths" in kw else [b - a for a, b in zip(off, off[1:])]
+        slots = [int(x) for x in kw.get("slots", range(len(lens)))]
+        seqs = [(range(off[i], off[i] + m), s) for i, (m, s) in enumerate(zip(lens, slots))]
+        out = ops.linear_attention(q, k, v, d, state=state, scale=0.5, **kw)
+        inside = sorted(r for rr, _ in seqs for r in rr)
+        if inside:
+            check_attention(q, k, v, d, seqs, before, 0.5, out, state, inside)
+        assert (out[[r for r in range(n) if r not in set(inside)]] == 0).all()
+        given = torch.full_like(v, 7.0)
+        again = before.clone()
+        assert ops.linear_attention(q, k, v, d, state=again, scale=0.5, out=given, **kw) is given
+        assert torch.equal(given[inside], out[inside]) and torch.equal(again, state)
+        assert (given[[r for r in range(n) if r not in set(inside)]] == 7).all()
+    for bad in (dict(offsets=np.array([0, 91], np.int32)), dict(offsets=np.array([50, 30], np.int32)),
+                dict(offsets=np.array([0, 30, 90], np.int32), slots=np.array([1, 1], np.int32)),
+                dict(offsets=np.array([0, 30, 90], np.int32), slots=np.array([3, 0], np.int32))):
+        with pytest.raises(SslaError):
+            ops.linear_attention(q, k, v, d, state=state, scale=0.5, **bad)
+    for bad in (dict(offsets=np.array([0, 30, 90], np.int32), slots=np.array([1], np.int32)), dict(lengths=[3]),
+                dict(offsets=np.array([], np.int32)), dict(offsets=np.zeros((2, 2), np.int32)),
+                dict(offsets=torch.tensor([0, 90], device="cuda", dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            ops.linear_attention(q, k, v, d, state=state, scale=0.5, **bad)
