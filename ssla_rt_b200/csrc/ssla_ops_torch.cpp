@@ -75,6 +75,22 @@ const at::Tensor* take(PyObject* o, Key& key, bool grad_mode, bool needed) {
     return &t;
 }
 
+// A Python int into the key; anything else (numpy's integers, tensors) has no
+// place there, and ops.py takes the call.
+void put_int(PyObject* o, Key& key) {
+    if (!PyLong_Check(o)) {
+        key.ok = false;
+        return;
+    }
+    const long long x = PyLong_AsLongLong(o);
+    if (x == -1 && PyErr_Occurred()) {
+        PyErr_Clear();
+        key.ok = false;
+        return;
+    }
+    key.put(x);
+}
+
 // The block under the key, copied; false: there is none.
 template <typename Block> bool find(const Key& key, Block& b) {
     if (!key.ok) return false;
@@ -239,17 +255,12 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
     SSLA_BEGIN
     // x, codes, scales, block, slots, key_only
     if (n != 6) Py_RETURN_NONE;
-    const long block = PyLong_Check(a[3]) ? PyLong_AsLong(a[3]) : -1;
-    if (PyErr_Occurred()) {
-        PyErr_Clear();
-        Py_RETURN_NONE;
-    }
     const bool gm = c10::GradMode::is_enabled();
     Key key;
     key.put<int32_t>(2);
     const at::Tensor *x = take(a[0], key, gm, true), *c = take(a[1], key, false, true), *s = take(a[2], key, gm, true);
     const at::Tensor* slots = take(a[4], key, false, false);
-    key.put(block);
+    put_int(a[3], key);
     if (a[5] == Py_True) return key_of(key);
     SslaStateCache b;
     if (!find(key, b)) Py_RETURN_NONE;
@@ -260,21 +271,15 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyObject* load(PyObject*, PyObject* const* a, Py_ssize_t n) {
     SSLA_BEGIN
-    // codes, scales, block, slots, dtype's example tensor, out, key_only
+    // codes, scales, block, slots, dtype's code (SSLA_DT_*), out, key_only
     if (n != 7) Py_RETURN_NONE;
-    const long block = PyLong_Check(a[2]) ? PyLong_AsLong(a[2]) : -1;
-    const long dtype = PyLong_Check(a[4]) ? PyLong_AsLong(a[4]) : -1;
-    if (PyErr_Occurred()) {
-        PyErr_Clear();
-        Py_RETURN_NONE;
-    }
     const bool gm = c10::GradMode::is_enabled();
     Key key;
     key.put<int32_t>(3);
     const at::Tensor *c = take(a[0], key, false, true), *s = take(a[1], key, gm, true);
     const at::Tensor *slots = take(a[3], key, false, false), *out = take(a[5], key, gm, false);
-    key.put(block);
-    key.put(dtype);
+    put_int(a[2], key);
+    put_int(a[4], key);
     if (a[6] == Py_True) return key_of(key);
     SslaStateCache b;
     if (!find(key, b)) Py_RETURN_NONE;
@@ -294,8 +299,6 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     SSLA_BEGIN
     // x, groups, weight, bias, eps, activation, out, key_only
     if (n != 8) Py_RETURN_NONE;
-    const long groups = PyLong_Check(a[1]) ? PyLong_AsLong(a[1]) : -1;
-    const long act = PyLong_Check(a[5]) ? PyLong_AsLong(a[5]) : -1;
     const double eps = PyFloat_AsDouble(a[4]);
     if (PyErr_Occurred()) {
         PyErr_Clear();
@@ -306,8 +309,8 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     key.put<int32_t>(4);
     const at::Tensor *x = take(a[0], key, gm, true), *w = take(a[2], key, gm, false), *bias = take(a[3], key, gm, false);
     const at::Tensor* out = take(a[6], key, gm, false);
-    key.put(groups);
-    key.put(act);
+    put_int(a[1], key);
+    put_int(a[5], key);
     key.put(eps);
     if (a[7] == Py_True) return key_of(key);
     SslaGroupNorm b;
