@@ -15,6 +15,7 @@ is no CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import Optional, Sequence, Tuple
 
 import numpy as np
@@ -64,6 +65,21 @@ def _fast_result(r):
     if type(r) is int:
         _check(-r)
     return r
+
+
+def _real(name: str, x) -> float:
+    """x's value now: a tensor would be kept, and compared, by what it is rather than by what it holds."""
+    try:
+        return float(x)
+    except (TypeError, ValueError, RuntimeError):
+        raise ValueError(f"{name} is {x!r}: a number is needed") from None
+
+
+def _whole(name: str, x) -> int:
+    try:
+        return operator.index(x)
+    except (TypeError, RuntimeError):
+        raise ValueError(f"{name} is {x!r}: a whole number is needed") from None
 
 
 def _sig(t: Optional[torch.Tensor]):
@@ -214,6 +230,7 @@ def _linattn_block(q, k, v, decay, state, scale, out, step_slots=None):
 def _linattn(q, k, v, decay, state, scale, out, slots=None):
     """The checked argument block of a call with every pointer but out's."""
     _no_grad(q, k, v, decay, state)
+    scale = _real("scale", scale)
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(),
            v.shape, v.stride(), v.dtype, v.get_device(), decay.shape, decay.stride(), decay.dtype, decay.get_device(),
            scale, _sig(state), _sig(out), _sig(slots))
@@ -380,6 +397,7 @@ def _cache(codes, scales, block, slots, n, name, x, dtype):
     if slots is not None and not isinstance(slots, torch.Tensor):
         raise ValueError("slots is a one-dimensional int32 tensor")
     _no_grad(x, scales)
+    block = _whole("block", block)
     key = ("cache", _sig(codes), _sig(scales), block, _sig(slots), n, name, _sig(x), dtype)
     c = abi.SslaStateCache.from_buffer_copy(
         _plan(key, lambda: _cache_block(codes, scales, block, slots, n, name, x, dtype)))
@@ -490,6 +508,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
                        out=None if out is None else out[:, None], stream=stream)
         return y[:, 0] if out is None else out
     _no_grad(x, weight, bias)
+    groups, eps = _whole("groups", groups), _real("eps", eps)
     given = out
     key = ("norm", _sig(x), groups, _sig(weight), _sig(bias), eps, activation, _sig(out))
     a = abi.SslaGroupNorm.from_buffer_copy(
