@@ -111,6 +111,8 @@ int ssla_state_load(const SslaStateCache* c, void* x, void* stream);
  *     y = act((x - mean) / sqrt(var + eps) * weight + bias),
  * mean and (biased) variance over the group's positions and channels.
  * weight and bias: [channels] 32-bit, each may be NULL.  y may be x itself.
+ * At most 2^24 channels, 2^40 values a sample, 2^31 - 2^16 positions and as
+ * many slabs (samples x groups).
  * `workspace`: ssla_group_norm_workspace bytes, 16-byte aligned. */
 typedef struct SslaGroupNorm {
     const void* x;

@@ -480,8 +480,10 @@ int check_gn(const SslaGroupNorm* a) {
         return fail(SSLA_ERR_ARG, "%s: %d channels in %d groups", who, a->channels, a->groups);
     if (!(a->eps >= 0.0f) || !std::isfinite(a->eps)) return fail(SSLA_ERR_ARG, "%s: eps %g", who, a->eps);
     if (a->n == 0 || a->positions == 0 || a->channels == 0) return SSLA_OK;
-    if (a->positions > (1LL << 40) / a->channels || a->channels > (1 << 24) || a->n > INT_MAX / a->groups)
-        return fail(SSLA_ERR_ARG, "%s: too large", who);
+    // positions and samples are stepped over in 32 bits, by a few thousand at most
+    if (a->positions > std::min((1LL << 40) / a->channels, INT_MAX - 65536LL) || a->channels > (1 << 24) ||
+        a->n > (INT_MAX - 65536) / a->groups)
+        return fail(SSLA_ERR_ARG, "%s: %d samples of %d positions, %d channels: too large", who, a->n, a->positions, a->channels);
     if (!a->x || !a->y) return fail(SSLA_ERR_ARG, "%s: null pointer", who);
     const int sz = dtype_size(a->dtype);
     if (!aligned(a->x, sz) || !aligned(a->y, sz) || !aligned(a->weight, 4) || !aligned(a->bias, 4))
