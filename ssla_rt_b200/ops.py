@@ -150,9 +150,16 @@ def _new(x: torch.Tensor, shape, dtype, stream) -> torch.Tensor:
         return x.new_empty(shape, dtype=dtype)
 
 
+def _counts(name: str, t: Optional[torch.Tensor]) -> None:
+    """An argument block counts in 32 bits, and ctypes would wrap what does not fit."""
+    if t is not None and t.dim() and max(t.shape) > 2**31 - 1:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}: sizes are below 2^31")
+
+
 def _rows_heads(name: str, t: torch.Tensor, dtype=None) -> None:
     if t.dim() != 3:
         raise ValueError(f"{name} has shape {tuple(t.shape)}: (rows, heads, width) is needed")
+    _counts(name, t)
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} is {t.dtype}, not {dtype}")
     if t.shape[2] > 1 and t.stride(2) != 1:
@@ -199,6 +206,7 @@ def _linattn_block(q, k, v, decay, state, scale, out, step_slots=None):
     if decay.dtype != torch.float32 or tuple(decay.shape) not in ((heads,), (n, heads)):
         raise ValueError(f"decay is {decay.dtype} {tuple(decay.shape)}: float32 ({heads},) or ({n}, {heads}) is needed")
     a = abi.SslaLinAttn()
+    _counts("state", state)
     if state is not None:
         if state.dtype != torch.float32 or state.dim() != 4 or tuple(state.shape[1:]) != (heads, dk, dv):
             raise ValueError(f"state is {state.dtype} {tuple(state.shape)}: float32 (slots, {heads}, {dk}, {dv}) is needed")
@@ -271,6 +279,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     if offsets is None:
         if lengths is not None:
             raise ValueError("lengths without offsets")
+        _counts("v", v)
         off = np.array([0, v.shape[0]], dtype=np.int32)
         n_seq, gaps = 1, False
     else:
@@ -366,6 +375,8 @@ def _cache_block(codes, scales, block, slots, n, name, x, dtype):
     """Checks a store or load; the argument block without its pointers."""
     if codes.dtype not in _FORMATS or codes.dim() != 3 or not codes.is_contiguous():
         raise ValueError("codes is a contiguous (slots, rows, cols) tensor of int8 or float8_e4m3fn")
+    _counts("codes", codes)
+    _counts(name, x)
     if not 1 <= block <= 256:
         raise ValueError(f"block {block} must be 1..256")
     n_slots, rows, cols = codes.shape
@@ -462,6 +473,7 @@ def _norm_block(x, groups, weight, bias, eps, activation, out):
     if x.dtype not in _DTYPES or x.dim() != 3:
         raise ValueError(f"x is {x.dtype} {tuple(x.shape)}: (samples, positions, channels) or (rows, channels) of "
                          f"float32, bfloat16 or float16 is needed")
+    _counts("x", x)
     n, positions, channels = x.shape
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation {activation!r}: silu or none")
