@@ -7,9 +7,18 @@
 //     registers; one read, two-pass statistics, one write;
 //   - slabs that fit the shared memory of a cluster of up to eight CTAs
 //     (k_gn_cluster): one read, one write;
-//   - others: k_gn_sums leaves every slab's shifted sums per slice of the
-//     positions in the workspace, k_gn_apply joins them (in 64 bits) and
-//     writes the outputs; the second read mostly comes from L2.
+//   - others: k_gn_sums leaves every slab's sums per slice of the positions in
+//     the workspace, k_gn_apply joins them and writes the outputs; the second
+//     read mostly comes from L2.
+//
+// The last two take the moments in one pass.  A thread sums the differences of
+// its values, and their squares, from the mean of its own first vector in 32
+// bits, and folds them into moments about zero in 64 (fold), in which they are
+// joined.  The mean of k of n values is at most sqrt(n / k) of their deviation
+// from the mean of all, so that the squares add up to at most 1 + n / k times
+// what is left of them, whatever the values are: n / k is a thread's vectors
+// between folds, at most kGnFold or a cluster's rounds.  (A shift by one value
+// of the whole slab lost three digits where that value was an outlier.)
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -32,7 +41,6 @@ struct GnArgs {
     int act;
     int wide;                                      // weight and bias are 16-byte aligned
     int stream;                                    // x and y are too large for L2
-    float* shift;                                  // large slabs: what their sums are shifted by
     float eps;
     double inv;                                    // 1 / values of a slab
 };
@@ -62,6 +70,15 @@ template <int VEC> __device__ __forceinline__ void moments(const float (&x)[VEC]
             s2 = __ffma2_rn(d, d, s2);
         }
     }
+}
+
+// Adds n values, given as the sums of their differences from `shift` and of
+// those' squares, to moments about zero (a mean of 2^20 deviations still
+// leaves 13 bits of the variance there).
+__device__ __forceinline__ void fold(double2& m, int n, float shift, float2 s1, float2 s2) {
+    const double d = static_cast<double>(s1.x) + s1.y, ns = static_cast<double>(n) * shift;
+    m.x += d + ns;
+    m.y += (static_cast<double>(s2.x) + s2.y) + shift * (2.0 * d + ns);
 }
 
 // y / (1 + e^-y) with the hardware's exponential and reciprocal: relative
@@ -242,38 +259,43 @@ struct GnSplit {
     int splits, chunks, gpc, tx, ty;
 };
 
-__device__ __forceinline__ float gn_shift(float x) { return fabsf(x) <= 3.402823466e38f ? x : 0.0f; }
+constexpr int kGnFold = 32;                       // vectors of a thread between two folds
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kGnThreads) k_gn_sums(GnArgs a, GnSplit s, const T* x, float2* part) {
-    __shared__ float2 red[kGnThreads];
+__global__ void __launch_bounds__(kGnThreads, 8) k_gn_sums(GnArgs a, GnSplit s, const T* x, double2* part) {
+    __shared__ double2 red[kGnThreads];
     const int n = blockIdx.z, g0 = blockIdx.y * s.gpc, ng = min(s.gpc, a.groups - g0);
     const int wv = a.width / VEC, cv = ng * wv;
     const int p0 = static_cast<int>(static_cast<long long>(a.positions) * blockIdx.x / s.splits);
     const int p1 = static_cast<int>(static_cast<long long>(a.positions) * (blockIdx.x + 1) / s.splits);
     const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx;
     const T* xn = x + n * a.x_sample + static_cast<long long>(g0) * a.width;
-    float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
+    red[threadIdx.x] = make_double2(0.0, 0.0);     // (here rather than in registers, which are what limits the CTAs)
     if (ty < s.ty)
-        for (int c = tx; c < cv; c += s.tx) {
-            // the first position's first channel of the group as the shift
-            const float shift = gn_shift(to_f<T>(xn[c / wv * a.width]));
+        for (int c = tx; c < cv; c += s.tx) {      // (more than one: all of one group)
             const T* xp = xn + c * VEC;
-#pragma unroll 4
-            for (int p = p0 + ty; p < p1; p += s.ty) {
+            for (int p = p0 + ty; p < p1;) {
+                const int end = min(p1, p + kGnFold * s.ty);
                 float v[VEC];
                 load_vec<T, VEC>(xp + p * a.x_pos, v);
-                moments<VEC>(v, shift, s1, s2);
+                const float shift = add_up<VEC>(v) * (1.0f / VEC);
+                const int count = ((end - p - 1) / s.ty + 1) * VEC;
+                float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
+#pragma unroll 4
+                for (; p < end; p += s.ty) {
+                    load_vec<T, VEC>(xp + p * a.x_pos, v);
+                    moments<VEC>(v, shift, s1, s2);
+                }
+                fold(red[threadIdx.x], count, shift, s1, s2);
             }
         }
-    red[threadIdx.x] = make_float2(s1.x + s1.y, s2.x + s2.y);
     __syncthreads();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     for (int g = warp; g < ng; g += kGnThreads / 32) {
         const int w = ng == 1 ? min(s.tx, wv) : wv, lo = ng == 1 ? 0 : g * wv;
-        float a1 = 0.0f, a2 = 0.0f;
+        double a1 = 0.0, a2 = 0.0;
         for (int k = lane; k < w * s.ty; k += 32) {
-            const float2 r = red[k / w * s.tx + lo + k % w];
+            const double2 r = red[k / w * s.tx + lo + k % w];
             a1 += r.x;
             a2 += r.y;
         }
@@ -282,18 +304,14 @@ __global__ void __launch_bounds__(kGnThreads) k_gn_sums(GnArgs a, GnSplit s, con
             a1 += __shfl_xor_sync(0xFFFFFFFFu, a1, m);
             a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
         }
-        if (lane == 0) {
-            const size_t slab = static_cast<size_t>(n) * a.groups + g0 + g;
-            part[slab * s.splits + blockIdx.x] = make_float2(a1, a2);
-            // (an output written in place has replaced the value itself by then)
-            if (blockIdx.x == 0) a.shift[slab] = to_f<T>(xn[g * a.width]);
-        }
+        if (lane == 0)
+            part[(static_cast<size_t>(n) * a.groups + g0 + g) * s.splits + blockIdx.x] = make_double2(a1, a2);
     }
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kGnThreads)
-k_gn_apply(GnArgs a, GnSplit s, const T* x, T* y, const float2* part) {
+__global__ void __launch_bounds__(kGnThreads, VEC * sizeof(T) < 16 ? 6 : VEC == 4 ? 5 : 4)
+k_gn_apply(GnArgs a, GnSplit s, const T* x, T* y, const double2* part) {
     extern __shared__ float2 stat[];               // (mean, 1 / deviation) of the CTA's groups
     const int n = blockIdx.z, g0 = blockIdx.y * s.gpc, ng = min(s.gpc, a.groups - g0);
     const int wv = a.width / VEC, cv = ng * wv;
@@ -303,11 +321,11 @@ k_gn_apply(GnArgs a, GnSplit s, const T* x, T* y, const float2* part) {
     const int ch0 = g0 * a.width;
     const T* xn = x + n * a.x_sample + ch0;
     asm volatile("griddepcontrol.wait;" ::: "memory");   // the sums of the kernel before
-    // one warp a slab joins the slices' sums, in 64 bits
+    // one warp a slab joins the slices' sums
     for (int g = threadIdx.x / 32; g < ng; g += kGnThreads / 32) {
         double a1 = 0.0, a2 = 0.0;
         for (int k = threadIdx.x % 32; k < s.splits; k += 32) {
-            const float2 r = part[(static_cast<size_t>(n) * a.groups + g0 + g) * s.splits + k];
+            const double2 r = part[(static_cast<size_t>(n) * a.groups + g0 + g) * s.splits + k];
             a1 += r.x;
             a2 += r.y;
         }
@@ -317,10 +335,8 @@ k_gn_apply(GnArgs a, GnSplit s, const T* x, T* y, const float2* part) {
             a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
         }
         if (threadIdx.x % 32 == 0) {
-            const double inv = a.inv;
-            const float shift = gn_shift(a.shift[static_cast<size_t>(n) * a.groups + g0 + g]);
-            const double m = a1 * inv, var = a2 * inv - m * m;   // a non-finite value: NaN
-            stat[g] = make_float2(static_cast<float>(shift + m), static_cast<float>(1.0 / sqrt((var < 0.0 ? 0.0 : var) + a.eps)));
+            const double m = a1 * a.inv, var = a2 * a.inv - m * m;   // a non-finite value: NaN
+            stat[g] = make_float2(static_cast<float>(m), static_cast<float>(1.0 / sqrt((var < 0.0 ? 0.0 : var) + a.eps)));
         }
     }
     __syncthreads();
@@ -348,7 +364,8 @@ k_gn_apply(GnArgs a, GnSplit s, const T* x, T* y, const float2* part) {
 // vectors, in its own places --, the CTAs read one another's sums through
 // distributed shared memory, and each writes its slice's outputs.
 constexpr int kGnClusterThreads = 1024;
-constexpr int kGnClusterBytes = 184 * 1024;    // of values; sums and the static part are below 36 KB more
+constexpr int kGnClusterBytes = 184 * 1024;    // of values
+constexpr int kGnClusterSmem = 227 * 1024 - kGnClusterThreads * static_cast<int>(sizeof(double2));   // and all but the static part
 
 struct GnCluster {
     int ctas, chunks, gpc, tx, ty, rounds;         // rounds: position steps of a thread
@@ -357,12 +374,11 @@ struct GnCluster {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCluster s, const T* x, T* y) {
     extern __shared__ __align__(16) uint8_t gn_smem[];
-    __shared__ float2 red[kGnClusterThreads];
+    __shared__ double2 red[kGnClusterThreads];
     Pack<T, VEC>* tile = reinterpret_cast<Pack<T, VEC>*>(gn_smem);
-    float2* sums = reinterpret_cast<float2*>(gn_smem + static_cast<size_t>(s.rounds) * kGnClusterThreads * sizeof(Pack<T, VEC>));
-    float2* stat = sums + s.gpc;
-    float2* part = stat + s.gpc;                   // max(32, gpc)
-    float* shifts = reinterpret_cast<float*>(part + max(32, s.gpc));
+    double2* sums = reinterpret_cast<double2*>(gn_smem + static_cast<size_t>(s.rounds) * kGnClusterThreads * sizeof(Pack<T, VEC>));
+    double2* part = sums + s.gpc;                  // max(32, gpc)
+    float2* stat = reinterpret_cast<float2*>(part + max(32, s.gpc));
     const int rank = blockIdx.x, n = blockIdx.z, g0 = blockIdx.y * s.gpc, ng = min(s.gpc, a.groups - g0);
     const int wv = a.width / VEC, cv = ng * wv;
     const int p0 = static_cast<int>(static_cast<long long>(a.positions) * rank / s.ctas);
@@ -372,17 +388,24 @@ __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCl
     const int g = on ? tx / wv : 0;
     const T* xn = x + n * a.x_sample + ch0;
     float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
-    const float shift = gn_shift(to_f<T>(xn[g * a.width]));
+    double2 m = make_double2(0.0, 0.0);
     float w[VEC], b[VEC];
     if (on) {
         const T* xp = xn + tx * VEC;
         constexpr int kBatch = 8;                  // loads in flight
+        float shift = 0.0f;
+        int count = 0;
         for (int r0 = 0; r0 < s.rounds; r0 += kBatch) {
             Pack<T, VEC> k[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
                 const int p = p0 + ty + (r0 + i) * s.ty;
                 if (p < p1) k[i] = *reinterpret_cast<const Pack<T, VEC>*>(xp + p * a.x_pos);
+            }
+            if (r0 == 0 && p0 + ty < p1) {
+                float v[VEC];
+                unpack_vec<T, VEC>(k[0], v);
+                shift = add_up<VEC>(v) * (1.0f / VEC);
             }
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
@@ -391,26 +414,27 @@ __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCl
                 float v[VEC];
                 unpack_vec<T, VEC>(k[i], v);
                 moments<VEC>(v, shift, s1, s2);
+                count += VEC;
             }
         }
+        fold(m, count, shift, s1, s2);
     }
     if (on) {
         channel_params<VEC>(a.weight, ch0 + tx * VEC, 1.0f, VEC >= 4 && a.wide, w);
         channel_params<VEC>(a.bias, ch0 + tx * VEC, 0.0f, VEC >= 4 && a.wide, b);
-        if (ty == 0 && tx == g * wv) shifts[g] = shift;
     }
-    red[tid] = make_float2(s1.x + s1.y, s2.x + s2.y);
+    red[tid] = m;
     __syncthreads();
     const int warp = tid / 32, lane = tid % 32;
     // group i's threads in `slices` parts, a warp each, then the parts
     const int slices = max(1, kGnClusterThreads / 32 / ng);
     for (int u = warp; u < ng * slices; u += kGnClusterThreads / 32) {
         const int i = u % ng, sl = u / ng;
-        float a1 = 0.0f, a2 = 0.0f;
+        double a1 = 0.0, a2 = 0.0;
         const int t0 = wv < 32 ? lane + 32 * sl : sl, dt = wv < 32 ? 32 * slices : slices, q0 = wv < 32 ? 0 : lane, dq = wv < 32 ? 1 : 32;
         for (int t = t0; t < s.ty; t += dt)
             for (int q = q0; q < wv; q += dq) {
-                const float2 r = red[t * s.tx + i * wv + q];
+                const double2 r = red[t * s.tx + i * wv + q];
                 a1 += r.x;
                 a2 += r.y;
             }
@@ -419,11 +443,11 @@ __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCl
             a1 += __shfl_xor_sync(0xFFFFFFFFu, a1, m);
             a2 += __shfl_xor_sync(0xFFFFFFFFu, a2, m);
         }
-        if (lane == 0) part[u] = make_float2(a1, a2);
+        if (lane == 0) part[u] = make_double2(a1, a2);
     }
     __syncthreads();
     for (int i = tid; i < ng; i += kGnClusterThreads) {
-        float2 r = part[i];
+        double2 r = part[i];
         for (int sl = 1; sl < slices; ++sl) {
             r.x += part[i + sl * ng].x;
             r.y += part[i + sl * ng].y;
@@ -432,14 +456,13 @@ __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCl
     }
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     for (int i = warp; i < ng; i += kGnClusterThreads / 32) {   // lane c: CTA c's sums
-        float u = 0.0f, v = 0.0f;
+        double a1 = 0.0, a2 = 0.0;
         if (lane < s.ctas) {
             uint32_t there;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
                          : "=r"(there) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(sums + i))), "r"(lane));
-            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(u), "=f"(v) : "r"(there) : "memory");
+            asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];" : "=d"(a1), "=d"(a2) : "r"(there) : "memory");
         }
-        double a1 = u, a2 = v;
 #pragma unroll
         for (int m = 4; m; m >>= 1) {
             a1 += __shfl_xor_sync(0xFFFFFFFFu, a1, m);
@@ -447,7 +470,7 @@ __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCl
         }
         if (lane == 0) {
             const double m = a1 * a.inv, var = a2 * a.inv - m * m;   // a non-finite value: NaN
-            stat[i] = make_float2(static_cast<float>(shifts[i] + m), 1.0f / sqrtf(static_cast<float>((var < 0.0 ? 0.0 : var) + a.eps)));
+            stat[i] = make_float2(static_cast<float>(m), 1.0f / sqrtf(static_cast<float>((var < 0.0 ? 0.0 : var) + a.eps)));
         }
     }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this CTA has read its peers' sums
@@ -531,7 +554,8 @@ bool gn_small(const SslaGroupNorm* a, int vec, int* lps, int* ept) {
 }
 
 size_t gn_cluster_bytes(const GnCluster& c, int vec, int sz) {
-    return static_cast<size_t>(c.rounds) * kGnClusterThreads * vec * sz + (c.gpc * 5 + 2 * std::max(32, c.gpc)) * sizeof(float);
+    return static_cast<size_t>(c.rounds) * kGnClusterThreads * vec * sz + c.gpc * (sizeof(double2) + sizeof(float2)) +
+           std::max(32, c.gpc) * sizeof(double2);
 }
 
 // The smallest cluster, of whole groups of at least 64 contiguous bytes,
@@ -556,6 +580,7 @@ bool gn_cluster(const SslaGroupNorm* a, int vec, GnCluster* c) {
             k.ty = kGnClusterThreads / k.tx;
             k.rounds = ((a->positions + ctas - 1) / ctas + k.ty - 1) / k.ty;
             if (k.rounds > kGnClusterBytes / (kGnClusterThreads * vec * sz)) continue;
+            if (gn_cluster_bytes(k, vec, sz) > kGnClusterSmem) continue;
             found = true;
             *c = k;
             if (static_cast<long long>(a->n) * k.chunks * ctas >= 128 || k.rounds <= 2) return true;
@@ -591,7 +616,7 @@ size_t gn_bytes(const SslaGroupNorm* a) {
         return std::max(whole, gn_bytes(&part));
     }
     if (gn_cluster(a, vec, &c)) return 0;
-    return static_cast<size_t>(a->n) * a->groups * (gn_split(a, vec).splits * sizeof(float2) + sizeof(float));
+    return static_cast<size_t>(a->n) * a->groups * gn_split(a, vec).splits * sizeof(double2);
 }
 
 }  // namespace
@@ -639,7 +664,6 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
     d.act = a->activation; d.eps = a->eps;
     d.inv = 1.0 / (static_cast<double>(a->positions) * d.width);
     d.wide = aligned(a->weight, 16) && aligned(a->bias, 16);
-    d.shift = nullptr;
     d.stream = 2LL * a->n * a->positions * a->channels * dtype_size(a->dtype) > kStreamBytes;
     const int vec = gn_vec(a);
     auto run = [&](auto t, auto v) {
@@ -674,7 +698,7 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
         GnCluster c;
         if (gn_cluster(a, vec, &c)) {
             const size_t bytes = gn_cluster_bytes(c, V, sizeof(T));
-            allow_smem<k_gn_cluster<T, V>>(kGnClusterBytes + 7 * kGnClusterThreads * static_cast<int>(sizeof(float)));
+            allow_smem<k_gn_cluster<T, V>>(kGnClusterSmem);
             cudaLaunchConfig_t cfg = {};
             cudaLaunchAttribute at;
             at.id = cudaLaunchAttributeClusterDimension;
@@ -691,8 +715,7 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
         }
         const GnSplit s = gn_split(a, vec);
         if (s.chunks > 65535) return fail(SSLA_ERR_ARG, "group norm: more than 65535 group chunks of large slabs");
-        float2* part = static_cast<float2*>(workspace);
-        d.shift = reinterpret_cast<float*>(part + static_cast<size_t>(slabs) * s.splits);
+        double2* part = static_cast<double2*>(workspace);
         const dim3 grid(s.splits, s.chunks, a->n);
         k_gn_sums<T, V><<<grid, kGnThreads, 0, st>>>(d, s, x, part);
         // the second launch's latency passes under the first kernel
@@ -706,7 +729,7 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
         cfg.stream = st;
         cfg.attrs = &at;
         cfg.numAttrs = 1;
-        cudaLaunchKernelEx(&cfg, k_gn_apply<T, V>, d, s, x, y, static_cast<const float2*>(part));
+        cudaLaunchKernelEx(&cfg, k_gn_apply<T, V>, d, s, x, y, static_cast<const double2*>(part));
         return launched("group norm");
     };
     auto by_vec = [&](auto t) {
