@@ -25,6 +25,7 @@
 #include <climits>
 #include <cmath>
 #include <numeric>
+#include <type_traits>
 
 #include "ssla_ops.cuh"
 
@@ -81,24 +82,58 @@ __device__ __forceinline__ void fold(double2& m, int n, float shift, float2 s1, 
     m.y += (static_cast<double>(s2.x) + s2.y) + shift * (2.0 * d + ns);
 }
 
-// y / (1 + e^-y) with the hardware's exponential and reciprocal: relative
-// errors of 2^-22 each and |y| 2^-24 from rounding the exponent, which is
-// below 2^-20 where the value counts and below half a step of 16-bit outputs
-// everywhere.  Where e^-y overflows the limit is -0.
-__device__ __forceinline__ float sigmoid_of(float neg_y_log2e) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(neg_y_log2e));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+// SiLU, y / (1 + e^-y), with the hardware's exponential and reciprocal:
+// relative errors of 2^-22 each and |y| 2^-23 from rounding the exponent,
+// which is below 2^-20 where the value counts and below half a step of 16-bit
+// outputs everywhere.  For y < -87 the reciprocal itself is below the normal
+// numbers, while y e^y, which is what is left of SiLU, is one down to -91.9.
+__device__ __forceinline__ float exp2_hw(float x) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+    return e;
+}
+__device__ __forceinline__ float rcp_hw(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+constexpr float kNegLog2e = -1.44269504f, kSiluTail = 125.0f;   // the exponent from where 32-bit results go by halves
+template <typename T, int VEC> __device__ __forceinline__ void silu(float (&x)[VEC]) {
+    constexpr int N = (VEC + 1) / 2;
+    float2 y[N];
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        y[j] = make_float2(x[2 * j], 2 * j + 1 < VEC ? x[2 * j + 1] : 0.0f);
+        float2 o;
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            // the quotient times 2^32, so that it stays normal as far as bf16 goes (the sum rounds the exponent to 2^-19)
+            const float2 t = __ffma2_rn(y[j], make_float2(kNegLog2e, kNegLog2e), make_float2(-32.0f, -32.0f));
+            o = __fmul2_rn(__fmul2_rn(y[j], make_float2(0x1p-32f, 0x1p-32f)),
+                           make_float2(rcp_hw(0x1p-32f + exp2_hw(t.x)), rcp_hw(0x1p-32f + exp2_hw(t.y))));
+        } else {                                   // (fp16 ends above all this)
+            const float2 t = __fmul2_rn(y[j], make_float2(kNegLog2e, kNegLog2e));
+            o = __fmul2_rn(y[j], make_float2(rcp_hw(1.0f + exp2_hw(t.x)), rcp_hw(1.0f + exp2_hw(t.y))));
+            if (sizeof(T) == 4) most = fmaxf(most, fmaxf(t.x, t.y));
+        }
+        x[2 * j] = o.x;
+        if (2 * j + 1 < VEC) x[2 * j + 1] = o.y;
+    }
+    if (sizeof(T) == 4 && most > kSiluTail)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float v = j % 2 ? y[j / 2].y : y[j / 2].x, t = v * kNegLog2e, h = exp2_hw(-0.5f * t);
+            if (t > kSiluTail) x[j] = (v * h) * h;
+        }
 }
 
 // x <- act((x - mean) * rstd * w + b)
-template <int VEC>
+template <typename T, int VEC>
 __device__ __forceinline__ void gn_finish(float (&x)[VEC], float mean, float rstd, const float (&w)[VEC], const float (&b)[VEC],
                                           int act) {
     if constexpr (VEC == 1) {
         x[0] = fmaf((x[0] - mean) * rstd, w[0], b[0]);
-        if (act == SSLA_ACT_SILU) x[0] *= sigmoid_of(x[0] * -1.44269504f);
+        if (act == SSLA_ACT_SILU) silu<T, 1>(x);
     } else {
         const float2 m = make_float2(-mean, -mean), r = make_float2(rstd, rstd);
 #pragma unroll
@@ -108,16 +143,7 @@ __device__ __forceinline__ void gn_finish(float (&x)[VEC], float mean, float rst
             x[j] = y.x;
             x[j + 1] = y.y;
         }
-        if (act == SSLA_ACT_SILU) {
-#pragma unroll
-            for (int j = 0; j < VEC; j += 2) {
-                const float2 y = make_float2(x[j], x[j + 1]);
-                const float2 t = __fmul2_rn(y, make_float2(-1.44269504f, -1.44269504f));
-                const float2 o = __fmul2_rn(y, make_float2(sigmoid_of(t.x), sigmoid_of(t.y)));
-                x[j] = o.x;
-                x[j + 1] = o.y;
-            }
-        }
+        if (act == SSLA_ACT_SILU) silu<T, VEC>(x);
     }
 }
 
@@ -243,7 +269,7 @@ __global__ void __launch_bounds__(kGnThreads, LPS <= 32 && EPT <= 2 ? kGnSlabCta
                 const int k = e * LPS + lane;
                 if (k < vecs) {
                     const int p = a.positions == 1 ? 0 : k / wv, c = (k - p * wv) * VEC;
-                    gn_finish<VEC>(v[u][e], mean[u], rstd[u], w[e], b[e], a.act);
+                    gn_finish<T, VEC>(v[u][e], mean[u], rstd[u], w[e], b[e], a.act);
                     store_vec_hint<T, VEC>(yp + p * a.y_pos + c, v[u][e], a.stream);
                 }
             }
@@ -352,7 +378,7 @@ k_gn_apply(GnArgs a, GnSplit s, const T* x, T* y, const double2* part) {
         for (int p = p0 + ty; p < p1; p += s.ty) {
             float v[VEC];
             load_vec<T, VEC>(xp + p * a.x_pos, v);
-            gn_finish<VEC>(v, st.x, st.y, w, b, a.act);
+            gn_finish<T, VEC>(v, st.x, st.y, w, b, a.act);
             store_vec<T, VEC>(yp + p * a.y_pos, v);
         }
     }
@@ -484,7 +510,7 @@ __global__ void __launch_bounds__(kGnClusterThreads) k_gn_cluster(GnArgs a, GnCl
             if (p >= p1) break;
             float v[VEC];
             unpack_vec<T, VEC>(tile[r * kGnClusterThreads + tid], v);
-            gn_finish<VEC>(v, st.x, st.y, w, b, a.act);
+            gn_finish<T, VEC>(v, st.x, st.y, w, b, a.act);
             store_vec<T, VEC>(yp + p * a.y_pos, v);
         }
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // no CTA leaves while a peer may read it
