@@ -246,7 +246,8 @@ __device__ __forceinline__ DecaySums chunk_decays(float2 g, int lane) {
         if (lane >= m) run += o;
     }
     d.total = __shfl_sync(0xFFFFFFFFu, run, 31);
-    const double before = run - s[1];
+    double before = __shfl_up_sync(0xFFFFFFFFu, run, 1);    // (not run - s[1]: a NaN there is this lane's second token's)
+    if (lane == 0) before = 0.0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const double G = j ? run : before + s[0];
