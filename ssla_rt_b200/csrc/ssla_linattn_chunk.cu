@@ -113,9 +113,17 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 __device__ __forceinline__ float2 unpack2(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
 }
+// The first of several pieces: 32-bit values above bf16's largest give that,
+// not infinity, and leave the rest to the next piece; so do infinities, whose
+// next piece is one.
+__device__ __forceinline__ uint32_t pack2_finite(float x, float y) {
+    uint32_t p;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(y), "f"(x));
+    return p;
+}
 // The next piece of (x, y); what is left stays in them.
-__device__ __forceinline__ uint32_t take(float& x, float& y) {
-    const uint32_t p = pack2(x, y);
+template <bool FIRST = false> __device__ __forceinline__ uint32_t take(float& x, float& y) {
+    const uint32_t p = FIRST ? pack2_finite(x, y) : pack2(x, y);
     const float2 f = unpack2(p);
     x -= f.x;
     y -= f.y;
@@ -182,8 +190,13 @@ template <int D> struct Moving {
 #pragma unroll
             for (int n = 0; n < IN; ++n) {
                 uint4 u;
-                u.x = take(x[i][0], x[i][1]); u.y = take(x[i][2], x[i][3]);
-                u.z = take(x[i][4], x[i][5]); u.w = take(x[i][6], x[i][7]);
+                if (IN == 3 && n == 0) {           // (16-bit inputs are not above bf16's largest)
+                    u.x = take<true>(x[i][0], x[i][1]); u.y = take<true>(x[i][2], x[i][3]);
+                    u.z = take<true>(x[i][4], x[i][5]); u.w = take<true>(x[i][6], x[i][7]);
+                } else {
+                    u.x = take(x[i][0], x[i][1]); u.y = take(x[i][2], x[i][3]);
+                    u.z = take(x[i][4], x[i][5]); u.w = take(x[i][6], x[i][7]);
+                }
                 *reinterpret_cast<uint4*>(s + n * kChunk * LD + r * LD + c) = u;
             }
         }
@@ -362,8 +375,8 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
                     __nv_bfloat16* p = sS + (m0 + i * 16 + g8) * LV + n0 + j * 8 + t2;
 #pragma unroll
                     for (int m = 0; m < MID; ++m) {
-                        *reinterpret_cast<uint32_t*>(p + m * DK * LV) = take(x0, x1);
-                        *reinterpret_cast<uint32_t*>(p + m * DK * LV + 8 * LV) = take(y0, y1);
+                        *reinterpret_cast<uint32_t*>(p + m * DK * LV) = m ? take(x0, x1) : take<true>(x0, x1);
+                        *reinterpret_cast<uint32_t*>(p + m * DK * LV + 8 * LV) = m ? take(y0, y1) : take<true>(y0, y1);
                     }
                 }
         }
@@ -437,10 +450,10 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
                     uint32_t pa[MID][4];
 #pragma unroll
                     for (int i = 0; i < MID; ++i) {
-                        pa[i][0] = take(P[0][0], P[0][1]);
-                        pa[i][1] = take(P[0][2], P[0][3]);
-                        pa[i][2] = take(P[1][0], P[1][1]);
-                        pa[i][3] = take(P[1][2], P[1][3]);
+                        pa[i][0] = i ? take(P[0][0], P[0][1]) : take<true>(P[0][0], P[0][1]);
+                        pa[i][1] = i ? take(P[0][2], P[0][3]) : take<true>(P[0][2], P[0][3]);
+                        pa[i][2] = i ? take(P[1][0], P[1][1]) : take<true>(P[1][0], P[1][1]);
+                        pa[i][3] = i ? take(P[1][2], P[1][3]) : take<true>(P[1][2], P[1][3]);
                     }
 #pragma unroll
                     for (int m = 0; m < NT / 2; ++m) {
@@ -486,7 +499,7 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
                 const int kr = ks + lane % 8 + lane / 16 * 8, kc = m0 + i * 16 + lane / 8 % 2 * 8;
                 float2 f[4] = {};
 #pragma unroll
-                for (int m = 0; m < IN; ++m) {
+                for (int m = IN - 1; m >= 0; --m) {         // the smallest first: the larger two may add up to above the largest float
                     uint32_t r[4];
                     ldsm4t(r, sK + m * kChunk * LK + kr * LK + kc);
 #pragma unroll
@@ -503,7 +516,7 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
 #pragma unroll
                 for (int m = 0; m < 3; ++m)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) ka[m][e] = take(f[e].x, f[e].y);
+                    for (int e = 0; e < 4; ++e) ka[m][e] = m ? take(f[e].x, f[e].y) : take<true>(f[e].x, f[e].y);
 #pragma unroll
                 for (int p = 0; p < SN / 2; ++p) {
                     uint32_t b[IN][4];

@@ -215,8 +215,8 @@ __device__ __forceinline__ uint32_t piece_at(int r, int ch) {
     return static_cast<uint32_t>(ch / 8 * kBlk + r * kSwRow + ((ch % 8 ^ r % 8) << 4));
 }
 // The next bf16 piece of a pair, packed; what is left stays in it.
-__device__ __forceinline__ uint32_t take2(float2& x) {
-    const uint32_t p = pack2(x.x, x.y);
+template <bool FIRST = false> __device__ __forceinline__ uint32_t take2(float2& x) {
+    const uint32_t p = FIRST ? pack2_finite(x.x, x.y) : pack2(x.x, x.y);
     x = __ffma2_rn(unpack2(p), make_float2(-1.0f, -1.0f), x);
     return p;
 }
@@ -428,9 +428,9 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         uint8_t* const to = j ? to1 : to0;
-                        *reinterpret_cast<uint32_t*>(to) = take2(x[j]);
+                        *reinterpret_cast<uint32_t*>(to) = take2<true>(x[j]);
                         *reinterpret_cast<uint32_t*>(to + kBlk) = pack2(x[j].x, x[j].y);
-                        *reinterpret_cast<uint32_t*>(to + 8 * kSwRow) = take2(y[j]);
+                        *reinterpret_cast<uint32_t*>(to + 8 * kSwRow) = take2<true>(y[j]);
                         *reinterpret_cast<uint32_t*>(to + 8 * kSwRow + kBlk) = pack2(y[j].x, y[j].y);
                     }
                     ld_wait(ahead);
@@ -469,7 +469,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     float2 x = S[b * 8 + i];
-                    big[i] = take2(x);
+                    big[i] = take2<true>(x);
                     small[i] = pack2(x.x, x.y);
                 }
                 tmem_st8(tm + lanes + L::kS + k0 / 2 + b * 8, big);
