@@ -245,8 +245,9 @@ LinArgs device_args(const SslaLinAttn* a) {
 
 bool state_vec4(const SslaLinAttn* a) { return a->dv % 4 == 0 && aligned(a->state, 16); }
 
-// The sequences of a chunked call, checked against each other and the rows.
-int check_seqs(const SslaLinAttn* a, const int* offsets, const int* lengths, const int* slots, int n_seq,
+// The sequences of a chunked call, checked against each other and the rows,
+// and, with `slotted`, their slots.
+int check_seqs(const SslaLinAttn* a, const int* offsets, const int* lengths, bool slotted, const int* slots, int n_seq,
                std::vector<Seq>& out) {
     const char* who = "linear attention";
     if (n_seq < 0 || (n_seq > 0 && !offsets)) return fail(SSLA_ERR_ARG, "%s: no offsets", who);
@@ -257,7 +258,7 @@ int check_seqs(const SslaLinAttn* a, const int* offsets, const int* lengths, con
         if (offsets[i] < 0 || len < 0 || offsets[i] + len > a->n_rows)
             return fail(SSLA_ERR_ARG, "%s: sequence %d is rows [%d, %lld) of %d", who, i, offsets[i], offsets[i] + len,
                         a->n_rows);
-        const int slot = slots ? slots[i] : i;
+        const int slot = !slotted ? -1 : slots ? slots[i] : i;
         if (slot < -1 || slot >= a->n_slots) {
             if (a->state || slots) return fail(SSLA_ERR_ARG, "%s: slot %d of %d", who, slot, a->n_slots);
         }
@@ -317,7 +318,7 @@ int ssla_linattn_chunk_workspace(const SslaLinAttn* a, const int* offsets, const
     if (const int rc = check_args(a, "linear attention", false); rc != SSLA_OK) return rc;
     try {
         std::vector<Seq> seqs;
-        if (const int rc = check_seqs(a, offsets, lengths, nullptr, n_seq, seqs); rc != SSLA_OK) return rc;
+        if (const int rc = check_seqs(a, offsets, lengths, false, nullptr, n_seq, seqs); rc != SSLA_OK) return rc;
         *bytes = a->n_rows ? chunk_workspace(device_args(a), a->dtype, seqs) : 0;
         return SSLA_OK;
     } catch (const std::exception&) {
@@ -331,7 +332,7 @@ int ssla_linattn_chunk(const SslaLinAttn* a, const int* offsets, const int* leng
     if (const int rc = check_args(a, who, false); rc != SSLA_OK) return rc;
     try {
         std::vector<Seq> seqs;
-        if (const int rc = check_seqs(a, offsets, lengths, slots, n_seq, seqs); rc != SSLA_OK) return rc;
+        if (const int rc = check_seqs(a, offsets, lengths, true, slots, n_seq, seqs); rc != SSLA_OK) return rc;
         if (a->n_rows == 0 || seqs.empty()) return SSLA_OK;
         const LinArgs d = device_args(a);
         const size_t need = chunk_workspace(d, a->dtype, seqs);
