@@ -633,7 +633,8 @@ Shape shape_of(const LinArgs& a, int dtype) {
 
 // Tokens of a segment for sequences [i0, i1).  Undivided, the longest sequence
 // bounds the time; divided, all resident CTAs share the work, but keys and
-// values pass twice (`cost`) and a last round of CTAs is half empty.
+// values pass twice (`cost`) and a last round of CTAs is half empty.  A group's
+// segments are a grid's depth: at most 65535.
 int segment_tokens(const LinArgs& a, const Shape& sh, const std::vector<Seq>& seqs, size_t i0, size_t i1) {
     const long long per = static_cast<long long>(a.heads) * ((a.dv + sh.dv - 1) / sh.dv), slots = 148LL * sh.ctas;
     long long longest = 0, all = 0;
@@ -647,9 +648,10 @@ int segment_tokens(const LinArgs& a, const Shape& sh, const std::vector<Seq>& se
     for (int parts = 2; parts <= 512; parts += parts < 32 ? 1 : parts / 16) {
         const long long step = (longest + parts - 1) / parts;
         if (step < 4) break;
-        long long ctas = 0;
-        for (size_t i = i0; i < i1; ++i) ctas += ((seqs[i].len + kChunk - 1LL) / kChunk + step - 1) / step * per;
-        const long long time = (std::max(step, share) + (ctas > slots ? step / 2 : 0)) * sh.cost;
+        long long segs = 0;
+        for (size_t i = i0; i < i1; ++i) segs += ((seqs[i].len + kChunk - 1LL) / kChunk + step - 1) / step;
+        if (segs > 65535) break;                            // (the steps only get smaller)
+        const long long ctas = segs * per, time = (std::max(step, share) + (ctas > slots ? step / 2 : 0)) * sh.cost;
         if (time < best_time) best = step, best_time = time;
     }
     return static_cast<int>(best == longest ? INT_MAX / 2 / kChunk * kChunk : best * kChunk);
@@ -657,7 +659,7 @@ int segment_tokens(const LinArgs& a, const Shape& sh, const std::vector<Seq>& se
 
 int segments(const Seq& s, int tokens) { return s.len ? (s.len - 1) / tokens + 1 : 0; }
 
-// Ends of the launch groups: at most kTable sequences and 65535 segments.
+// Ends of the launch groups: at most kTable sequences (and 65535 segments, segment_tokens).
 size_t group_end(const std::vector<Seq>& seqs, size_t i0) { return std::min(seqs.size(), i0 + kTable); }
 
 }  // namespace
