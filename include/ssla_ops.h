@@ -33,7 +33,9 @@ enum { SSLA_LINATTN_MAX_DK = 128, SSLA_LINATTN_MAX_DV = 256 };
  * [n_rows][heads][dv]; the last index is contiguous, row and head strides are
  * in elements.  Head h reads query head h / (heads / q_heads), keys alike.
  * decay: logarithms, at most 0, strides decay_row and decay_head (decay_row 0:
- * one decay per head); -infinity clears the state before the token.
+ * one decay per head); -infinity clears the state before the token, NaN and
+ * infinities in it too (where there are any, the chunked form goes through
+ * that part of the sequence token by token: 0.7 to 3.5 us a token).
  * state: [n_slots][heads][dk][dv], contiguous, updated in place.  `out` and
  * `state` overlap neither each other nor an input (the address ranges are
  * compared). */

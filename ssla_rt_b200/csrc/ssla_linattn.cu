@@ -75,6 +75,11 @@ struct StepTile {
     // The fetched token: updates the state, and leaves its output's parts in o.
     __device__ void apply(const LinArgs& a, float (&o)[VEC]) {
         const float e = expf(g);
+        if (g == -INFINITY)                        // clears the state, NaN and infinities in it too
+#pragma unroll
+            for (int i = 0; i < RPT; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) s[i][j] = 0.0f;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) o[j] = 0.0f;
 #pragma unroll

@@ -33,6 +33,15 @@
 // before s, but 0 * inf in a masked place would take it there.  Masked scores
 // are replaced, not multiplied, and a non-finite v is taken out of the tile
 // and put back as NaN into its column from its own token on.
+//
+// Clears.  A decay of -infinity replaces the state by zero, whatever it holds.
+// As a decay of -1e5 it takes every finite value before it to zero in the
+// products above; 0 * infinity would stay, in the state too.  So a CTA that
+// ends with a state that is not finite looks for a clear among its decays, and
+// where there is one goes through its tokens again, one by one (walk): 0.7 us a
+// token, 3.5 us in the tcgen05 form.  The others pay 1 to 3 % for the question.
+// Masks for the tokens from one clear to the next, in the products themselves,
+// cost every call 2 to 20 %.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -273,6 +282,90 @@ __device__ __forceinline__ DecaySums chunk_decays(float2 g, int lane) {
     return d;
 }
 
+// The recurrence itself, over rows [row0, row0 + count) of head h, by
+// THREADS = COLS * PARTS threads (`tid`, which meet at sync()): thread (col,
+// part) has state rows [part * N, part * N + N) of value column c0 + col, from
+// `from` (null: zero) to `to` (null: nowhere).  mem: walk_floats of shared
+// memory.  A token's keys and queries pass through it, the next token's in
+// flight; with SHARED the state is there as well (where registers are short).
+// Returns the sum of the log2 decays, -infinity with a clear.
+template <int DK, int COLS, int PARTS, bool SHARED> constexpr int walk_floats = 4 * DK + 2 * COLS * PARTS + (SHARED ? DK * COLS : 0);
+template <typename T, int DK, int COLS, int PARTS, bool OUT, bool SHARED, typename Sync>
+__device__ __forceinline__ double walk(const LinArgs& a, int h, long long row0, int count, int c0, int tid, const float* from, float* to, float* mem,
+                                       Sync sync) {
+    constexpr int N = DK / PARTS, THREADS = COLS * PARTS, MOVES = (2 * DK + THREADS - 1) / THREADS;
+    const int col = c0 + tid % COLS, part = tid / COLS, k0 = part * N;
+    const bool live = col < a.dv;
+    const int rows = live ? min(N, a.dk - k0) : 0;
+    const T* q = static_cast<const T*>(a.q) + (h / a.q_share) * a.q_head + row0 * a.q_row;
+    const T* k = static_cast<const T*>(a.k) + (h / a.k_share) * a.k_head + row0 * a.k_row;
+    const T* v = static_cast<const T*>(a.v) + h * a.v_head + row0 * a.v_row + col;
+    const float* decay = a.decay + h * a.decay_head + row0 * a.decay_row;
+    T* out = static_cast<T*>(a.out) + h * a.out_head + row0 * a.out_row + col;
+    float kept[SHARED ? 1 : N], move[MOVES], g = 0.0f, x = 0.0f;
+    auto S = [&](int i) -> float& {
+        if constexpr (SHARED) return mem[4 * DK + 2 * THREADS + i * THREADS + tid];
+        else return kept[i];
+    };
+    constexpr int UNROLL = SHARED ? 8 : N;
+#pragma unroll UNROLL
+    for (int i = 0; i < N; ++i) S(i) = from && i < rows ? from[static_cast<size_t>(k0 + i) * a.dv + col] : 0.0f;
+    auto ask = [&](int t) {
+        g = decay[t * a.decay_row];
+        x = live ? to_f<T>(v[t * a.v_row]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < MOVES; ++i) {
+            const int e = tid + i * THREADS, c = e % DK;
+            move[i] = e >= 2 * DK || c >= a.dk ? 0.0f : to_f<T>(e < DK ? k[t * a.k_row + c] : q[t * a.q_row + c]);
+        }
+    };
+    ask(0);
+    double total = 0.0;
+#pragma unroll 1
+    for (int t = 0; t < count; ++t) {
+        float* const kq = mem + t % 2 * 2 * DK;
+        float* const parts = mem + 4 * DK + t % 2 * THREADS;
+#pragma unroll
+        for (int i = 0; i < MOVES; ++i)
+            if (tid + i * THREADS < 2 * DK) kq[tid + i * THREADS] = move[i];
+        const float e = expf(g), vt = x;
+        total = g == -INFINITY ? -INFINITY : total + g * 1.4426950408889634;
+        if (g == -INFINITY)
+#pragma unroll UNROLL
+            for (int i = 0; i < N; ++i) S(i) = 0.0f;
+        sync();
+        if (t + 1 < count) ask(t + 1);
+        float sums[4] = {};
+#pragma unroll UNROLL
+        for (int i = 0; i < N; ++i) {
+            const float s = fmaf(kq[k0 + i], vt, e * S(i));
+            S(i) = i < rows ? s : 0.0f;                     // (0 * NaN from dk on)
+            sums[i % 4] = fmaf(kq[DK + k0 + i], i < rows ? s : 0.0f, sums[i % 4]);
+        }
+        if (OUT) {
+            float o = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            parts[tid] = o;
+            sync();
+            if (part == 0 && live) {
+#pragma unroll
+                for (int i = 1; i < PARTS; ++i) o += parts[tid + i * COLS];
+                out[t * a.out_row] = from_f<T>(o * a.scale);
+            }
+        }
+    }
+    if (to)
+#pragma unroll UNROLL
+        for (int i = 0; i < N; ++i)
+            if (i < rows) to[static_cast<size_t>(k0 + i) * a.dv + col] = S(i);
+    return total;
+}
+// Whether one of the threads' decays (thread t of `threads`) is a clear.
+__device__ __forceinline__ bool some_clear(const LinArgs& a, int h, long long row0, int count, int t, int threads) {
+    bool found = false;
+    for (; t < count; t += threads) found |= a.decay[(row0 + t) * a.decay_row + h * a.decay_head] == -INFINITY;
+    return found;
+}
+
 // Segment states: [segment][head][dk][dv]; segment decays: [segment][head].
 // Where a divided sequence's segment finds its first state: the place of the
 // segment before it, the first one that of the last (which leaves none), since
@@ -329,6 +422,7 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
         }
     bool zero = from == nullptr;                           // S is zero: no product with it
     double total = 0.0;
+    bool cleared = false;                                  // (this lane's tokens)
 
     const int row0 = tab.start[seq];
     const T* Q = static_cast<const T*>(a.q) + (h / a.q_share) * a.q_head;
@@ -381,7 +475,9 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
                 }
         }
         if (warp == 0) {
-            const DecaySums d = chunk_decays(chunk_decay_values(a, row, n, h, lane), lane);
+            const float2 g = chunk_decay_values(a, row, n, h, lane);
+            const DecaySums d = chunk_decays(g, lane);
+            if (!OUT) cleared |= g.x == -INFINITY || g.y == -INFINITY;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int t = 2 * lane + j;
@@ -546,6 +642,22 @@ k_chunk(LinArgs a, const __grid_constant__ Table tab, float* seg_state, double* 
     if (!OUT) to = seg_state + (static_cast<size_t>(blockIdx.z) * a.heads + h) * head_state;
     else if (seg == nseg - 1 && slot >= 0 && last > first)
         to = a.state + (static_cast<size_t>(slot) * a.heads + h) * head_state;
+    if (!OUT && warp == 0 && __any_sync(0xFFFFFFFFu, cleared)) total = -INFINITY;
+    float nought[4] = {};                                  // NaN where one is not finite
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < SN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) nought[e] = fmaf(S[i][j][e], 0.0f, nought[e]);
+    const bool fine = (nought[0] + nought[1]) + (nought[2] + nought[3]) == 0.0f;
+    const long long row1 = static_cast<long long>(row0) + first;
+    if (__syncthreads_or(!fine) && __syncthreads_or(some_clear(a, h, row1, last - first, tid, kThreads))) {
+        static_assert(walk_floats<DK, DV, kThreads / DV, false> * 4 <= L::bytes, "shared memory");
+        total = walk<T, DK, DV, kThreads / DV, OUT, false>(a, h, row1, last - first, c0, tid, from, to, reinterpret_cast<float*>(smem),
+                                                    [] { __syncthreads(); });
+        to = nullptr;
+    }
     if (to)
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -579,12 +691,13 @@ k_chunk_join(LinArgs a, const __grid_constant__ Table tab, float* seg_state, con
         for (int i = 0; i < 8; ++i)
             if (s + i < s1) {
                 x[i] = seg_state[(static_cast<size_t>(s + i) * a.heads + h) * head_state + e];
-                g[i] = exp2f(static_cast<float>(seg_decay[static_cast<size_t>(s + i) * a.heads + h]));
+                const double d = seg_decay[static_cast<size_t>(s + i) * a.heads + h];
+                g[i] = d == -INFINITY ? -1.0f : exp2f(static_cast<float>(d));   // negative: a clear
             }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (s + i < s1) {
-                run = fmaf(g[i], run, x[i]);
+                run = g[i] < 0.0f ? x[i] : fmaf(g[i], run, x[i]);
                 seg_state[(static_cast<size_t>(s + i) * a.heads + h) * head_state + e] = run;
             }
     }

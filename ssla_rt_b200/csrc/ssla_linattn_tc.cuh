@@ -80,6 +80,7 @@ struct Side {                                     // what the roles share beside
     // next phase by itself (a stage comes again only after everyone has left
     // it); the others' next phase needs every waiter's own arrival first.
     uint64_t full[kStages], empty[kStages], checked[kStages], p_full[kStages], wk_full[kStages];
+    int again;                                    // bits: the state is not finite; there is a clear
     uint64_t sc_full, sc_free, o_full, o_free, wk_free[2], u_full, u_free, s_full, qs_full;
     uint32_t tmem;
     int abort;
@@ -292,9 +293,36 @@ __device__ __forceinline__ void stmatrix4_trans(uint32_t addr, const uint32_t (&
 // Piece `ch` (16 bytes) of row t of an output warp's [64][32] tile, 64-byte swizzle.
 __device__ __forceinline__ uint32_t out_piece(int t, int ch) { return static_cast<uint32_t>(t * 64 + ((ch ^ (t >> 1 & 3)) << 4)); }
 
+// Apart, like what follows: in place it cost every call 1 %.
+__device__ __noinline__ void chunk_scan(const LinArgs& a, int h, long long row0, int count, int* again) {
+    if (some_clear(a, h, row0, count, threadIdx.x - 128, 256)) atomicOr(again, 2);
+}
+// The CTA's tokens again, one by one, by warps 4 to 11.  (Everything is found anew, and the code is apart: both would
+// take registers from what runs every time.)
+template <int DK, bool OUT>
+__device__ __noinline__ void chunk_again(const LinArgs& a, const Table& tab, float* seg_state, double* seg_decay, float* mem) {
+    const int z = blockIdx.z, h = blockIdx.y, tid = threadIdx.x - 128;
+    int seq = 0;
+    while (tab.seg0[seq + 1] <= z) ++seq;
+    const int seg = z - tab.seg0[seq], nseg = tab.seg0[seq + 1] - tab.seg0[seq], first = seg * tab.step[seq];
+    const int count = min(tab.len[seq] - first, tab.step[seq]), slot = tab.slot[seq];
+    const long long row0 = static_cast<long long>(tab.start[seq]) + first;
+    const size_t head_state = static_cast<size_t>(a.dk) * a.dv;
+    const float* from = nullptr;
+    float* to = nullptr;
+    if (OUT && nseg > 1) from = seg_state + (static_cast<size_t>(first_state_of(tab, seq, seg)) * a.heads + h) * head_state;
+    else if (OUT && slot >= 0) from = a.state + (static_cast<size_t>(slot) * a.heads + h) * head_state;
+    if (!OUT) to = seg_state + (static_cast<size_t>(z) * a.heads + h) * head_state;
+    else if (seg == nseg - 1 && slot >= 0) to = a.state + (static_cast<size_t>(slot) * a.heads + h) * head_state;
+    static_assert(walk_floats<DK, 128, 2, true> * 4 <= Plan<DK>::kEnd, "shared memory");
+    const double total = walk<__nv_bfloat16, DK, 128, 2, OUT, true>(a, h, row0, count, blockIdx.x * 128, tid, from, to, mem,
+                                                                    [] { asm volatile("bar.sync 1, 256;" ::: "memory"); });
+    if (!OUT && tid == 0 && blockIdx.x == 0) seg_decay[static_cast<size_t>(z) * a.heads + h] = total;
+}
+
 template <int DK, bool OUT>
 __global__ void __launch_bounds__(kTcThreads, 1)
-k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__ Maps maps, int use_tma, int tma_out, float* seg_state,
+k_chunk_tc(const __grid_constant__ LinArgs a, const __grid_constant__ Table tab, const __grid_constant__ Maps maps, int use_tma, int tma_out, float* seg_state,
            double* seg_decay) {
     using L = Plan<DK>;
     using T = __nv_bfloat16;
@@ -333,6 +361,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         bar_init(&s.sc_full, 1); bar_init(&s.sc_free, 4);
         bar_init(&s.o_full, 1); bar_init(&s.o_free, 4);
         bar_init(&s.wk_free[0], 1); bar_init(&s.wk_free[1], 1); bar_init(&s.u_full, 1); bar_init(&s.u_free, 8); bar_init(&s.s_full, 8); bar_init(&s.qs_full, 1);
+        s.again = 0;
         s.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -523,7 +552,19 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         float* to = nullptr;
         if (!OUT) to = seg_state + (static_cast<size_t>(blockIdx.z) * a.heads + h) * head_state;
         else if (seg == nseg - 1 && slot >= 0) to = a.state + (static_cast<size_t>(slot) * a.heads + h) * head_state;
-        if (to && d < width) {
+        // Not finite, and a clear among the decays: all of it again at the end.  (The eight warps all come here,
+        // whatever they waited for in vain.)
+        float2 zero[4] = {};
+#pragma unroll
+        for (int i = 0; i < HC / 2; ++i) zero[i % 4] = __ffma2_rn(S[i], make_float2(0.0f, 0.0f), zero[i % 4]);   // NaN where one is not finite
+        const float2 all = __fadd2_rn(__fadd2_rn(zero[0], zero[1]), __fadd2_rn(zero[2], zero[3]));
+        if (all.x + all.y != 0.0f) atomicOr(&s.again, 1);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (s.again) {
+            chunk_scan(a, h, row0, count, &s.again);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
+        if (to && d < width && s.again != 3) {
             float* p = to + static_cast<size_t>(k0) * a.dv + c0 + d;
             int left = a.dk - k0;
 #pragma unroll
@@ -657,6 +698,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
         const T* K = static_cast<const T*>(a.k) + hk * a.k_head + row0 * a.k_row;
         const T* V = static_cast<const T*>(a.v) + h * a.v_head + c0 + row0 * a.v_row;
         double total = 0.0;
+        bool cleared = false;                      // (this lane's tokens)
         float2 g = make_float2(0.0f, 0.0f);
         if (warp == 18) g = chunk_decay_values(a, row0, min(kChunk, count), h, lane);
         Turn at;
@@ -690,6 +732,7 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
                 if (c + 1 < chunks)
                     ahead = chunk_decay_values(a, row0 + (c + 1LL) * kChunk, min(kChunk, count - (c + 1) * kChunk), h, lane);
                 const DecaySums d = chunk_decays(g, lane);
+                if (!OUT) cleared |= g.x == -INFINITY || g.y == -INFINITY;
                 total += d.total;
                 *reinterpret_cast<float4*>(&s.g[st][2 * lane]) = make_float4(d.hi[0], d.lo[0], d.hi[1], d.lo[1]);
                 *reinterpret_cast<float2*>(&s.eg[st][2 * lane]) = make_float2(d.grown[0] * a.scale, d.grown[1] * a.scale);
@@ -707,7 +750,10 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
             }
             if (!tma || warp == 19) warp_arrive(bar);
         }
-        if (!OUT && warp == 18 && lane == 0 && blockIdx.x == 0) seg_decay[static_cast<size_t>(blockIdx.z) * a.heads + h] = total;
+        if (!OUT && warp == 18) {
+            if (__any_sync(0xFFFFFFFFu, cleared)) total = -INFINITY;
+            if (lane == 0 && blockIdx.x == 0) seg_decay[static_cast<size_t>(blockIdx.z) * a.heads + h] = total;
+        }
     } else if (warp == 16) {
         // ---- matrix instructions of the state: update, carried (the warp as one, one lane issues) ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -800,6 +846,11 @@ k_chunk_tc(LinArgs a, const __grid_constant__ Table tab, const __grid_constant__
     __syncwarp();
     before_sync();
     __syncthreads();
+    if (s.again == 3) {                           // by the state's warps, whose registers are enough for it
+        if (warp >= 12 && warp < 16 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n\tfence.proxy.async;" ::: "memory");
+        __syncthreads();
+        if (warp >= 4 && warp < 12) chunk_again<DK, OUT>(a, tab, seg_state, seg_decay, reinterpret_cast<float*>(gen));
+    }
     if (warp == 18) {
         after_sync();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm));

@@ -262,7 +262,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     q, k: (rows, heads or a divisor of them, dk); v: (rows, heads, dv); any row
     and head strides, last dimension contiguous; float32, bfloat16 or float16.
     decay: float32 logarithms, at most 0, (heads,) or (rows, heads); -inf
-    clears the state.
+    clears the state, whatever it holds.
     Sequence i is rows offsets[i] : offsets[i + 1], or lengths[i] rows from
     offsets[i] (a padded batch); one sequence of all rows without offsets.
     state: (slots, heads, dk, dv) float32, contiguous: sequence i starts from
