@@ -7,7 +7,8 @@
 // the block is copied, its pointers are set, the output is allocated, and the
 // C entry (which checks the pointers) is called on torch's current stream.
 // Anything else -- no block under the key, something that is not a tensor, an
-// input that requires a gradient -- returns None, and ops.py takes the call.
+// input that requires a gradient or has a tangent -- returns None, and ops.py
+// takes the call.
 //
 // Host time of a call: a single-token step 5.1 us (10.8 through ctypes alone),
 // linear attention over five short prompts 6.6 us (15).
@@ -65,7 +66,7 @@ const at::Tensor* take(PyObject* o, Key& key, bool grad_mode, bool needed) {
         return nullptr;
     }
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (grad_mode && t.requires_grad()) key.ok = false;
+    if ((grad_mode && t.requires_grad()) || t._fw_grad(0).defined()) key.ok = false;
     key.put<int8_t>(static_cast<int8_t>(t.scalar_type()));
     key.put<int8_t>(static_cast<int8_t>(t.device().type()));
     key.put<int16_t>(t.device().index());

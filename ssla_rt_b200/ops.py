@@ -8,7 +8,8 @@ current stream of the tensors' device), is asynchronous, takes its workspace
 from torch's allocator, keeps nothing between calls, and can be captured into
 a CUDA graph.  With an explicit ``stream``, ordering against work on other
 streams is the caller's, as it is for the engine's drains.  Inference only:
-inputs that require a gradient are refused while gradients are enabled.
+inputs and given outputs that require a gradient are refused while gradients
+are enabled, those with a forward-mode tangent always.
 Wrong arguments raise ValueError (SslaError where the C entry finds them); there
 is no CPU fallback.
 """
@@ -20,6 +21,7 @@ from typing import Optional, Sequence, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import abi
 from .engine import _check, load_library
@@ -100,7 +102,12 @@ def _no_grad(*tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
-                raise ValueError("inference only: an input requires a gradient")
+                raise ValueError("inference only: an input or a given output requires a gradient")
+    level = forward_ad._current_level
+    if level >= 0:
+        for t in tensors:
+            if t is not None and torch._VF._unpack_dual(t, level=level)[1] is not None:
+                raise ValueError("inference only: an input or a given output has a forward-mode tangent")
 
 
 def _device(first: torch.Tensor, **others) -> int:
@@ -237,7 +244,7 @@ def _linattn_block(q, k, v, decay, state, scale, out, step_slots=None):
 
 def _linattn(q, k, v, decay, state, scale, out, slots=None):
     """The checked argument block of a call with every pointer but out's."""
-    _no_grad(q, k, v, decay, state)
+    _no_grad(q, k, v, decay, state, out)
     scale = _real("scale", scale)
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(),
            v.shape, v.stride(), v.dtype, v.get_device(), decay.shape, decay.stride(), decay.dtype, decay.get_device(),
@@ -519,7 +526,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         y = group_norm(x[:, None], groups, weight, bias, eps=eps, activation=activation,
                        out=None if out is None else out[:, None], stream=stream)
         return y[:, 0] if out is None else out
-    _no_grad(x, weight, bias)
+    _no_grad(x, weight, bias, out)
     groups, eps = _whole("groups", groups), _real("eps", eps)
     given = out
     key = ("norm", _sig(x), groups, _sig(weight), _sig(bias), eps, activation, _sig(out))
