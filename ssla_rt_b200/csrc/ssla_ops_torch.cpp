@@ -114,6 +114,10 @@ template <typename T> T* ptr(const at::Tensor* t) { return t ? static_cast<T*>(t
 void* current_stream(int device) {
     return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
 }
+// Tells autograd that a tensor was changed in place.
+void written(const at::Tensor* t) {
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 PyObject* give(PyObject* given, const at::Tensor& made) {
     if (given == Py_None) return THPVariable_Wrap(made);
     Py_INCREF(given);
@@ -217,6 +221,8 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
                      current_stream(b.device));
     }
     if (rc != SSLA_OK) return PyLong_FromLong(-rc);
+    written(t[4]);
+    written(t[5]);
     return give(a[6], made);
     SSLA_END
 }
@@ -248,6 +254,8 @@ PyObject* step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     b.out = t[6] ? t[6]->data_ptr() : made.data_ptr();
     const int rc = g_step(&b, ptr<int>(t[5]), current_stream(b.device));
     if (rc != SSLA_OK) return PyLong_FromLong(-rc);
+    written(t[4]);
+    written(t[6]);
     return give(a[7], made);
     SSLA_END
 }
@@ -266,7 +274,12 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
     SslaStateCache b;
     if (!find(key, b)) Py_RETURN_NONE;
     b.codes = ptr<void>(c); b.scales = ptr<float>(s); b.slots = ptr<int>(slots);
-    return PyLong_FromLong(-g_store(&b, x->data_ptr(), current_stream(b.device)));
+    const int rc = g_store(&b, x->data_ptr(), current_stream(b.device));
+    if (rc == SSLA_OK) {
+        written(c);
+        written(s);
+    }
+    return PyLong_FromLong(-rc);
     SSLA_END
 }
 
@@ -292,6 +305,7 @@ PyObject* load(PyObject*, PyObject* const* a, Py_ssize_t n) {
     b.codes = ptr<void>(c); b.scales = ptr<float>(s); b.slots = ptr<int>(slots);
     const int rc = g_load(&b, out ? out->data_ptr() : made.data_ptr(), current_stream(b.device));
     if (rc != SSLA_OK) return PyLong_FromLong(-rc);
+    written(out);
     return give(a[5], made);
     SSLA_END
 }
@@ -328,6 +342,7 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         rc = g_norm(&b, need ? ws.data_ptr() : nullptr, need, current_stream(b.device));
     }
     if (rc != SSLA_OK) return PyLong_FromLong(-rc);
+    written(out);
     return give(a[6], made);
     SSLA_END
 }

@@ -110,6 +110,13 @@ def _no_grad(*tensors) -> None:
                 raise ValueError("inference only: an input or a given output has a forward-mode tangent")
 
 
+def _written(*tensors) -> None:
+    """Tells autograd that these were changed in place, as torch's own operators do."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _device(first: torch.Tensor, **others) -> int:
     """The CUDA device index that every given tensor is on."""
     dev = first.device
@@ -320,6 +327,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     ws = _new(v, (need.value,), torch.uint8, ts) if need.value else None
     _check(lib.ssla_linattn_chunk(C.byref(a), po, pl, slots.ctypes.data if slots is not None else None, n_seq,
                                   ws.data_ptr() if ws is not None else None, need.value, handle))
+    _written(state, given)
     if ts is not None:
         _keep(ts, q, k, v, decay, state, out)
     return out
@@ -362,6 +370,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dec
         out = _like(v, ts)
     a.out = out.data_ptr()
     _check(load_library().ssla_linattn_step(C.byref(a), slots.data_ptr() if slots is not None else None, handle))
+    _written(state, given)
     if ts is not None:
         _keep(ts, q, k, v, decay, state, slots, out)
     return out
@@ -446,6 +455,7 @@ def state_store(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, b
         _keep_plan(_fast.store(x, codes, scales, block, slots, True), c)
     handle, ts = _stream_of(stream, c.device)
     _check(load_library().ssla_state_store(C.byref(c), x.data_ptr(), handle))
+    _written(codes, scales)
     if ts is not None:
         _keep(ts, x, codes, scales, slots)
 
@@ -455,6 +465,7 @@ def state_load(codes: torch.Tensor, scales: torch.Tensor, *, block: int = 64, sl
     """Reads states back from the 8-bit cache: (states, rows, cols), state i
     from slot slots[i] (every slot in order without); a slot outside the cache
     gives zeros."""
+    given = out
     code = _DTYPES.get(out.dtype if out is not None else dtype, -1)
     if _fast is not None and stream is None:
         r = _fast.load(codes, scales, block, slots, code, out, False)
@@ -471,6 +482,7 @@ def state_load(codes: torch.Tensor, scales: torch.Tensor, *, block: int = 64, sl
     if out is None:
         out = _new(codes, (n, c.rows, c.cols), dtype, ts)
     _check(load_library().ssla_state_load(C.byref(c), out.data_ptr(), handle))
+    _written(given)
     if ts is not None:
         _keep(ts, codes, scales, slots, out)
     return out
@@ -547,6 +559,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     _check(lib.ssla_group_norm_workspace(C.byref(a), C.byref(need)))
     ws = _new(x, (need.value,), torch.uint8, ts) if need.value else None
     _check(lib.ssla_group_norm(C.byref(a), ws.data_ptr() if ws is not None else None, need.value, handle))
+    _written(given)
     if ts is not None:
         _keep(ts, x, weight, bias, out)
     return out
