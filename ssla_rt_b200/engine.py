@@ -421,17 +421,26 @@ class SslaEngine:
             raise ValueError("a parking buffer is a contiguous CUDA tensor")
         return buf.numel() * buf.element_size()
 
+    def _parking(self, buf) -> int:
+        """Size of a parking buffer, which is on the engine's device."""
+        n = self._buffer_bytes(buf)
+        if buf.get_device() != self.device:
+            raise ValueError(f"the parking buffer is on device {buf.get_device()}, the engine on {self.device}")
+        return n
+
     def park(self, buf, partition: int = 0, fmt: int = abi.FMT_INT8, stream=None) -> None:
         """Writes a partition's state into ``buf`` (a CUDA tensor of
         park_bytes): hidden layers as abi.FMT_INT8 or abi.FMT_E4M3 with one
         scale per cell, everything else unchanged.  Asynchronous on
         ``stream``, like a drain."""
-        _check(self.lib.ssla_engine_park(self.h, partition, fmt, _ptr(buf), self._buffer_bytes(buf), _stream(stream)))
+        n = self._parking(buf)
+        _check(self.lib.ssla_engine_park(self.h, partition, fmt, _ptr(buf), n, _stream(stream)))
 
     def resume(self, buf, partition: int = 0, fmt: int = abi.FMT_INT8, stream=None) -> None:
-        """Puts a parked state back, into the same partition or another one.
-        Asynchronous on ``stream``."""
-        _check(self.lib.ssla_engine_resume(self.h, partition, fmt, _ptr(buf), self._buffer_bytes(buf), _stream(stream)))
+        """Puts a parked state back, into the same partition or another one;
+        ``fmt`` is the one it was parked in.  Asynchronous on ``stream``."""
+        n = self._parking(buf)
+        _check(self.lib.ssla_engine_resume(self.h, partition, fmt, _ptr(buf), n, _stream(stream)))
 
     def set_profiling(self, on: bool) -> None:
         _check(self.lib.ssla_engine_set_profiling(self.h, 1 if on else 0))
