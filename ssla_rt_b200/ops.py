@@ -98,6 +98,13 @@ def _plan(key, make):
     return p
 
 
+def _tensors(needed: dict, **optional) -> None:
+    for given, may_lack in ((needed, False), (optional, True)):
+        for name, t in given.items():
+            if not isinstance(t, torch.Tensor) and not (may_lack and t is None):
+                raise ValueError(f"{name} is {type(t).__name__}: a tensor is needed")
+
+
 def _no_grad(*tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -290,10 +297,13 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
         if r is not None:
             return _fast_result(r)
     given = out
+    _tensors({"q": q, "k": k, "v": v, "decay": decay}, state=state, out=out)
+    if v.dim() != 3:
+        raise ValueError(f"v has shape {tuple(v.shape)}: (rows, heads, width) is needed")
+    _counts("v", v)
     if offsets is None:
         if lengths is not None:
             raise ValueError("lengths without offsets")
-        _counts("v", v)
         off = np.array([0, v.shape[0]], dtype=np.int32)
         n_seq, gaps = 1, False
     else:
@@ -360,6 +370,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dec
     given = out
     if state is None:
         raise ValueError("state is needed")
+    _tensors({"q": q, "k": k, "v": v, "decay": decay, "state": state}, out=out)
     if slots is not None and not isinstance(slots, torch.Tensor):
         raise ValueError("slots is a one-dimensional int32 tensor")
     a = _linattn(q, k, v, decay, state, scale, out, slots)
@@ -438,7 +449,7 @@ def state_store(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, b
                 slots: Optional[torch.Tensor] = None, stream=None) -> None:
     """Quantises states into the 8-bit cache as they are written.
 
-    x: (states, rows, cols); codes: (slots, rows, cols) int8 or float8_e4m3fn;
+    x: (states, rows, cols), no two of them in one place; codes: (slots, rows, cols) int8 or float8_e4m3fn;
     scales: (slots, rows, ceil(cols / block)) float32.  State i goes to slot
     slots[i] (int32 CUDA tensor; slot i without).  Each ``block`` values of a
     row share scale = max|x| / 127 (int8) or / 448 (e4m3); a code is x / scale,
@@ -450,6 +461,9 @@ def state_store(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, b
         r = _fast.store(x, codes, scales, block, slots, False)
         if r is not None:
             return _check(-r)
+    _tensors({"x": x, "codes": codes, "scales": scales})
+    if x.dim() == 0:
+        raise ValueError("x has no dimensions: (states, rows, cols) is needed")
     c = _cache(codes, scales, block, slots, x.shape[0], "x", x, x.dtype)
     if _fast is not None:
         _keep_plan(_fast.store(x, codes, scales, block, slots, True), c)
@@ -466,11 +480,16 @@ def state_load(codes: torch.Tensor, scales: torch.Tensor, *, block: int = 64, sl
     from slot slots[i] (every slot in order without); a slot outside the cache
     gives zeros."""
     given = out
+    _tensors({"codes": codes, "scales": scales}, out=out)
+    if not all(t.dim() for t in (codes, slots, out) if isinstance(t, torch.Tensor)):
+        raise ValueError("codes, slots and out have at least one dimension")
     code = _DTYPES.get(out.dtype if out is not None else dtype, -1)
     if _fast is not None and stream is None:
         r = _fast.load(codes, scales, block, slots, code, out, False)
         if r is not None:
             return _fast_result(r)
+    if slots is not None and not isinstance(slots, torch.Tensor):
+        raise ValueError("slots is a one-dimensional int32 tensor")
     if out is not None:
         n, dtype = out.shape[0], out.dtype
     else:
@@ -501,11 +520,11 @@ def _norm_block(x, groups, weight, bias, eps, activation, out):
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (channels,) or not t.is_contiguous()):
             raise ValueError(f"{name} is {t.dtype} {tuple(t.shape)}: contiguous float32 ({channels},) is needed")
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
+        raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, x {x.dtype} {tuple(x.shape)}")
     for name, t in (("x", x), ("out", out)):
         if t is not None and channels > 1 and t.stride(2) != 1:
             raise ValueError(f"{name}'s channels are not contiguous")
-    if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
-        raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, x {x.dtype} {tuple(x.shape)}")
     a = abi.SslaGroupNorm()
     a.device = _device(x, weight=weight, bias=bias, out=out)
     a.x_sample, a.x_pos, _ = x.stride()
@@ -534,7 +553,10 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         r = _fast.norm(x, groups, weight, bias, eps, act, out, False)
         if r is not None:
             return _fast_result(r)
+    _tensors({"x": x}, weight=weight, bias=bias, out=out)
     if x.dim() == 2:
+        if out is not None and out.shape != x.shape:
+            raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, x {x.dtype} {tuple(x.shape)}")
         y = group_norm(x[:, None], groups, weight, bias, eps=eps, activation=activation,
                        out=None if out is None else out[:, None], stream=stream)
         return y[:, 0] if out is None else out
