@@ -61,7 +61,8 @@ typedef struct SslaLinAttn {
  * and so is the state of a sequence of length 0.  state may be NULL if every
  * slot is -1.  A token's non-finite value makes the outputs of its own and
  * later tokens non-finite where they depend on it, never earlier ones.
- * `workspace`: ssla_linattn_chunk_workspace bytes, 16-byte aligned. */
+ * `workspace`: ssla_linattn_chunk_workspace bytes, 16-byte aligned, apart from
+ * the tensors. */
 int ssla_linattn_chunk(const SslaLinAttn* a, const int* offsets, const int* lengths, const int* slots, int n_seq,
                        void* workspace, size_t workspace_bytes, void* stream);
 int ssla_linattn_chunk_workspace(const SslaLinAttn* a, const int* offsets, const int* lengths, int n_seq,
@@ -76,7 +77,8 @@ int ssla_linattn_status(int device, unsigned* status);
 /* Recurrent form: one token per row, at most 65535 rows.  Row r updates state slot slots[r]
  * (device array; NULL: slot r, n_rows <= n_slots).  Rows that name the same
  * slot are applied in row order.  A slot outside [0, n_slots) marks a padding
- * row: its output is zero and no state is touched. */
+ * row: its output is zero and no state is touched.  slots overlaps neither
+ * `out` nor `state`. */
 int ssla_linattn_step(const SslaLinAttn* a, const int* slots, void* stream);
 
 /* 8-bit cache of recurrent states.  A state is `rows` rows of `cols` values;
@@ -115,7 +117,8 @@ int ssla_state_load(const SslaStateCache* c, void* x, void* stream);
  * weight and bias: [channels] 32-bit, each may be NULL.  y may be x itself.
  * At most 2^24 channels, 2^40 values a sample, 2^31 - 2^16 positions and as
  * many slabs (samples x groups).
- * `workspace`: ssla_group_norm_workspace bytes, 16-byte aligned. */
+ * `workspace`: ssla_group_norm_workspace bytes, 16-byte aligned, apart from
+ * the tensors. */
 typedef struct SslaGroupNorm {
     const void* x;
     void* y;

@@ -666,6 +666,12 @@ int ssla_group_norm(const SslaGroupNorm* a, void* workspace, size_t workspace_by
     const size_t need = gn_bytes(a);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
         return fail(SSLA_ERR_ARG, "group norm: workspace of %zu bytes, %zu needed, 16-byte aligned", workspace_bytes, need);
+    auto meets = [&](const void* p, long long s, long long q, int sz) {
+        return p && overlaps(workspace, need, p, static_cast<size_t>((a->n - 1) * s + (a->positions - 1) * q + a->channels) * sz);
+    };
+    if (need && (meets(a->x, a->x_sample, a->x_pos, dtype_size(a->dtype)) || meets(a->y, a->y_sample, a->y_pos, dtype_size(a->dtype)) ||
+                 meets(a->weight, 0, 0, 4) || meets(a->bias, 0, 0, 4)))
+        return fail(SSLA_ERR_ARG, "group norm: the workspace overlaps a tensor");
     int lps, ept;
     if (a->n > 65535 && !gn_small(a, gn_vec(a), &lps, &ept)) {
         // more samples than a grid's depth: in parts, one after the other on the stream

@@ -236,6 +236,19 @@ int check_args(const SslaLinAttn* a, const char* who, bool need_state) {
     return SSLA_OK;
 }
 
+// Whether [p, p + n) meets a tensor of the (checked) call; `written` ones only, or all.
+bool meets(const SslaLinAttn* a, const void* p, size_t n, bool written) {
+    const int sz = dtype_size(a->dtype);
+    auto in = [&](const Span& s) { return overlaps(p, n, s.p, s.n); };
+    if (in(span_of(a->out, a->out_row, a->out_head, a->n_rows, a->heads, a->dv, sz)) ||
+        in({a->state, static_cast<size_t>(a->state ? a->n_slots : 0) * a->heads * a->dk * a->dv * 4}))
+        return true;
+    return !written && (in(span_of(a->q, a->q_row, a->q_head, a->n_rows, a->q_heads, a->dk, sz)) ||
+                        in(span_of(a->k, a->k_row, a->k_head, a->n_rows, a->k_heads, a->dk, sz)) ||
+                        in(span_of(a->v, a->v_row, a->v_head, a->n_rows, a->heads, a->dv, sz)) ||
+                        in(span_of(a->decay, a->decay_row, a->decay_head, a->n_rows, a->heads, 1, 4)));
+}
+
 LinArgs device_args(const SslaLinAttn* a) {
     LinArgs d;
     d.q = a->q; d.k = a->k; d.v = a->v; d.out = a->out; d.decay = a->decay; d.state = a->state;
@@ -306,6 +319,7 @@ int ssla_linattn_step(const SslaLinAttn* a, const int* slots, void* stream) {
         return fail(SSLA_ERR_ARG, "%s: %d rows for %d slots", who, a->n_rows, a->n_slots);
     if (!aligned(slots, 4)) return fail(SSLA_ERR_ARG, "%s: slots are not aligned", who);
     if (a->n_rows == 0) return SSLA_OK;
+    if (slots && meets(a, slots, 4ull * a->n_rows, true)) return fail(SSLA_ERR_ARG, "%s: out or state overlaps slots", who);
     OnDevice dev(a->device);
     if (dev.err != SSLA_OK) return dev.err;
     const LinArgs d = device_args(a);
@@ -343,6 +357,7 @@ int ssla_linattn_chunk(const SslaLinAttn* a, const int* offsets, const int* leng
         const size_t need = chunk_workspace(d, a->dtype, seqs);
         if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
             return fail(SSLA_ERR_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who, workspace_bytes, need);
+        if (need && meets(a, workspace, need, false)) return fail(SSLA_ERR_ARG, "%s: the workspace overlaps a tensor", who);
         OnDevice dev(a->device);
         if (dev.err != SSLA_OK) return dev.err;
         return chunk_launch(d, a->dtype, seqs, workspace, static_cast<cudaStream_t>(stream));
