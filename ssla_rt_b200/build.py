@@ -64,14 +64,33 @@ def build_consumer(force: bool = False, verbose: bool = False) -> str:
 
 
 # The repeated calls of ops.py in one step: a Python extension module over
-# torch's tensors (the library itself stays free of torch).
+# torch's tensors (the library itself stays free of torch).  It fits the torch
+# and Python that it was built with; the stamp beside it names them.
 OPS_TORCH_SRC = os.path.join(CSRC, "ssla_ops_torch.cpp")
 OPS_TORCH = os.path.join(HERE, "_ops_torch.so")
+OPS_TORCH_STAMP = os.path.join(HERE, "_build", "ops_torch.stamp")
+
+
+def ops_torch_abi() -> str:
+    import sysconfig
+
+    import torch
+    return f"torch {torch.__version__} python {sysconfig.get_config_var('SOABI')}"
+
+
+def _read(path: str) -> str:
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return ""
 
 
 def build_ops_torch(force: bool = False, verbose: bool = False) -> str:
+    abi = ops_torch_abi()
     deps = [OPS_TORCH_SRC] + [os.path.join(REPO, "include", f) for f in ("ssla_b200.h", "ssla_ops.h")]
-    if not force and os.path.exists(OPS_TORCH) and os.path.getmtime(OPS_TORCH) >= max(map(os.path.getmtime, deps)):
+    if (not force and os.path.exists(OPS_TORCH) and os.path.getmtime(OPS_TORCH) >= max(map(os.path.getmtime, deps)) and
+            _read(OPS_TORCH_STAMP) == abi):
         return OPS_TORCH
     import sysconfig
 
@@ -85,13 +104,29 @@ def build_ops_torch(force: bool = False, verbose: bool = False) -> str:
            "-ltorch_python"]
     if verbose:
         print(" ".join(cmd), flush=True)
+    # a module of another torch would take the process down when it is imported: it goes first
+    if os.path.exists(OPS_TORCH):
+        os.remove(OPS_TORCH)
     subprocess.run(cmd, check=True)
+    os.makedirs(os.path.dirname(OPS_TORCH_STAMP), exist_ok=True)
+    with open(OPS_TORCH_STAMP, "w") as f:
+        f.write(abi)
     return OPS_TORCH
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """The library and the consumer module; then the extension module, which
+    may fail (no torch, or one without CUDA): ops.py does without it."""
     build_consumer(force=force, verbose=verbose)
-    build_ops_torch(force=force, verbose=verbose)
+    lib = build_library(force=force, verbose=verbose)
+    try:
+        build_ops_torch(force=force, verbose=verbose)
+    except (ImportError, OSError, subprocess.CalledProcessError) as e:
+        print(f"ssla_rt_b200: repeated operator calls go without their extension module: {e}", file=sys.stderr)
+    return lib
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
         return LIB
     cmd = [_nvcc(), *NVCC_FLAGS, f"-I{os.path.join(REPO, 'include')}", f"-I{CSRC}",
