@@ -47,6 +47,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 #include "ssla_linattn.cuh"
 
@@ -708,6 +709,7 @@ struct Shape {
     int dk, dv, ctas;               // tile and resident CTAs per SM
     bool tc;                        // the tcgen05 form
     int cost;                       // a divided sequence's time over a whole one's, percent
+    double setup, launches;         // in chunks' times: a segment's set-up and state traffic; the two further launches
 };
 
 template <typename F> auto with_shape(int dtype, int dk, int dv, F&& f) {
@@ -736,18 +738,25 @@ int wide_inputs(const LinArgs& a, int dtype) {
 Shape shape_of(const LinArgs& a, int dtype) {
     // bf16 with wide heads: the tcgen05 form, whose copies are 16 bytes wide
     if (dtype == SSLA_DT_BF16 && a.dk > 32 && a.dv > 32 && wide_inputs(a, dtype) == 7)
-        return Shape{a.dk <= 64 ? 64 : 128, 128, 1, true, 155};
+        return Shape{a.dk <= 64 ? 64 : 128, 128, 1, true, 160, 3.5, 12.0};
     return with_shape(dtype, a.dk, a.dv, [](auto t, auto k, auto v) {
         constexpr int K = decltype(k)::value, V = decltype(v)::value;
         const int bytes = Tile<decltype(t), K, V>::bytes;
-        return Shape{K, V, std::max(1, std::min(K * V >= 128 * 64 ? 2 : 4, (227 * 1024) / (bytes + 1024))), false, 145};
+        return Shape{K, V, std::max(1, std::min(K * V >= 128 * 64 ? 2 : 4, (227 * 1024) / (bytes + 1024))), false, 145, 0.0, 0.0};
     });
 }
 
 // Tokens of a segment for sequences [i0, i1).  Undivided, the longest sequence
 // bounds the time; divided, all resident CTAs share the work, but keys and
-// values pass twice (`cost`) and a last round of CTAs is half empty.  A group's
-// segments are a grid's depth: at most 65535.
+// values pass twice (`cost`), every segment is set up and its state goes
+// through memory (`setup`: the tcgen05 form's tensor memory, barriers and first
+// copies), two more launches follow one another (nothing of both to speak of in
+// the other form), and a last round of CTAs is half empty.  Measured,
+// microseconds undivided / in segments of 32 chunks / of 5: prompts of 4,096 to
+// 511 tokens, 16 heads of 128 (bf16): 169 / 174 / 240; two of 8,192: 293 / 160 /
+// 218; one of 65,537, 4 heads of 64: 1,729 / 118 / 200; eight of 25,000, 4 heads of
+// 24, fp32: 2,302 / 400 / 388, and 352 in segments of 22.  A group's segments are
+// a grid's depth: at most 65535.
 int segment_tokens(const LinArgs& a, const Shape& sh, const std::vector<Seq>& seqs, size_t i0, size_t i1) {
     const long long per = static_cast<long long>(a.heads) * ((a.dv + sh.dv - 1) / sh.dv), slots = 148LL * sh.ctas;
     long long longest = 0, all = 0;
@@ -756,15 +765,19 @@ int segment_tokens(const LinArgs& a, const Shape& sh, const std::vector<Seq>& se
         longest = std::max(longest, n);
         all += n;
     }
-    const long long share = (all * per + slots - 1) / slots;
-    long long best = longest, best_time = std::max(longest, share) * 100;
+    auto time_of = [&](long long step, long long segs) {
+        const double share = std::ceil((all + segs * sh.setup) * per / slots);
+        return std::max(step + sh.setup, share);
+    };
+    long long best = longest;
+    double best_time = time_of(longest, static_cast<long long>(i1 - i0)) * 100;
     for (int parts = 2; parts <= 512; parts += parts < 32 ? 1 : parts / 16) {
         const long long step = (longest + parts - 1) / parts;
         if (step < 4) break;
         long long segs = 0;
         for (size_t i = i0; i < i1; ++i) segs += ((seqs[i].len + kChunk - 1LL) / kChunk + step - 1) / step;
         if (segs > 65535) break;                            // (the steps only get smaller)
-        const long long ctas = segs * per, time = (std::max(step, share) + (ctas > slots ? step / 2 : 0)) * sh.cost;
+        const double time = (time_of(step, segs) + (segs * per > slots ? step / 2 : 0)) * sh.cost + 100 * sh.launches;
         if (time < best_time) best = step, best_time = time;
     }
     return static_cast<int>(best == longest ? INT_MAX / 2 / kChunk * kChunk : best * kChunk);

@@ -37,3 +37,11 @@ def test_ordinary_calls_are_divided_as_before():
     assert segments(8, 25000, heads=4) == 144
     assert segments(1, 65537, heads=4, dk=64, dv=64, dtype=abi.DT_BF16) == 36
     assert segments(8, 2048, heads=16, dk=128, dv=128, dtype=abi.DT_BF16) == 0
+
+
+def test_segments_pay_for_their_setup():
+    """Enough CTAs without a division, if not evenly loaded: none in the tcgen05 form."""
+    assert segments(8, 4096, heads=16, dk=128, dv=128, dtype=abi.DT_BF16) == 0
+    assert segments(4, 4096, heads=16, dk=128, dv=128, dtype=abi.DT_BF16) == 0
+    assert segments(2, 8192, heads=16, dk=128, dv=128, dtype=abi.DT_BF16) == 8
+    assert segments(8, 8192, heads=4, dk=64, dv=64, dtype=abi.DT_BF16) == 32
