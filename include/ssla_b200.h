@@ -390,10 +390,11 @@ void* ssla_engine_state_ptr(SslaEngine* eng, int kind, int partition, int index)
 int  ssla_engine_info(SslaEngine* eng, SslaEngineInfo* info);
 
 /* Parks a partition's whole state in a device buffer of
- * ssla_engine_park_bytes (16-byte aligned), a third or less of its size, and
+ * ssla_engine_park_bytes (16-byte aligned), about a third of its size, and
  * resumes it, into the same partition or another one (of an engine of the
  * same model and layout).  Hidden states are held in 8 bits, `format` an
- * SSLA_FMT_* of ssla_ops.h, with one scale per cell (ssla_state_store); gate
+ * SSLA_FMT_* of ssla_ops.h (resumed in the one it was parked in), with one
+ * scale per cell (ssla_state_store); gate
  * counters, timestamps, predictions and versions unchanged, so that the gates
  * go on exactly.  Asynchronous on `stream`, ordered with drains on the same
  * stream; not while a live loop runs on the partition.  No reference

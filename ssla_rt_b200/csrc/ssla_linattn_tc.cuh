@@ -25,14 +25,16 @@
 //                  decay sums
 //     warps 16, 17 issue the matrix instructions: update and carried; scores and
 //                  inner
-// Measured: 4,096-token prompts of 16 heads of 128 take 220 us on 128 SMs, 3.4 us
-// a chunk, where the chunk's products take 1,680 cycles of about 4,400; what
-// bounds it is the roles' arithmetic (2,400 issue slots a chunk in each
-// quarter of the SM) and the chain update -> state -> next wK -> update.
+// Measured: eight prompts of up to 4,096 tokens, 16 heads of 128, take 166 us on
+// 128 SMs (one CTA for each prompt and head), 2.6 us a chunk of the longest,
+// where the chunk's products take 1,680 cycles of about 4,900; what bounds it is
+// the roles' arithmetic (2,400 issue slots a chunk in each quarter of the SM)
+// and the chain update -> state -> next wK -> update.
 // Hence the division of labour below, loops that keep the roles' code in the
 // instruction cache, and the state's pieces in tensor memory, where they cost
 // no shared memory bandwidth.
-// They meet at mbarriers only.  Every wait is bounded: one that runs out sets
+// They meet at mbarriers only (and the state's warps, when all eight are done, at
+// a named barrier).  Every wait is bounded: one that runs out sets
 // the abort flag and a bit of the device's status word, all roles leave, and
 // the tensor memory is freed.
 #pragma once
