@@ -479,17 +479,17 @@ def state_load(codes: torch.Tensor, scales: torch.Tensor, *, block: int = 64, sl
     """Reads states back from the 8-bit cache: (states, rows, cols), state i
     from slot slots[i] (every slot in order without); a slot outside the cache
     gives zeros."""
-    given = out
-    _tensors({"codes": codes, "scales": scales}, out=out)
-    if not all(t.dim() for t in (codes, slots, out) if isinstance(t, torch.Tensor)):
-        raise ValueError("codes, slots and out have at least one dimension")
-    code = _DTYPES.get(out.dtype if out is not None else dtype, -1)
+    code = _DTYPES.get(dtype if out is None else getattr(out, "dtype", None), -1)
     if _fast is not None and stream is None:
         r = _fast.load(codes, scales, block, slots, code, out, False)
         if r is not None:
             return _fast_result(r)
+    given = out
+    _tensors({"codes": codes, "scales": scales}, out=out)
     if slots is not None and not isinstance(slots, torch.Tensor):
         raise ValueError("slots is a one-dimensional int32 tensor")
+    if not all(t.dim() for t in (codes, slots, out) if t is not None):
+        raise ValueError("codes, slots and out have at least one dimension")
     if out is not None:
         n, dtype = out.shape[0], out.dtype
     else:
